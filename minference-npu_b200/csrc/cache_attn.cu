@@ -1,0 +1,575 @@
+// Attention over a shared prefix and per-sequence caches: the kernel for few
+// query rows, the kernel that joins partial results, and the C entry point.
+// The split of the work is described at the top of cache_attn.cuh.
+#include "cache_attn.cuh"
+#include "host_util.h"
+#include "mma_sync.cuh"
+
+namespace mib200 {
+
+// ---------------------------------------------------------------------------
+// Few rows (1 to 32 per key/value head): a work item is one tile of 16*MT
+// rows against `chunk` keys.  Its four warps take groups of 16 keys in turn;
+// each warp streams its own groups through its own shared-memory ring
+// (cp.async) and keeps its own running maximum, sum and O, so there is no
+// barrier in the loop.  The four states are joined at the end.
+//   S (16 rows x 16 keys) = Q K^T     Q fragments stay in registers
+//   O (16 rows x D) += P V            P is S's registers, rounded to the
+//                                     inputs' type for the tensor core
+// Rows of a ring stage are padded by 16 bytes, which makes the ldmatrix rows
+// of 128, 192 and 256 bytes fall into distinct banks.  Keys past the end of
+// the range are filled with zeros instead of being read, so whatever a cache
+// holds past its length cannot reach O through 0 * V.
+// ---------------------------------------------------------------------------
+constexpr int kRowsWarps = 4;
+
+template <int DK, bool STATS>
+struct RowsSmem {
+  static constexpr int kPitch = DK * 2 + 16;
+  static constexpr int kTile = 16 * kPitch;                   // 16 keys of K or V
+  static constexpr int kStage = (STATS ? 1 : 2) * kTile;      // one warp's stage
+  static constexpr int ST = DK == 64 ? 5 : (DK == 96 ? 4 : 3);  // ~100 KB a block: two per SM
+  static constexpr int kWarpRing = ST * kStage;
+  static constexpr int kRing = kRowsWarps * kWarpRing;
+};
+
+template <typename DT, int DK, int MT, bool STATS>
+__global__ void __launch_bounds__(32 * kRowsWarps, 2)
+    cache_rows_kernel(const __grid_constant__ CacheParams p) {
+  using L = RowsSmem<DK, STATS>;
+  constexpr int KS = DK / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float sm_m[kRowsWarps][16 * MT], sm_l[kRowsWarps][16 * MT];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch();
+
+  long long it = blockIdx.x;
+  const bool own = it >= p.items0;
+  if (own) it -= p.items0;
+  const CacheSeg& sg = p.seg[own ? 1 : 0];
+  const int rt = (int)(it % sg.rtiles);
+  it /= sg.rtiles;
+  const int sp = (int)(it % sg.nsplit);
+  it /= sg.nsplit;
+  const int h = (int)(it % p.Hkv);
+  const int e = (int)(it / p.Hkv);
+  const int r0 = rt * 16 * MT;
+  const int nrows = min(16 * MT, sg.rows - r0);
+  const int len = cache_len(sg, e);
+  // Keys that the tile's last token sees (its rows cover tokens in order
+  // unless they wrap into another head).
+  int end = len;
+  if (sg.causal) {
+    const int last = r0 + nrows - 1;
+    const int smax = (r0 / p.Sq != last / p.Sq) ? p.Sq - 1 : last % p.Sq;
+    end = max(0, len - (p.Sq - 1 - smax));
+  }
+  const int kb = sp * sg.chunk;
+  const int ke = min(end, (int)min((long long)kb + sg.chunk, (long long)end));
+  const int ngroups = ke > kb ? (ke - kb + 15) >> 4 : 0;
+
+  // ---- Q tile -> shared (ring area) -> fragments ----------------------------
+  constexpr int CPR = DK / 8;
+  for (int i = tid; i < 16 * MT * CPR; i += 32 * kRowsWarps) {
+    const int r = i / CPR, c = i - r * CPR;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < nrows && c * 8 < p.D) {
+      int b, hd, tk;
+      cache_row(p, sg, e, h, r0 + r, b, hd, tk);
+      x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b + hd * p.qs_h + tk * p.qs_s + c * 8);
+    }
+    *reinterpret_cast<uint4*>(smem + r * L::kPitch + c * 16) = x;
+  }
+  __syncthreads();
+  uint32_t qf[MT][KS][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      ldsm4(qf[i][ks], smem_u32(smem) + (i * 16 + (lane & 15)) * L::kPitch + ks * 32 +
+                           (lane >> 4) * 16);
+  __syncthreads();  // the ring reuses the Q area
+
+  // ---- per-thread rows: lane/4 and lane/4 + 8 of every 16-row tile ----------
+  int lim[MT][2];  // keys that the row sees
+  int minlim = ke;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = i * 16 + (lane >> 2) + 8 * j;
+      lim[i][j] = 0;
+      if (r < nrows) lim[i][j] = sg.causal ? len - (p.Sq - 1 - (r0 + r) % p.Sq) : len;
+      if (r < nrows) minlim = min(minlim, lim[i][j]);
+    }
+  minlim = __reduce_min_sync(0xffffffffu, minlim);
+
+  // ---- loader: lane l brings 16-byte pieces (l&3) + 4v of rows l/4 and l/4+8 -
+  const uint32_t ring = smem_u32(smem) + warp * L::kWarpRing;
+  const int lrow = lane >> 2, lcol = lane & 3;
+  const uint32_t ldst = ring + lrow * L::kPitch + lcol * 16;
+  const uint16_t* kbase = sg.k + e * sg.ks_b + h * sg.ks_h + lcol * 8;
+  const uint16_t* vbase = STATS ? nullptr : sg.v + e * sg.vs_b + h * sg.vs_h + lcol * 8;
+  auto load = [&](int g) {
+    if (g < ngroups) {
+      const uint32_t st = ldst + ((g / kRowsWarps) % L::ST) * L::kStage;
+      const int key = kb + g * 16 + lrow;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool in = key + 8 * u < ke;
+        const long long kk = in ? key + 8 * u : 0;
+        const uint16_t* kr = kbase + kk * sg.ks_s;
+        const uint16_t* vr = STATS ? nullptr : vbase + kk * sg.vs_s;
+#pragma unroll
+        for (int v = 0; v < CPR / 4; ++v) {
+          const bool ok = in && (lcol + 4 * v) * 8 < p.D;
+          cp16(st + u * 8 * L::kPitch + v * 64, ok ? kr + v * 32 : kbase, ok);
+          if constexpr (!STATS)
+            cp16(st + L::kTile + u * 8 * L::kPitch + v * 64, ok ? vr + v * 32 : vbase, ok);
+        }
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < L::ST - 1; ++s) load(warp + s * kRowsWarps);
+
+  float m[MT][2], l[MT][2];
+  float o[MT][STATS ? 1 : DK / 8][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    m[i][0] = m[i][1] = -INFINITY;
+    l[i][0] = l[i][1] = 0.f;
+    if constexpr (!STATS)
+#pragma unroll
+      for (int d = 0; d < DK / 8; ++d) o[i][d][0] = o[i][d][1] = o[i][d][2] = o[i][d][3] = 0.f;
+  }
+
+  for (int g = warp; g < ngroups; g += kRowsWarps) {
+    load(g + (L::ST - 1) * kRowsWarps);
+    cp_wait<L::ST - 1>();
+    __syncwarp();
+    const uint32_t st = ring + ((g / kRowsWarps) % L::ST) * L::kStage;
+    float s[MT][2][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
+    // K: keys 0-7 / 8-15 (second pair of matrices) x dims 0-7 / 8-15 of the step
+    const uint32_t ka =
+        st + ((lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t b[4];
+      ldsm4(b, ka + ks * 32);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        mma16816<DT>(s[i][0], qf[i][ks], b[0], b[1]);
+        mma16816<DT>(s[i][1], qf[i][ks], b[2], b[3]);
+      }
+    }
+    const int key0 = kb + g * 16;
+    const bool full = key0 + 16 <= minlim;
+    uint32_t pa[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[i][n][c] *= p.scale_log2;
+      if (!full) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = key0 + n * 8 + (lane & 3) * 2 + (c & 1);
+            if (key >= min(lim[i][c >> 1], ke)) s[i][n][c] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float t = fmaxf(fmaxf(s[i][0][2 * j], s[i][0][2 * j + 1]),
+                        fmaxf(s[i][1][2 * j], s[i][1][2 * j + 1]));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        const float mn = fmaxf(m[i][j], t);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float f = fast_exp2(m[i][j] - base);
+        m[i][j] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float x0 = fast_exp2(s[i][n][2 * j] - base);
+          const float x1 = fast_exp2(s[i][n][2 * j + 1] - base);
+          sum += x0 + x1;
+          pa[i][n * 2 + j] = DType<DT>::pack2(x0, x1);
+        }
+        l[i][j] = l[i][j] * f + sum;
+        if constexpr (!STATS) {
+          if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < DK / 8; ++d) {
+              o[i][d][2 * j] *= f;
+              o[i][d][2 * j + 1] *= f;
+            }
+          }
+        }
+      }
+    }
+    if constexpr (!STATS) {
+      // V (transposed by the load): keys 0-7 / 8-15 x dims 0-7 / 8-15
+      const uint32_t va = st + L::kTile + (lane & 15) * L::kPitch + (lane >> 4) * 16;
+#pragma unroll
+      for (int d = 0; d < DK / 16; ++d) {
+        uint32_t b[4];
+        ldsm4_t(b, va + d * 32);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma16816<DT>(o[i][2 * d], pa[i], b[0], b[1]);
+          mma16816<DT>(o[i][2 * d + 1], pa[i], b[2], b[3]);
+        }
+      }
+    }
+    __syncwarp();  // the stage is free for the load of the next step
+  }
+  cp_wait<0>();
+  __syncthreads();
+
+  // ---- join the four warps ---------------------------------------------------
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 1);
+      l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 2);
+      const int r = i * 16 + (lane >> 2) + 8 * j;
+      if ((lane & 3) == 0) {
+        sm_m[warp][r] = m[i][j];
+        sm_l[warp][r] = l[i][j];
+      }
+      if constexpr (!STATS) {
+        float* row = reinterpret_cast<float*>(smem) + (warp * 16 * MT + r) * (DK + 4);
+#pragma unroll
+        for (int d = 0; d < DK / 8; ++d)
+          *reinterpret_cast<float2*>(row + d * 8 + (lane & 3) * 2) =
+              make_float2(o[i][d][2 * j], o[i][d][2 * j + 1]);
+      }
+    }
+  __syncthreads();
+  const int D4 = p.D >> 2;
+  const bool direct = !STATS && p.NS == 1;
+  for (int i = tid; i < nrows * D4; i += 32 * kRowsWarps) {
+    const int r = i / D4, c = i - r * D4;
+    float M = sm_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kRowsWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float lt = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) {
+      const float f = fast_exp2(sm_m[w][r] - base);
+      lt += f * sm_l[w][r];
+      if constexpr (!STATS) {
+        const float4 x = *reinterpret_cast<const float4*>(
+            reinterpret_cast<float*>(smem) + (w * 16 * MT + r) * (DK + 4) + c * 4);
+        acc.x += f * x.x;
+        acc.y += f * x.y;
+        acc.z += f * x.z;
+        acc.w += f * x.w;
+      }
+    }
+    if (STATS && c) continue;
+    int b, hd, tk;
+    cache_row(p, sg, e, h, r0 + r, b, hd, tk);
+    const long long row = ((long long)b * p.Hq + hd) * p.Sq + tk;
+    if (direct) {
+      const float inv = lt > 0.f ? 1.f / lt : 0.f;
+      const uint2 x = make_uint2(DType<DT>::pack2(acc.x * inv, acc.y * inv),
+                                 DType<DT>::pack2(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s + c * 4) =
+          M == -INFINITY ? make_uint2(0, 0) : x;
+      if (c == 0 && p.lse)
+        p.lse[row] = M == -INFINITY ? M : (M + log2f(lt)) * 0.69314718055994531f;
+    } else {
+      const long long at = row * p.NS + sg.slot0 + sp;
+      if (!STATS && M != -INFINITY) *reinterpret_cast<float4*>(p.opart + at * p.D + c * 4) = acc;
+      if (c == 0) p.ml[at] = make_float2(M, lt);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the partial results of a row: one warp per row, a lane per 4 dims.
+// Slots without a visible key have m = -inf and are not read.
+// ---------------------------------------------------------------------------
+template <typename DT>
+__global__ void __launch_bounds__(128) cache_combine_kernel(const __grid_constant__ CacheParams p,
+                                                            long long nrows) {
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_wait();
+  if (row >= nrows) return;
+  const float2* ml = p.ml + row * p.NS;
+  float M = -INFINITY;
+  for (int i = lane; i < p.NS; i += 32) M = fmaxf(M, ml[i].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float base = M == -INFINITY ? 0.f : M;
+  float lt = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool act = lane * 4 < p.D;
+  const float* op = p.opart + row * p.NS * p.D + lane * 4;
+  for (int s0 = 0; s0 < p.NS; s0 += 32) {
+    const float2 x = s0 + lane < p.NS ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+    const float f = fast_exp2(x.x - base);
+    lt += f * x.y;
+    const int n = min(32, p.NS - s0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if (fi != 0.f && act) {
+        const float4 v = *reinterpret_cast<const float4*>(op + (long long)(s0 + i) * p.D);
+        acc.x += fi * v.x;
+        acc.y += fi * v.y;
+        acc.z += fi * v.z;
+        acc.w += fi * v.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+  const float inv = lt > 0.f ? 1.f / lt : 0.f;
+  const int tk = (int)(row % p.Sq);
+  const long long bh = row / p.Sq;
+  const int hd = (int)(bh % p.Hq);
+  const long long b = bh / p.Hq;
+  if (act)
+    *reinterpret_cast<uint2*>(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s + lane * 4) =
+        M == -INFINITY ? make_uint2(0, 0)
+                       : make_uint2(DType<DT>::pack2(acc.x * inv, acc.y * inv),
+                                    DType<DT>::pack2(acc.z * inv, acc.w * inv));
+  if (lane == 0 && p.lse)
+    p.lse[row] = M == -INFINITY ? M : (M + log2f(lt)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------------------
+// Host: the split, checks and launches
+// ---------------------------------------------------------------------------
+struct CachePlan {
+  int mt;                  // 16-row tiles per item
+  int rtiles[2], nsplit[2], chunk[2];
+  int NS;
+};
+
+// Cuts both segments into ranges of one length, so that about six items per
+// SM exist (two run at a time; the rest evens out ragged lengths) but none is
+// shorter than kMinChunk keys, below which an item's set-up and its partial
+// result cost more than its keys.
+constexpr long long kItemsWanted = 148 * 6;
+constexpr long long kMinChunk = 256;
+
+static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
+                            int64_t P, int64_t C) {
+  CachePlan pl{};
+  const int64_t rows[2] = {P ? B / G * group * Sq : 0, group * Sq};
+  const int64_t most = rows[0] > rows[1] ? rows[0] : rows[1];
+  pl.mt = most > 16 ? 2 : 1;
+  double total = 0;
+  const int64_t cap[2] = {P, C}, nb[2] = {G, B};
+  for (int s = 0; s < 2; ++s) {
+    pl.rtiles[s] = (int)((rows[s] + 16 * pl.mt - 1) / (16 * pl.mt));
+    total += (double)nb[s] * Hkv * pl.rtiles[s] * cap[s];
+  }
+  int64_t chunk = (int64_t)(total / kItemsWanted) + 1;
+  if (chunk < kMinChunk) chunk = kMinChunk;
+  if (chunk > (1 << 30)) chunk = 1 << 30;
+  chunk = (chunk + 63) & ~63ll;
+  for (int s = 0; s < 2; ++s) {
+    pl.chunk[s] = (int)chunk;
+    pl.nsplit[s] = (int)((cap[s] + chunk - 1) / chunk);
+  }
+  if (P == 0 && C == 0) pl.nsplit[1] = 1;  // nothing to see: an item that writes zeros
+  pl.NS = pl.nsplit[0] + pl.nsplit[1];
+  return pl;
+}
+
+static bool cache_sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t G, int64_t P,
+                           int64_t C, int64_t D) {
+  if (B < 0 || Hq < 0 || Hkv < 1 || Sq < 0 || G < 1 || P < 0 || C < 0) return false;
+  if (D < 8 || D > 128 || D % 8) return false;
+  if (P > (1 << 30) || C > (1 << 30)) return false;
+  if (Hq % Hkv || B % G) return false;
+  // rows are counted in 32 bits
+  const int64_t lim = 1ll << 30;
+  return B <= lim && Hq <= lim && Sq <= lim && B * Hq <= lim && B * Hq * Sq <= lim;
+}
+
+// A view that 16-byte loads can read; the strides of dimensions of one entry
+// are not looked at.
+static int cache_view_ok(const mi_tensor4& t, int64_t n0, int64_t n1, int64_t n2) {
+  if (t.head_index || t.n_replica) return MI_ERR_SHAPE;
+  if (t.stride_d != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15)) return MI_ERR_ALIGN;
+  if ((n0 > 1 && t.stride_b % 8) || (n1 > 1 && t.stride_h % 8) || (n2 > 1 && t.stride_s % 8))
+    return MI_ERR_ALIGN;
+  return MI_OK;
+}
+
+template <typename K, typename... A>
+static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                A... args) {
+  // Programmatic launch: the kernel may be set up while the one before it
+  // drains; it waits (griddepcontrol.wait) before it reads its results.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <typename DT, int DK, int MT, bool STATS>
+static int launch_rows(const CacheParams& p, long long items, cudaStream_t stream) {
+  using L = RowsSmem<DK, STATS>;
+  auto kern = cache_rows_kernel<DT, DK, MT, STATS>;
+  constexpr int kJoin = STATS ? 0 : kRowsWarps * 16 * MT * (DK + 4) * 4;
+  constexpr int kQ = 16 * MT * L::kPitch;
+  constexpr int bytes = L::kRing > kJoin ? (L::kRing > kQ ? L::kRing : kQ) : kJoin;
+  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) {
+    kern<<<(unsigned)items, 32 * kRowsWarps, bytes, stream>>>(p);
+    err = cudaGetLastError();
+  }
+  if (err != cudaSuccess) {
+    debug_launch_failure("cache_rows_kernel", reinterpret_cast<const void*>(kern), err,
+                         32 * kRowsWarps, bytes);
+    return MI_ERR_LAUNCH;
+  }
+  return MI_OK;
+}
+
+template <typename DT, bool STATS>
+static int launch_rows_dk(const CacheParams& p, int mt, long long items, cudaStream_t st) {
+  if (p.D <= 64)
+    return mt == 1 ? launch_rows<DT, 64, 1, STATS>(p, items, st)
+                   : launch_rows<DT, 64, 2, STATS>(p, items, st);
+  if (p.D <= 96)
+    return mt == 1 ? launch_rows<DT, 96, 1, STATS>(p, items, st)
+                   : launch_rows<DT, 96, 2, STATS>(p, items, st);
+  return mt == 1 ? launch_rows<DT, 128, 1, STATS>(p, items, st)
+                 : launch_rows<DT, 128, 2, STATS>(p, items, st);
+}
+
+static void set_seg(CacheSeg& s, const mi_tensor4& k, const mi_tensor4& v, const int32_t* len,
+                    int64_t cap, int64_t nb, int64_t seqs, int64_t rows, int causal) {
+  s.k = static_cast<const uint16_t*>(k.ptr);
+  s.v = static_cast<const uint16_t*>(v.ptr);
+  s.ks_b = nb > 1 ? k.stride_b : 0;
+  s.ks_h = k.stride_h;
+  s.ks_s = k.stride_s;
+  s.vs_b = nb > 1 ? v.stride_b : 0;
+  s.vs_h = v.stride_h;
+  s.vs_s = v.stride_s;
+  s.len = len;
+  s.cap = (int)cap;
+  s.nb = (int)nb;
+  s.seqs = (int)seqs;
+  s.rows = (int)rows;
+  s.causal = causal;
+}
+
+}  // namespace mib200
+
+using namespace mib200;
+
+extern "C" size_t mi_shared_prefix_fwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv,
+                                                      int64_t S_q, int64_t G, int64_t P,
+                                                      int64_t C, int64_t D) {
+  if (!cache_sizes_ok(B, Hq, Hkv, S_q, G, P, C, D)) return SIZE_MAX;
+  if (B == 0 || Hq == 0 || S_q == 0) return 0;
+  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, G, P, C);
+  if (pl.NS == 1) return 0;
+  const double need = (double)B * Hq * S_q * pl.NS * (D * 4 + 8);
+  if (need > 1e15) return SIZE_MAX;
+  const size_t slots = (size_t)(B * Hq * S_q) * pl.NS;
+  return align_up(slots * D * 4) + align_up(slots * 8);
+}
+
+extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor4 v_prefix,
+                                    mi_tensor4 k, mi_tensor4 v, mi_tensor4 out, float* lse,
+                                    int64_t B, int64_t Hq, int64_t Hkv, int64_t S_q, int64_t G,
+                                    int64_t P, int64_t C, int64_t D, int dtype,
+                                    const int32_t* prefix_lengths, const int32_t* lengths,
+                                    int causal, float softmax_scale, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (dtype != MI_F16 && dtype != MI_BF16) return MI_ERR_DTYPE;
+  if (!cache_sizes_ok(B, Hq, Hkv, S_q, G, P, C, D)) return MI_ERR_SHAPE;
+  if (B == 0 || Hq == 0 || S_q == 0) return MI_OK;
+  int rc;
+  if ((rc = cache_view_ok(q, B, Hq, S_q)) != MI_OK) return rc;
+  if ((rc = cache_view_ok(out, B, Hq, S_q)) != MI_OK) return rc;
+  if (P && ((rc = cache_view_ok(k_prefix, G, Hkv, P)) != MI_OK ||
+            (rc = cache_view_ok(v_prefix, G, Hkv, P)) != MI_OK))
+    return rc;
+  if (C && ((rc = cache_view_ok(k, B, Hkv, C)) != MI_OK ||
+            (rc = cache_view_ok(v, B, Hkv, C)) != MI_OK))
+    return rc;
+  const int64_t group = Hq / Hkv;
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C);
+  const size_t need = mi_shared_prefix_fwd_workspace_size(B, Hq, Hkv, S_q, G, P, C, D);
+  if (need == SIZE_MAX) return MI_ERR_SHAPE;
+  if (need && (!workspace || workspace_bytes < need ||
+               (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return MI_ERR_WORKSPACE;
+
+  CacheParams p{};
+  p.q = static_cast<const uint16_t*>(q.ptr);
+  p.qs_b = q.stride_b;
+  p.qs_h = q.stride_h;
+  p.qs_s = q.stride_s;
+  p.out = static_cast<uint16_t*>(out.ptr);
+  p.os_b = out.stride_b;
+  p.os_h = out.stride_h;
+  p.os_s = out.stride_s;
+  p.lse = lse;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.group = (int)group;
+  p.Sq = (int)S_q;
+  p.D = (int)D;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  set_seg(p.seg[0], k_prefix, v_prefix, prefix_lengths, P, G, B / G, B / G * group * S_q, 0);
+  set_seg(p.seg[1], k, v, lengths, C, B, 1, group * S_q, causal ? 1 : 0);
+  for (int s = 0; s < 2; ++s) {
+    p.seg[s].rtiles = pl.rtiles[s];
+    p.seg[s].nsplit = pl.nsplit[s];
+    p.seg[s].chunk = pl.chunk[s];
+  }
+  p.seg[1].slot0 = pl.nsplit[0];
+  p.NS = pl.NS;
+  const int64_t slots = B * Hq * S_q * pl.NS;
+  p.opart = static_cast<float*>(workspace);
+  if (need)
+    p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) +
+                                     align_up((size_t)slots * D * 4));
+  const long long items[2] = {(long long)G * Hkv * pl.rtiles[0] * pl.nsplit[0],
+                              (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1]};
+  p.items0 = items[0];
+  if (items[0] + items[1] > 0x7fffffffll) return MI_ERR_SHAPE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool bf = dtype == MI_BF16;
+  rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, items[0] + items[1], st)
+          : launch_rows_dk<__half, false>(p, pl.mt, items[0] + items[1], st);
+  if (rc != MI_OK || p.NS == 1) return rc;
+  const long long nrows = B * Hq * S_q;
+  const dim3 grid((unsigned)((nrows + 3) / 4));
+  const cudaError_t err =
+      bf ? launch_after(cache_combine_kernel<__nv_bfloat16>, grid, 128, 0, st, p, nrows)
+         : launch_after(cache_combine_kernel<__half>, grid, 128, 0, st, p, nrows);
+  return err == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;
+}

@@ -5,3 +5,6 @@
 #include "block_sparse.cu"
 #include "vs_index.cu"
 #include "noalloc.cu"
+#include "cache_attn.cu"
+#include "cache_weights.cu"
+#include "evict.cu"

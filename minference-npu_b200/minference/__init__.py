@@ -7,8 +7,11 @@ sparse ops, with the device work done by hand-written sm_100a CUDA kernels
 """
 
 from .ops import (
+    accumulate_attention_weights,
     block_sparse_attention,
     dense_attention,
+    evict_cache,
+    shared_prefix_attention,
     streaming_forward,
     vertical_slash_sparse_attention,
 )
@@ -23,6 +26,9 @@ __all__ = [
     "dense_attention",
     "streaming_forward",
     "vertical_slash_sparse_attention",
+    "shared_prefix_attention",
+    "accumulate_attention_weights",
+    "evict_cache",
 ]
 
 

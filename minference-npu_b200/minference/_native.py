@@ -104,6 +104,20 @@ def lib() -> ctypes.CDLL:
         L.mi_vs_sparse_fwd_rows.restype = I
         L.mi_vs_convert_indexes.argtypes = [P, P, I64, P, I64, I64, I64, I64, P, P, P, P, P]
         L.mi_vs_convert_indexes.restype = I
+        L.mi_shared_prefix_fwd_workspace_size.argtypes = [I64] * 8
+        L.mi_shared_prefix_fwd_workspace_size.restype = SZ
+        L.mi_shared_prefix_fwd.argtypes = [T4] * 6 + [P] + [I64] * 8 + [I, P, P, I, F, P, SZ, P]
+        L.mi_shared_prefix_fwd.restype = I
+        L.mi_attn_weights_workspace_size.argtypes = [I64] * 6 + [I]
+        L.mi_attn_weights_workspace_size.restype = SZ
+        L.mi_attn_weights.argtypes = ([T4, T4, P, P, P, I64, I64, P, I64, I64] + [I64] * 6
+                                      + [I, I, F, P, SZ, P])
+        L.mi_attn_weights.restype = I
+        L.mi_evict_cache_workspace_size.argtypes = [I64] * 3
+        L.mi_evict_cache_workspace_size.restype = SZ
+        L.mi_evict_cache.argtypes = ([T4, T4, P, I64, I64, T4, T4, P, I64, I64, P, P]
+                                     + [I64] * 7 + [P, P, SZ, P])
+        L.mi_evict_cache.restype = I
         _lib = L
     return _lib
 

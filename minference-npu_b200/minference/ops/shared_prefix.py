@@ -1,0 +1,118 @@
+"""Attention of new tokens over a shared prefix and per-sequence caches.
+
+After the prefill of one long prompt, a batch of sequences continues from it:
+each new token attends to the prompt's keys, which every sequence shares, and
+to its own sequence's cache.  ``shared_prefix_attention`` reads the shared keys
+once for the whole batch, splits both caches along their length, and joins the
+parts by their log-sum-exp.  Without a prefix it is the decode attention of a
+batch of caches with their own lengths and grouped key/value heads, where
+``dense_attention`` takes one length and repeated heads.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _native
+from ._cache import check_output, check_query, check_same, lengths_arg, overlap, rows_view
+from ._common import output as _common_out
+
+__all__ = ["shared_prefix_attention"]
+
+_NULL = _native.mi_tensor4(0, 0, 0, 0, 1)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
+                            v_prefix: torch.Tensor | None, k: torch.Tensor | None,
+                            v: torch.Tensor | None, lengths: torch.Tensor | None = None, *,
+                            prefix_lengths: torch.Tensor | None = None,
+                            scale: float | None = None, causal: bool = True,
+                            return_lse: bool = False, out: torch.Tensor | None = None):
+    """Attention of the new tokens ``q`` ``[B,Hq,S_q,D]``.
+
+    ``k_prefix`` / ``v_prefix`` ``[G,Hkv,P,D]`` (or ``[Hkv,P,D]``: one prefix)
+    hold G prefixes, each shared by ``B/G`` consecutive sequences; ``k`` / ``v``
+    ``[B,Hkv,C,D]`` are the sequences' own caches, in which the new tokens are
+    the last of the ``lengths[b]`` valid rows.  Either pair may be None.
+    ``Hq`` is a multiple of ``Hkv``: consecutive query heads share a key/value
+    head.  A token sees the first ``prefix_lengths[g]`` prefix keys and, if
+    ``causal``, the own keys up to itself (bottom-right aligned), otherwise
+    every valid own key.  Lengths are integer device tensors (None: whole),
+    clamped to the capacity; rows past them are never used, whatever they hold.
+    A token that sees nothing gives 0.
+
+    ``scale`` defaults to ``1/sqrt(D)``.  Returns the output, of q's dtype, or
+    with ``return_lse`` the pair (output, lse float32 ``[B,Hq,S_q]``: natural
+    log of the sum of exponentials, -inf where nothing is seen).  ``out`` is an
+    optional caller-owned view, which must not overlap the inputs."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be [B,Hq,S_q,D]")
+    B, Hq, S_q, D = q.shape
+    if (k_prefix is None) != (v_prefix is None) or (k is None) != (v is None):
+        raise ValueError("keys and values come in pairs")
+    if k is None and k_prefix is None:
+        raise ValueError("neither a prefix nor a cache to attend to")
+    if k_prefix is not None and k_prefix.dim() == 3 and v_prefix.dim() == 3:
+        k_prefix, v_prefix = k_prefix[None], v_prefix[None]
+    kv = k if k is not None else k_prefix
+    if kv.dim() != 4:
+        raise ValueError("keys must be [B,Hkv,C,D] and prefix keys [G,Hkv,P,D] or [Hkv,P,D]")
+    Hkv = kv.shape[1]
+    check_query(q, Hkv)
+    G = P = C = 0
+    if k_prefix is not None:
+        if k_prefix.dim() != 4:
+            raise ValueError("prefix keys must be [G,Hkv,P,D] or [Hkv,P,D]")
+        G, P = k_prefix.shape[0], k_prefix.shape[2]
+        for name, x in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+            check_same(name, x, q, (G, Hkv, P, D))
+        if G < 1 or B % G:
+            raise ValueError(f"{B} sequences over {G} prefixes")
+    elif prefix_lengths is not None:
+        raise ValueError("prefix_lengths without a prefix")
+    if k is not None:
+        C = k.shape[2]
+        for name, x in (("k", k), ("v", v)):
+            check_same(name, x, q, (B, Hkv, C, D))
+    elif lengths is not None:
+        raise ValueError("lengths without own caches")
+    plen = lengths_arg("prefix_lengths", prefix_lengths, G, P, q.device)
+    clen = lengths_arg("lengths", lengths, B, C, q.device)
+    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
+
+    dk = -(-D // 8) * 8
+    if out is not None:
+        res = _common_out(out, (B, Hq, S_q, D), q) if dk == D else out
+        check_same("out", out, q, (B, Hq, S_q, D))
+        check_output("out", out)
+        for name, x in (("q", q), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("k", k),
+                        ("v", v)):
+            if x is not None and overlap(out, x):
+                raise ValueError(f"out overlaps {name}")
+    if out is None or dk != D:
+        res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, S_q), dtype=torch.float32, device=q.device) if return_lse else None
+    qp = rows_view(q, dk)
+    pre = [rows_view(x, dk) for x in (k_prefix, v_prefix)] if P else None
+    cache = [rows_view(x, dk) for x in (k, v)] if C else None
+    L = _native.lib()
+    sizes = (B, Hq, Hkv, S_q, max(G, 1), P, C, dk)
+    need = L.mi_shared_prefix_fwd_workspace_size(*sizes)
+    if need > 1 << 62:
+        raise ValueError(f"sizes not supported: q {tuple(q.shape)}, prefix {P}, cache {C}")
+    with torch.cuda.device(q.device):
+        ws = _native.workspace(need, q.device) if need else None
+        rc = L.mi_shared_prefix_fwd(
+            _native.t4(qp), *([_native.t4(x) for x in pre] if pre else (_NULL, _NULL)),
+            *([_native.t4(x) for x in cache] if cache else (_NULL, _NULL)), _native.t4(res),
+            lse.data_ptr() if return_lse else None, *sizes, _native.dtype_code(q),
+            plen.data_ptr() if plen is not None and P else None,
+            clen.data_ptr() if clen is not None and C else None, int(bool(causal)), sc,
+            ws.data_ptr() if need else None, ws.numel() if need else 0,
+            _native.stream_ptr(q.device))
+    _native.check(rc, "mi_shared_prefix_fwd")
+    if dk != D:
+        res = res[..., :D] if out is None else out.copy_(res[..., :D])
+    return (res, lse) if return_lse else res
