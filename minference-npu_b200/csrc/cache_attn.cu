@@ -2,6 +2,7 @@
 // query rows, the kernel that joins partial results, and the C entry point.
 // The split of the work is described at the top of cache_attn.cuh.
 #include "cache_attn.cuh"
+#include "cache_tiles.cu"
 #include "host_util.h"
 #include "mma_sync.cuh"
 
@@ -297,6 +298,9 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
       if (c == 0) p.ml[at] = make_float2(M, lt);
     }
   }
+  // The tile kernel of the same call may still run: end after it, so that what
+  // waits for this kernel waits for both.
+  pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -357,39 +361,94 @@ __global__ void __launch_bounds__(128) cache_combine_kernel(const __grid_constan
 // Host: the split, checks and launches
 // ---------------------------------------------------------------------------
 struct CachePlan {
-  int mt;                  // 16-row tiles per item
-  int rtiles[2], nsplit[2], chunk[2];
+  // rows of a sequence walk prefix and own cache in one tile (segment 1's
+  // fields below; ranges cover both)
+  bool joint;
+  bool tile[2];            // segment by cache_tiles_kernel, otherwise by cache_rows_kernel
+  int mt;                  // 16-row tiles per item of cache_rows_kernel
+  int rtiles[2], nsplit[2];
+  int chunk[2];            // keys per range
   int NS;
 };
 
-// Cuts both segments into ranges of one length, so that about six items per
-// SM exist (two run at a time; the rest evens out ragged lengths) but none is
-// shorter than kMinChunk keys, below which an item's set-up and its partial
-// result cost more than its keys.
+// cache_rows_kernel: ranges of one length over its segments, so that about six
+// items per SM exist (two run at a time; the rest evens out ragged lengths)
+// but none is shorter than kMinChunk keys, below which an item's set-up and
+// its partial result cost more than its keys.
 constexpr long long kItemsWanted = 148 * 6;
 constexpr long long kMinChunk = 256;
+// Most rows for which streaming the keys past warp-level tiles beats a 128-row
+// tcgen05 tile.
+constexpr int64_t kRowsMost = 32;
+constexpr int64_t kTileMinDim = 32;
+
+// cache_tiles_kernel: ranges per tile.  Two items run on each of the 148 SMs;
+// an item costs its blocks plus kItemCost (set-up, first loads, epilogue), and
+// a partial result to be joined kJoinCost more, in units of a 64-key block.
+static int tile_ranges(int64_t tiles, int64_t blocks) {
+  constexpr double kItemCost = 6, kJoinCost = 4;
+  const int64_t slots = 2 * 148;
+  int best = 1;
+  double best_cost = 1e300;
+  for (int64_t ns = 1; ns <= slots && ns <= blocks; ++ns) {
+    const int64_t per = (blocks + ns - 1) / ns;
+    const int64_t waves = (tiles * ns + slots - 1) / slots;
+    const double cost = (double)waves * (per + kItemCost + (ns > 1 ? kJoinCost : 0));
+    if (cost < best_cost) best_cost = cost, best = (int)ns;
+  }
+  return best;
+}
 
 static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
-                            int64_t P, int64_t C) {
+                            int64_t P, int64_t C, int64_t D) {
   CachePlan pl{};
-  const int64_t rows[2] = {P ? B / G * group * Sq : 0, group * Sq};
-  const int64_t most = rows[0] > rows[1] ? rows[0] : rows[1];
-  pl.mt = most > 16 ? 2 : 1;
-  double total = 0;
+  const bool use[2] = {P > 0, C > 0 || P == 0};
+  const int64_t rows[2] = {use[0] ? B / G * group * Sq : 0, use[1] ? group * Sq : 0};
   const int64_t cap[2] = {P, C}, nb[2] = {G, B};
+  const bool can = D >= kTileMinDim;
+  for (int s = 0; s < 2; ++s) pl.tile[s] = can && cap[s] > 0 && rows[s] > kRowsMost;
+  // One walk over prefix and own keys where a sequence's rows fill tiles about
+  // as well as all sequences' rows together do.
+  const int64_t own_tiles = B * ((rows[1] + 127) / 128);
+  const int64_t all_tiles = G * ((rows[0] + 127) / 128);
+  pl.joint = pl.tile[0] && pl.tile[1] && own_tiles * 4 <= all_tiles * 5;
+  if (pl.joint) {
+    pl.tile[0] = false;
+    pl.rtiles[1] = (int)((rows[1] + 127) / 128);
+    const int64_t blocks = (P + 63) / 64 + (C + 63) / 64;
+    const int ns = tile_ranges(B * Hkv * pl.rtiles[1], blocks);
+    pl.chunk[1] = (int)((blocks + ns - 1) / ns) * 64;
+    pl.nsplit[1] = (int)((blocks * 64 + pl.chunk[1] - 1) / pl.chunk[1]);
+    pl.NS = pl.nsplit[1];
+    return pl;
+  }
+  double total = 0;
+  int64_t most = 0;
+  for (int s = 0; s < 2; ++s)
+    if (use[s] && !pl.tile[s] && rows[s] > most) most = rows[s];
+  pl.mt = most > 16 ? 2 : 1;
   for (int s = 0; s < 2; ++s) {
-    pl.rtiles[s] = (int)((rows[s] + 16 * pl.mt - 1) / (16 * pl.mt));
-    total += (double)nb[s] * Hkv * pl.rtiles[s] * cap[s];
+    if (!use[s]) continue;
+    const int per = pl.tile[s] ? 128 : 16 * pl.mt;
+    pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
+    if (!pl.tile[s]) total += (double)nb[s] * Hkv * pl.rtiles[s] * cap[s];
   }
   int64_t chunk = (int64_t)(total / kItemsWanted) + 1;
   if (chunk < kMinChunk) chunk = kMinChunk;
   if (chunk > (1 << 30)) chunk = 1 << 30;
   chunk = (chunk + 63) & ~63ll;
   for (int s = 0; s < 2; ++s) {
-    pl.chunk[s] = (int)chunk;
-    pl.nsplit[s] = (int)((cap[s] + chunk - 1) / chunk);
+    if (!use[s]) continue;
+    int64_t ch = chunk;
+    if (pl.tile[s]) {
+      const int64_t blocks = (cap[s] + 63) / 64;
+      const int ns = tile_ranges(nb[s] * Hkv * pl.rtiles[s], blocks);
+      ch = (blocks + ns - 1) / ns * 64;
+    }
+    pl.chunk[s] = (int)ch;
+    // at least one range: with no key at all it writes the zeros
+    pl.nsplit[s] = cap[s] ? (int)((cap[s] + ch - 1) / ch) : 1;
   }
-  if (P == 0 && C == 0) pl.nsplit[1] = 1;  // nothing to see: an item that writes zeros
   pl.NS = pl.nsplit[0] + pl.nsplit[1];
   return pl;
 }
@@ -398,20 +457,21 @@ static bool cache_sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64
                            int64_t C, int64_t D) {
   if (B < 0 || Hq < 0 || Hkv < 1 || Sq < 0 || G < 1 || P < 0 || C < 0) return false;
   if (D < 8 || D > 128 || D % 8) return false;
-  if (P > (1 << 30) || C > (1 << 30)) return false;
+  if (P > (1 << 30) || C > (1 << 30) || P + C > (1 << 30)) return false;
   if (Hq % Hkv || B % G) return false;
   // rows are counted in 32 bits
   const int64_t lim = 1ll << 30;
   return B <= lim && Hq <= lim && Sq <= lim && B * Hq <= lim && B * Hq * Sq <= lim;
 }
 
-// A view that 16-byte loads can read; the strides of dimensions of one entry
-// are not looked at.
+// A view that 16-byte loads and tensor maps can read; the strides of dimensions
+// of one entry are not looked at.
 static int cache_view_ok(const mi_tensor4& t, int64_t n0, int64_t n1, int64_t n2) {
   if (t.head_index || t.n_replica) return MI_ERR_SHAPE;
   if (t.stride_d != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15)) return MI_ERR_ALIGN;
-  if ((n0 > 1 && t.stride_b % 8) || (n1 > 1 && t.stride_h % 8) || (n2 > 1 && t.stride_s % 8))
-    return MI_ERR_ALIGN;
+  const int64_t n[3] = {n0, n1, n2}, s[3] = {t.stride_b, t.stride_h, t.stride_s};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return MI_ERR_ALIGN;
   return MI_OK;
 }
 
@@ -434,7 +494,7 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
 }
 
 template <typename DT, int DK, int MT, bool STATS>
-static int launch_rows(const CacheParams& p, long long items, cudaStream_t stream) {
+static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
   using L = RowsSmem<DK, STATS>;
   auto kern = cache_rows_kernel<DT, DK, MT, STATS>;
   constexpr int kJoin = STATS ? 0 : kRowsWarps * 16 * MT * (DK + 4) * 4;
@@ -442,8 +502,12 @@ static int launch_rows(const CacheParams& p, long long items, cudaStream_t strea
   constexpr int bytes = L::kRing > kJoin ? (L::kRing > kQ ? L::kRing : kQ) : kJoin;
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (err == cudaSuccess) {
-    kern<<<(unsigned)items, 32 * kRowsWarps, bytes, stream>>>(p);
-    err = cudaGetLastError();
+    if (after) {
+      err = launch_after(kern, dim3((unsigned)items), 32 * kRowsWarps, bytes, stream, p);
+    } else {
+      kern<<<(unsigned)items, 32 * kRowsWarps, bytes, stream>>>(p);
+      err = cudaGetLastError();
+    }
   }
   if (err != cudaSuccess) {
     debug_launch_failure("cache_rows_kernel", reinterpret_cast<const void*>(kern), err,
@@ -454,15 +518,16 @@ static int launch_rows(const CacheParams& p, long long items, cudaStream_t strea
 }
 
 template <typename DT, bool STATS>
-static int launch_rows_dk(const CacheParams& p, int mt, long long items, cudaStream_t st) {
+static int launch_rows_dk(const CacheParams& p, int mt, long long items, bool after,
+                          cudaStream_t st) {
   if (p.D <= 64)
-    return mt == 1 ? launch_rows<DT, 64, 1, STATS>(p, items, st)
-                   : launch_rows<DT, 64, 2, STATS>(p, items, st);
+    return mt == 1 ? launch_rows<DT, 64, 1, STATS>(p, items, after, st)
+                   : launch_rows<DT, 64, 2, STATS>(p, items, after, st);
   if (p.D <= 96)
-    return mt == 1 ? launch_rows<DT, 96, 1, STATS>(p, items, st)
-                   : launch_rows<DT, 96, 2, STATS>(p, items, st);
-  return mt == 1 ? launch_rows<DT, 128, 1, STATS>(p, items, st)
-                 : launch_rows<DT, 128, 2, STATS>(p, items, st);
+    return mt == 1 ? launch_rows<DT, 96, 1, STATS>(p, items, after, st)
+                   : launch_rows<DT, 96, 2, STATS>(p, items, after, st);
+  return mt == 1 ? launch_rows<DT, 128, 1, STATS>(p, items, after, st)
+                 : launch_rows<DT, 128, 2, STATS>(p, items, after, st);
 }
 
 static void set_seg(CacheSeg& s, const mi_tensor4& k, const mi_tensor4& v, const int32_t* len,
@@ -492,7 +557,7 @@ extern "C" size_t mi_shared_prefix_fwd_workspace_size(int64_t B, int64_t Hq, int
                                                       int64_t C, int64_t D) {
   if (!cache_sizes_ok(B, Hq, Hkv, S_q, G, P, C, D)) return SIZE_MAX;
   if (B == 0 || Hq == 0 || S_q == 0) return 0;
-  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, G, P, C);
+  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, G, P, C, D);
   if (pl.NS == 1) return 0;
   const double need = (double)B * Hq * S_q * pl.NS * (D * 4 + 8);
   if (need > 1e15) return SIZE_MAX;
@@ -520,7 +585,7 @@ extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor
             (rc = cache_view_ok(v, B, Hkv, C)) != MI_OK))
     return rc;
   const int64_t group = Hq / Hkv;
-  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C);
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C, D);
   const size_t need = mi_shared_prefix_fwd_workspace_size(B, Hq, Hkv, S_q, G, P, C, D);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||
@@ -559,13 +624,39 @@ extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor
                                      align_up((size_t)slots * D * 4));
   const long long items[2] = {(long long)G * Hkv * pl.rtiles[0] * pl.nsplit[0],
                               (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1]};
-  p.items0 = items[0];
   if (items[0] + items[1] > 0x7fffffffll) return MI_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = dtype == MI_BF16;
-  rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, items[0] + items[1], st)
-          : launch_rows_dk<__half, false>(p, pl.mt, items[0] + items[1], st);
-  if (rc != MI_OK || p.NS == 1) return rc;
+  TileParams tp{};
+  long long rows_items = 0;
+  for (int s = 0; s < 2; ++s) {
+    if (!pl.tile[s]) {
+      rows_items += items[s];
+      continue;
+    }
+    TileGroup& g = tp.grp[s];
+    g.rows_of = s;
+    g.use0 = s == 0 || pl.joint;
+    g.use1 = s == 1;
+    g.rtiles = pl.rtiles[s];
+    g.nsplit = pl.nsplit[s];
+    g.blocks = pl.chunk[s] / 64;
+    g.slot0 = p.seg[s].slot0;
+    g.items = items[s];
+  }
+  const bool tiles = pl.tile[0] || pl.tile[1];
+  if (tiles) {
+    tp.c = p;
+    rc = launch_tiles<false>(tp, dtype, k_prefix, v_prefix, k, v, st);
+    if (rc != MI_OK) return rc;
+  }
+  if (rows_items) {
+    p.items0 = pl.tile[0] ? 0 : items[0];
+    rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, rows_items, tiles, st)
+            : launch_rows_dk<__half, false>(p, pl.mt, rows_items, tiles, st);
+    if (rc != MI_OK) return rc;
+  }
+  if (p.NS == 1) return MI_OK;
   const long long nrows = B * Hq * S_q;
   const dim3 grid((unsigned)((nrows + 3) / 4));
   const cudaError_t err =

@@ -1,0 +1,493 @@
+// Attention over caches for many query rows per key/value head (tcgen05).
+//
+// A work item is one 128-row tile of query rows -- the rows of all sequences
+// that share a prefix, or of one sequence -- against a range of the 64-key
+// blocks that the tile walks: prefix blocks, then (if the tile's rows belong
+// to one sequence) the blocks of its own cache.  Warp roles and the TMEM
+// hand-over are those of attn_fwd_kernel: warps 0-3 softmax (one row per
+// thread), warp 4 TMA, warp 5 MMA issue, two items per SM so that one item's
+// softmax overlaps the other's products.  Differences, each for this shape of
+// work: the tile's rows come from several heads and sequences, so Q is
+// gathered with plain loads; row sums are kept in registers, because at
+// D = 128 O fills what the two S buffers leave of half the TMEM; O leaves
+// unnormalised (or finished, when the item has the whole row).
+//
+// STATS computes the rows' (maximum, sum) only: no V, no P, no O.
+#include <cstring>
+
+#include "cache_attn.cuh"
+#include "host_util.h"
+#include "mma_sync.cuh"
+
+namespace mib200 {
+
+// Items of one kind: rows of segment `rows_of`, keys of segment 0 and / or 1.
+struct TileGroup {
+  int rows_of;
+  int use0, use1;
+  int rtiles, nsplit, blocks;  // blocks: key blocks per range
+  int slot0;
+  long long items;
+};
+
+struct TileParams {
+  CacheParams c;
+  TileGroup grp[2];
+};
+
+template <int DK, bool STATS>
+struct TileSmem {
+  static constexpr int NC = DK / 32;
+  static constexpr int kQBytes = NC * 128 * 64;
+  static constexpr int kBlock = NC * 64 * 64;  // 64 keys of K or V
+  // two blocks per SM: 113 KB each at most
+  static constexpr int KS = STATS ? (DK == 128 ? 4 : 5) : (DK == 128 ? 2 : (DK == 96 ? 3 : 5));
+  static constexpr int VS = STATS ? 0 : (DK == 128 ? 3 : (DK == 96 ? 4 : 5));
+  static constexpr int kKOff = kQBytes;
+  static constexpr int kVOff = kKOff + KS * kBlock;
+  static constexpr int kBarOff = kVOff + VS * kBlock;
+  // k_full[KS] k_empty[KS] v_full[VS] v_empty[VS] s_full[2] p_full[2] pv_done[2]
+  static constexpr int kNumBars = 2 * KS + 2 * VS + 6;
+  static constexpr int kSlotOff = kBarOff + kNumBars * 8;
+  static constexpr int kBytes = kSlotOff + 8;
+  static constexpr int kAlloc = kBytes + 512;  // the base is aligned to a swizzle atom
+  static constexpr uint32_t kTmemCols = STATS ? 128 : 256;
+  static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
+  static_assert(STATS || 128 + DK <= 256, "TMEM");
+};
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+
+constexpr int kTileThreads = 192;
+constexpr float kTileRescale = 12.0f;  // log2 growth of a row's maximum that rescales O
+
+template <typename DT, int DK, bool STATS>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    cache_tiles_kernel(const __grid_constant__ CUtensorMap tm_kp,
+                       const __grid_constant__ CUtensorMap tm_vp,
+                       const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ TileParams tp) {
+  using L = TileSmem<DK, STATS>;
+  constexpr int NC = L::NC, KS = L::KS, VS = L::VS;
+  constexpr bool kBF16 = DType<DT>::kBF16;
+  const CacheParams& p = tp.c;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~static_cast<uintptr_t>(511));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* pv_done = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlotOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kSlotOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch();
+
+  // ---- the item ---------------------------------------------------------------
+  long long it = blockIdx.x;
+  const bool second = it >= tp.grp[0].items;
+  if (second) it -= tp.grp[0].items;
+  const TileGroup& gr = tp.grp[second ? 1 : 0];
+  const CacheSeg& rs = p.seg[gr.rows_of];
+  const int rt = (int)(it % gr.rtiles);
+  it /= gr.rtiles;
+  const int sp = (int)(it % gr.nsplit);
+  it /= gr.nsplit;
+  const int h = (int)(it % p.Hkv);
+  const int e = (int)(it / p.Hkv);                        // entry of the row segment
+  const int e0 = gr.rows_of == 0 ? e : e / p.seg[0].seqs;  // prefix
+  const int r0 = rt * 128;
+  const int nrows = min(128, rs.rows - r0);
+  const int len0 = gr.use0 ? cache_len(p.seg[0], e0) : 0;
+  const int len1 = gr.use1 ? cache_len(p.seg[1], e) : 0;
+  const bool causal = p.seg[1].causal != 0;
+  int end1 = len1;  // own keys that the tile's last token sees
+  if (gr.use1 && causal) {
+    const int last = r0 + nrows - 1;
+    const int smax = (r0 / p.Sq != last / p.Sq) ? p.Sq - 1 : last % p.Sq;
+    end1 = max(0, len1 - (p.Sq - 1 - smax));
+  }
+  const int n0 = (len0 + 63) >> 6, n1 = (end1 + 63) >> 6;
+  const int j0 = min(n0 + n1, (int)min((long long)sp * gr.blocks, (long long)(n0 + n1)));
+  const int nent = min(n0 + n1 - j0, gr.blocks);
+
+  // ---- set-up: barriers, TMEM, Q (64-byte swizzled chunks of 32 dims) -----------
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < KS; ++s) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
+    for (int s = 0; s < VS; ++s) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
+    for (int i = 0; i < 2; ++i)
+      mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128), mbar_init(&pv_done[i], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
+  // A negative scale is taken into Q (its sign bits), so that the largest
+  // score is the largest product.
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  if (nent > 0) {
+    for (int i = threadIdx.x; i < 128 * (DK / 8); i += kTileThreads) {
+      const int r = i / (DK / 8), u = i - r * (DK / 8);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < nrows && u * 8 < p.D) {
+        int b, hd, tk;
+        cache_row(p, rs, e, h, r0 + r, b, hd, tk);
+        x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b + hd * p.qs_h + tk * p.qs_s + u * 8);
+        x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+      }
+      *reinterpret_cast<uint4*>(smem + (u >> 2) * (128 * 64) + r * 64 +
+                                (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x;
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 4) {
+    // ---- TMA: K0, K1, V0, K2, V1, ... ---------------------------------------
+    if (lane == 0) {
+      auto load = [&](uint8_t* dst, uint64_t* full, int j, bool val) {
+        const int J = j0 + j;
+        const bool own = J >= n0;
+        const CUtensorMap* map = own ? (val ? &tm_v : &tm_k) : (val ? &tm_vp : &tm_kp);
+        const int key = (own ? J - n0 : J) * 64, ent = own ? e : e0;
+        mbar_arrive_expect_tx(full, L::kBlock);
+        for (int c = 0; c < NC; ++c) tma_load_4d(dst + c * (64 * 64), map, full, c * 32, key, h, ent);
+      };
+      bool ok = true;
+      for (int j = 0; ok && j < nent + (STATS ? 0 : 1); ++j) {
+        if (*abort_flag) break;
+        if (j < nent) {
+          const int st = j % KS, use = j / KS;
+          if (use > 0 && !mbar_wait(&k_empty[st], (use - 1) & 1, 131)) { ok = false; break; }
+          load(smem + L::kKOff + st * L::kBlock, &k_full[st], j, false);
+        }
+        if constexpr (!STATS) {
+          if (j >= 1) {
+            const int st = (j - 1) % VS, use = (j - 1) / VS;
+            if (use > 0 && !mbar_wait(&v_empty[st], (use - 1) & 1, 132)) { ok = false; break; }
+            load(smem + L::kVOff + st * L::kBlock, &v_full[st], j - 1, true);
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 5) {
+    // ---- MMA issue (converged warp, one elected lane) ------------------------
+    constexpr uint32_t idesc_qk = make_idesc_f16(kBF16, 128, 64, false, false);
+    constexpr uint32_t idesc_pv = make_idesc_f16(kBF16, 128, DK, false, true);
+    const uint64_t qd0 = make_desc_sw64(smem_u32(smem), 16, 512);
+    const uint64_t kd0 = make_desc_sw64(smem_u32(smem + L::kKOff), 16, 512);
+    const uint64_t vd0 = make_desc_sw64(smem_u32(smem + L::kVOff), 64 * 64, 512);
+    auto issue_qk = [&](int j) -> bool {
+      const int st = j % KS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&k_full[st], (j / KS) & 1, 133))) return false;
+      tc_fence_after();
+      if (elect_one_sync()) {
+        const uint64_t kd = kd0 + (uint64_t)((st * L::kBlock) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ++ks) {
+          const uint32_t off = (ks & 1) * 32;
+          umma_f16_ss(tmem_base + (j & 1) * 64, qd0 + (((ks >> 1) * (128 * 64) + off) >> 4),
+                      kd + (((ks >> 1) * (64 * 64) + off) >> 4), idesc_qk, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[j & 1]);
+        umma_commit(&k_empty[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+    if (nent > 0) ok = issue_qk(0);
+    if (STATS && ok && nent > 1) ok = issue_qk(1);
+    for (int j = 0; ok && j < nent; ++j) {
+      if (*abort_flag) { ok = false; break; }
+      // S buffer (j+1)&1 last held P(j-1), which PV(j-1) has read: products of
+      // one thread run in issue order.
+      if (!STATS && j + 1 < nent && !issue_qk(j + 1)) { ok = false; break; }
+      if (STATS && j + 2 >= nent) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(&p_full[j & 1], (j >> 1) & 1, 134))) {
+        ok = false;
+        break;
+      }
+      if constexpr (STATS) {
+        tc_fence_after();
+        if (!issue_qk(j + 2)) { ok = false; break; }  // its S buffer has been read
+      } else {
+        const int st = j % VS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / VS) & 1, 135))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (elect_one_sync()) {
+          const uint64_t vd = vd0 + (uint64_t)((st * L::kBlock) >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f16_ts(tmem_base + 128, tmem_base + (j & 1) * 64 + ks * 8,
+                        vd + (uint64_t)((ks * 1024) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[j & 1]);
+          umma_commit(&v_empty[st]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+  } else {
+    // ---- softmax: thread = row ---------------------------------------------------
+    const int row = threadIdx.x;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+    const bool live = row < nrows;
+    int lim0 = len0, lim1 = len1;  // keys that the row sees
+    if (live && causal) lim1 = len1 - (p.Sq - 1 - (r0 + row) % p.Sq);
+    // Blocks below `full` are whole for every row of the warp, blocks from
+    // `none` on empty.  Rows past the tile's last (Q = 0) take what the others
+    // see; a warp of such rows only sees nothing.
+    const int full0 = __reduce_min_sync(0xffffffffu, live ? lim0 : 0x7fffffff);
+    const int full1 = __reduce_min_sync(0xffffffffu, live ? lim1 : 0x7fffffff);
+    const int none0 = __reduce_max_sync(0xffffffffu, live ? lim0 : 0);
+    const int none1 = __reduce_max_sync(0xffffffffu, live ? lim1 : 0);
+    if (!live) lim0 = none0, lim1 = none1;
+    // not 0: a hidden score of -inf has to stay -inf when it is scaled
+    const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+    for (int j = 0; j < nent; ++j) {
+      const int J = j0 + j;
+      const bool own = J >= n0;
+      const int key0 = (own ? J - n0 : J) * 64;
+      if (!all(mbar_wait(&s_full[j & 1], (j >> 1) & 1, 136))) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t tmem_s = lane_base + (j & 1) * 64;
+      const bool empty = key0 >= (own ? none1 : none0);
+      const bool whole = key0 + 64 <= (own ? full1 : full0);
+      if constexpr (!STATS) {
+        // a cache's stale rows: 0 * V must not let them through
+        const int held = own ? len1 : len0;
+        if (key0 + 64 > held) {
+          if (!all(mbar_wait(&v_full[j % VS], (j / VS) & 1, 137))) { ok = false; break; }
+          uint8_t* vb = smem + L::kVOff + (j % VS) * L::kBlock;
+          for (int i = threadIdx.x; i < NC * 64 * 4; i += 128)
+            if (((i >> 2) & 63) >= held - key0)
+              *reinterpret_cast<uint4*>(vb + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
+      float s[64];
+      uint32_t pk[32];
+      if (!empty) {
+        tmem_ld32(tmem_s, *reinterpret_cast<float(*)[32]>(&s[0]));
+        tmem_ld32(tmem_s + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
+        tmem_wait_ld();
+        if (!whole) {
+          const uint64_t vis = bits_below((long long)(own ? lim1 : lim0) - key0);
+#pragma unroll
+          for (int c = 0; c < 64; ++c) s[c] = ((vis >> c) & 1ull) ? s[c] : -INFINITY;
+        }
+      }
+      auto row_max = [&]() -> float {
+        float a = fmax3(s[0], s[1], s[2]), b = fmax3(s[3], s[4], s[5]);
+        float c = fmax3(s[6], s[7], s[8]), d = fmax3(s[9], s[10], s[11]);
+#pragma unroll
+        for (int x = 12; x < 60; x += 8) {
+          a = fmax3(a, s[x], s[x + 1]);
+          b = fmax3(b, s[x + 2], s[x + 3]);
+          c = fmax3(c, s[x + 4], s[x + 5]);
+          d = fmax3(d, s[x + 6], s[x + 7]);
+        }
+        return fmaxf(fmax3(a, b, fmax3(s[60], s[61], s[62])), fmax3(c, d, s[63]));
+      };
+      auto exp_block = [&](float nm) -> float {
+        float2 t0 = make_float2(0.f, 0.f), t1 = t0;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float x0 = fast_exp2(__fmaf_rn(s[2 * c], sc, nm));
+          const float x1 = fast_exp2(__fmaf_rn(s[2 * c + 1], sc, nm));
+          if (c & 1) t1 = add2(t1, make_float2(x0, x1));
+          else t0 = add2(t0, make_float2(x0, x1));
+          if constexpr (!STATS) pk[c] = DType<DT>::pack2(x0, x1);
+        }
+        t0 = add2(t0, t1);
+        return t0.x + t0.y;
+      };
+      // P against the running maximum straight away; only if some row's maximum
+      // grew by more than 2^12 (or none is known yet) is it computed again.
+      const bool spec = !empty && all(m != -INFINITY);
+      float sum = 0.f, tmax = -INFINITY;
+      if (spec) sum = exp_block(-m);
+      if (!empty) tmax = row_max() * sc;
+      const float mn = fmaxf(m, tmax);
+      const bool need = mn > m + kTileRescale;
+      bool again = !spec;
+      if (__any_sync(0xffffffffu, need)) {
+        if constexpr (!STATS) {
+          if (j > 0) {
+            if (!all(mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, 138))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+        }
+        const float f = need ? (m == -INFINITY ? 0.f : fast_exp2(m - mn)) : 1.f;
+        l *= f;
+        if constexpr (!STATS) {
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < DK / 16; ++c) {
+              float o[16];
+              tmem_ld16(lane_base + 128 + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[x] *= f;
+              tmem_st16(lane_base + 128 + c * 16, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (need) m = mn;
+        again = true;
+      }
+      if (again) {
+        if (empty || m == -INFINITY) {  // nothing seen yet
+          sum = 0.f;
+          if constexpr (!STATS)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pk[c] = 0u;
+        } else {
+          sum = exp_block(-m);
+        }
+      }
+      l += sum;
+      if constexpr (!STATS) {
+        tmem_st32u(tmem_s, pk);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive(&p_full[j & 1]);
+    }
+
+    // ---- epilogue ------------------------------------------------------------
+    if (!STATS && ok && nent > 0) {
+      ok = all(mbar_wait(&pv_done[(nent - 1) & 1], ((nent - 1) >> 1) & 1, 139));
+      tc_fence_after();
+    }
+    if (!ok) *abort_flag = 1;
+    int b = 0, hd = 0, tk = 0;
+    if (live) cache_row(p, rs, e, h, r0 + row, b, hd, tk);
+    const long long grow = ((long long)b * p.Hq + hd) * p.Sq + tk;
+    const bool direct = !STATS && p.NS == 1;
+    const bool seen = m != -INFINITY && ok;
+    const float inv = direct ? (seen && l > 0.f ? 1.f / l : 0.f) : 1.f;
+    const long long at = grow * p.NS + gr.slot0 + sp;
+    if constexpr (!STATS) {
+      if (nent > 0 || direct) {
+#pragma unroll
+        for (int c = 0; c < DK / 32; ++c) {
+          float o[32];
+          __syncwarp();
+          if (nent > 0 && ok) {
+            tmem_ld32(lane_base + 128 + c * 32, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int d = c * 32 + u * 8;
+            if (d >= p.D || !live || (!direct && !seen)) continue;
+            if (direct) {
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (seen) {
+                x.x = DType<DT>::pack2(o[u * 8] * inv, o[u * 8 + 1] * inv);
+                x.y = DType<DT>::pack2(o[u * 8 + 2] * inv, o[u * 8 + 3] * inv);
+                x.z = DType<DT>::pack2(o[u * 8 + 4] * inv, o[u * 8 + 5] * inv);
+                x.w = DType<DT>::pack2(o[u * 8 + 6] * inv, o[u * 8 + 7] * inv);
+              }
+              *reinterpret_cast<uint4*>(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s + d) = x;
+            } else {
+              float4* dst = reinterpret_cast<float4*>(p.opart + at * p.D + d);
+              dst[0] = make_float4(o[u * 8], o[u * 8 + 1], o[u * 8 + 2], o[u * 8 + 3]);
+              dst[1] = make_float4(o[u * 8 + 4], o[u * 8 + 5], o[u * 8 + 6], o[u * 8 + 7]);
+            }
+          }
+        }
+      }
+    }
+    if (live) {
+      if (!direct) p.ml[at] = make_float2(m, l);
+      else if (p.lse) p.lse[grow] = seen ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
+}
+
+template <typename DT, int DK, bool STATS>
+static int launch_tiles_t(const TileParams& tp, const mi_tensor4& kp, const mi_tensor4& vp,
+                          const mi_tensor4& k, const mi_tensor4& v, cudaStream_t st) {
+  using L = TileSmem<DK, STATS>;
+  const CacheParams& p = tp.c;
+  CUtensorMap m[4];
+  memset(m, 0, sizeof(m));
+  const mi_tensor4* t[4] = {&kp, &vp, &k, &v};
+  const bool use0 = (tp.grp[0].items && tp.grp[0].use0) || (tp.grp[1].items && tp.grp[1].use0);
+  const bool use1 = (tp.grp[0].items && tp.grp[0].use1) || (tp.grp[1].items && tp.grp[1].use1);
+  for (int i = 0; i < 4; ++i) {
+    if (!(i < 2 ? use0 : use1) || (STATS && (i & 1))) continue;
+    const CacheSeg& s = p.seg[i / 2];
+    const int rc = make_bnsd_map(&m[i], *t[i], s.nb, p.Hkv, s.cap, p.D, 32, 64);
+    if (rc != MI_OK) return rc;
+  }
+  auto kern = cache_tiles_kernel<DT, DK, STATS>;
+  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         L::kAlloc);
+  if (err == cudaSuccess) {
+    kern<<<(unsigned)(tp.grp[0].items + tp.grp[1].items), kTileThreads, L::kAlloc, st>>>(
+        m[0], m[1], m[2], m[3], tp);
+    err = cudaGetLastError();
+  }
+  if (err != cudaSuccess) {
+    debug_launch_failure("cache_tiles_kernel", reinterpret_cast<const void*>(kern), err,
+                         kTileThreads, L::kAlloc);
+    return MI_ERR_LAUNCH;
+  }
+  return MI_OK;
+}
+
+template <bool STATS>
+static int launch_tiles(const TileParams& tp, int dtype, const mi_tensor4& kp,
+                        const mi_tensor4& vp, const mi_tensor4& k, const mi_tensor4& v,
+                        cudaStream_t st) {
+  const bool bf = dtype == MI_BF16;
+  const int D = tp.c.D;
+  if (D <= 64)
+    return bf ? launch_tiles_t<__nv_bfloat16, 64, STATS>(tp, kp, vp, k, v, st)
+              : launch_tiles_t<__half, 64, STATS>(tp, kp, vp, k, v, st);
+  if (D <= 96)
+    return bf ? launch_tiles_t<__nv_bfloat16, 96, STATS>(tp, kp, vp, k, v, st)
+              : launch_tiles_t<__half, 96, STATS>(tp, kp, vp, k, v, st);
+  return bf ? launch_tiles_t<__nv_bfloat16, 128, STATS>(tp, kp, vp, k, v, st)
+            : launch_tiles_t<__half, 128, STATS>(tp, kp, vp, k, v, st);
+}
+
+}  // namespace mib200

@@ -129,8 +129,293 @@ __global__ void __launch_bounds__(128) weight_cols_kernel(const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: S^T = K Q^T on tcgen05, a tile of 128 keys (the M rows, one per
+// thread) against blocks of 64 query rows.  A key's weight is then a sum along
+// its own TMEM lane: 64 exponentials and adds per block and thread, no exchange
+// between threads, nothing written back.  Bound by the exponentials (16 per
+// clock and SM).  What a cache holds past its length stays in its own lanes,
+// whose sums are dropped.
+//
+// RESQ: all rows of the key/value head (at most QS blocks, packed over its
+// query heads) stay in shared memory while key tiles stream; otherwise a key
+// tile stays while the blocks of each head's rows that see it stream.
+// ---------------------------------------------------------------------------
+template <int DK>
+struct ColsSmem {
+  static constexpr int NC = DK / 32;
+  static constexpr int KS = 2, QS = DK == 128 ? 2 : (DK == 96 ? 4 : 6), SB = 4;
+  static constexpr int kKTile = NC * 128 * 64, kQBlock = NC * 64 * 64;
+  static constexpr int kQOff = KS * kKTile;
+  static constexpr int kRowOff = kQOff + QS * kQBlock;  // per warp: 64 x (-lse), 64 x token
+  static constexpr int kBarOff = kRowOff + 4 * 2 * 512;
+  // k_full[KS] k_empty[KS] q_full[QS] q_empty[QS] s_full[SB] s_empty[SB]
+  static constexpr int kSlotOff = kBarOff + (2 * KS + 2 * QS + 2 * SB) * 8;
+  static constexpr int kAlloc = kSlotOff + 8 + 512;
+  static constexpr uint32_t kTmemCols = SB * 64;
+  static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
+};
+
+struct ColsParams {
+  WeightParams w;
+  int tiles, per;    // key tiles of a (b, h); tiles per item
+  int ranges;        // items per (b, h)
+};
+
+template <typename DT, int DK, bool RESQ>
+__global__ void __launch_bounds__(192, 2)
+    weight_tiles_kernel(const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_q,
+                        const __grid_constant__ ColsParams cp) {
+  using L = ColsSmem<DK>;
+  constexpr int NC = L::NC, KS = L::KS, QS = L::QS, SB = L::SB;
+  const WeightParams& p = cp.w;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~static_cast<uintptr_t>(511));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* q_full = k_empty + KS;
+  uint64_t* q_empty = q_full + QS;
+  uint64_t* s_full = q_empty + QS;
+  uint64_t* s_empty = s_full + SB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlotOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kSlotOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  long long it = blockIdx.x;
+  const int range = (int)(it % cp.ranges);
+  it /= cp.ranges;
+  const int h = (int)(it % p.Hkv), b = (int)(it / p.Hkv);
+  const int len = p.len ? min(max(p.len[b], 0), p.C) : p.C;
+  const int t0 = range * cp.per, t1 = min(cp.tiles, t0 + cp.per);
+  const int tv = min(t1, (len + 127) >> 7);  // tiles from tv on hold no valid key
+  const int rows = p.group * p.Sq;
+  const int nsb = RESQ ? (rows + 63) >> 6 : (p.Sq + 63) >> 6;
+  // First 64-row block of a head that sees key tile t.
+  auto first_block = [&](int t) {
+    return !RESQ && p.causal ? max(0, t * 128 - len + p.Sq) >> 6 : 0;
+  };
+  const int heads = RESQ ? 1 : p.group;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < QS; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < SB; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 128);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
+  if constexpr (RESQ) {
+    if (tv > t0) {
+      for (int i = threadIdx.x; i < nsb * 64 * (DK / 8); i += 192) {
+        const int r = i / (DK / 8), u = i - r * (DK / 8);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && u * 8 < p.D)
+          x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b +
+                                              (long long)(h * p.group + r / p.Sq) * p.qs_h +
+                                              (long long)(r % p.Sq) * p.qs_s + u * 8);
+        *reinterpret_cast<uint4*>(smem + L::kQOff + (r >> 6) * L::kQBlock + (u >> 2) * (64 * 64) +
+                                  (r & 63) * 64 + (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x;
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      bool ok = true;
+      int nq = 0;
+      for (int t = t0; ok && t < tv; ++t) {
+        if (*abort_flag) break;
+        const int st = (t - t0) % KS, use = (t - t0) / KS;
+        if (use > 0 && !mbar_wait(&k_empty[st], (use - 1) & 1, 141)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[st], L::kKTile);
+        for (int c = 0; c < NC; ++c)
+          tma_load_4d(smem + st * L::kKTile + c * (128 * 64), &tm_k, &k_full[st], c * 32, t * 128,
+                      h, b);
+        if constexpr (!RESQ) {
+          for (int g = 0; ok && g < heads; ++g)
+            for (int sb = first_block(t); sb < nsb; ++sb, ++nq) {
+              const int qs = nq % QS, qu = nq / QS;
+              if (qu > 0 && !mbar_wait(&q_empty[qs], (qu - 1) & 1, 142)) { ok = false; break; }
+              mbar_arrive_expect_tx(&q_full[qs], L::kQBlock);
+              for (int c = 0; c < NC; ++c)
+                tma_load_4d(smem + L::kQOff + qs * L::kQBlock + c * (64 * 64), &tm_q, &q_full[qs],
+                            c * 32, sb * 64, h * p.group + g, b);
+            }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 5) {
+    constexpr uint32_t idesc = make_idesc_f16(DType<DT>::kBF16, 128, 64, false, false);
+    const uint64_t kd0 = make_desc_sw64(smem_u32(smem), 16, 512);
+    const uint64_t qd0 = make_desc_sw64(smem_u32(smem + L::kQOff), 16, 512);
+    auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+    bool ok = true;
+    int n = 0;
+    for (int t = t0; ok && t < tv; ++t) {
+      const int st = (t - t0) % KS;
+      if (*abort_flag) { ok = false; break; }
+      if (!all(mbar_wait(&k_full[st], ((t - t0) / KS) & 1, 143))) { ok = false; break; }
+      const int f = first_block(t);
+      for (int g = 0; ok && g < heads; ++g)
+        for (int sb = f; sb < nsb; ++sb, ++n) {
+          const int qs = RESQ ? sb : n % QS, buf = n % SB;
+          if (!RESQ && !all(mbar_wait(&q_full[qs], (n / QS) & 1, 144))) { ok = false; break; }
+          if (n >= SB && !all(mbar_wait(&s_empty[buf], (n / SB - 1) & 1, 145))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one_sync()) {
+            const uint64_t kd = kd0 + (uint64_t)((st * L::kKTile) >> 4);
+            const uint64_t qd = qd0 + (uint64_t)((qs * L::kQBlock) >> 4);
+#pragma unroll
+            for (int ks = 0; ks < DK / 16; ++ks) {
+              const uint32_t off = (ks & 1) * 32;
+              umma_f16_ss(tmem_base + buf * 64, kd + (((ks >> 1) * (128 * 64) + off) >> 4),
+                          qd + (((ks >> 1) * (64 * 64) + off) >> 4), idesc, ks > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[buf]);
+            if constexpr (!RESQ) umma_commit(&q_empty[qs]);
+            if (g == heads - 1 && sb == nsb - 1) umma_commit(&k_empty[st]);
+          }
+          __syncwarp();
+        }
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+  } else {
+    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
+    float* srow = reinterpret_cast<float*>(smem + L::kRowOff) + warp * 256;
+    const float* win = p.win ? p.win + b * p.wi_b + h * p.wi_h : nullptr;
+    float* wout = p.wout + b * p.wo_b + h * p.wo_h;
+    bool ok = true;
+    auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+    int n = 0;
+    for (int t = t0; t < t1; ++t) {
+      const int j = t * 128 + threadIdx.x;
+      float tot = 0.f;
+      // token from which a row sees the key; whole: every row of the block does
+      const int smin = p.causal ? j - len + p.Sq : 0;
+      const int wmin = __shfl_sync(0xffffffffu, smin, 31);
+      if (ok && t < tv) {
+        const int f = first_block(t);
+        for (int g = 0; ok && g < heads; ++g)
+          for (int sb = f; sb < nsb; ++sb, ++n) {
+            // this block's rows: -lse (log2 units; -inf: adds nothing) and tokens
+            float* nz = srow + (n & 1) * 128;
+            int* tok = reinterpret_cast<int*>(nz) + 64;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = sb * 64 + lane + 32 * x;
+              const int hd = RESQ ? r / p.Sq : g, s = RESQ ? r - hd * p.Sq : r;
+              float z = -INFINITY;
+              if (RESQ ? r < rows : s < p.Sq)
+                z = p.lse[((long long)b * p.Hq + h * p.group + hd) * p.Sq + s];
+              nz[lane + 32 * x] = z == -INFINITY ? z : -z * p.lse_mul;
+              tok[lane + 32 * x] = s;
+            }
+            __syncwarp();
+            const int buf = n % SB;
+            if (!all(mbar_wait(&s_full[buf], (n / SB) & 1, 146))) { ok = false; break; }
+            tc_fence_after();
+            float s[64];
+            tmem_ld32(lane_base + buf * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
+            tmem_ld32(lane_base + buf * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
+            tmem_wait_ld();
+            tc_fence_before();
+            mbar_arrive(&s_empty[buf]);
+            const bool whole = RESQ ? wmin <= 0 : wmin <= sb * 64;
+            float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+            if (whole) {
+#pragma unroll
+              for (int c = 0; c < 64; c += 4) {
+                const float4 z = *reinterpret_cast<const float4*>(nz + c);
+                a0 = add2(a0, make_float2(fast_exp2(fmaf(s[c], p.scale_log2, z.x)),
+                                          fast_exp2(fmaf(s[c + 1], p.scale_log2, z.y))));
+                a1 = add2(a1, make_float2(fast_exp2(fmaf(s[c + 2], p.scale_log2, z.z)),
+                                          fast_exp2(fmaf(s[c + 3], p.scale_log2, z.w))));
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 64; ++c)
+                if (tok[c] >= smin) a0.x += fast_exp2(fmaf(s[c], p.scale_log2, nz[c]));
+            }
+            a0 = add2(a0, a1);
+            tot += a0.x + a0.y;  // two-level sum: a block, then the blocks
+          }
+      }
+      if (j < len) {
+        if (ok) wout[j] = (win ? win[j] : 0.f) + tot;
+      } else if (j < p.C && win != wout) {
+        wout[j] = win ? win[j] : 0.f;
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
+}
+
+template <typename DT, int DK>
+static int launch_weight_tiles(const WeightParams& w, const mi_tensor4& q, const mi_tensor4& k,
+                               cudaStream_t st) {
+  using L = ColsSmem<DK>;
+  ColsParams cp{};
+  cp.w = w;
+  cp.tiles = (w.C + 127) / 128;
+  const long long rows = (long long)w.group * w.Sq;
+  const bool resq = rows <= 64 * L::QS;
+  const long long all = (long long)w.B * w.Hkv * cp.tiles;
+  // tiles per item: with resident rows, three rounds of two items per SM;
+  // otherwise enough that an item has 16 blocks
+  const long long steps = (long long)w.group * ((w.Sq + 63) / 64);
+  long long per = resq ? (all + 148 * 6 - 1) / (148 * 6) : (16 + steps - 1) / steps;
+  cp.per = (int)(per < 1 ? 1 : (per > cp.tiles ? cp.tiles : per));
+  cp.ranges = (cp.tiles + cp.per - 1) / cp.per;
+  const long long items = (long long)w.B * w.Hkv * cp.ranges;
+  if (items > 0x7fffffffll) return MI_ERR_SHAPE;
+  CUtensorMap tk, tq;
+  memset(&tq, 0, sizeof(tq));
+  int rc = make_bnsd_map(&tk, k, w.B, w.Hkv, w.C, w.D, 32, 128);
+  if (rc == MI_OK && !resq) rc = make_bnsd_map(&tq, q, w.B, w.Hq, w.Sq, w.D, 32, 64);
+  if (rc != MI_OK) return rc;
+  auto kern = resq ? weight_tiles_kernel<DT, DK, true> : weight_tiles_kernel<DT, DK, false>;
+  cudaError_t err =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+  if (err == cudaSuccess) {
+    kern<<<(unsigned)items, 192, L::kAlloc, st>>>(tk, tq, cp);
+    err = cudaGetLastError();
+  }
+  if (err != cudaSuccess) {
+    debug_launch_failure("weight_tiles_kernel", reinterpret_cast<const void*>(kern), err, 192,
+                         L::kAlloc);
+    return MI_ERR_LAUNCH;
+  }
+  return MI_OK;
+}
+
 template <typename DT>
-static int launch_cols(const WeightParams& p, cudaStream_t st) {
+static int launch_cols(const WeightParams& p, const mi_tensor4& q, const mi_tensor4& k,
+                       cudaStream_t st) {
+  if ((long long)p.group * p.Sq > kRowsMost && p.D >= kTileMinDim) {
+    if (p.D <= 64) return launch_weight_tiles<DT, 64>(p, q, k, st);
+    if (p.D <= 96) return launch_weight_tiles<DT, 96>(p, q, k, st);
+    return launch_weight_tiles<DT, 128>(p, q, k, st);
+  }
   const long long items = (long long)p.tiles * p.Hkv * p.B;
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   if (p.D <= 64) weight_cols_kernel<DT, 64><<<(unsigned)items, 128, 0, st>>>(p);
@@ -147,7 +432,7 @@ extern "C" size_t mi_attn_weights_workspace_size(int64_t B, int64_t Hq, int64_t 
                                                  int64_t C, int64_t D, int have_lse) {
   if (!cache_sizes_ok(B, Hq, Hkv, S_q, 1, 0, C, D)) return SIZE_MAX;
   if (B == 0 || Hq == 0 || S_q == 0 || C == 0 || have_lse) return 0;
-  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, 1, 0, C);
+  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, 1, 0, C, D);
   const size_t rows = (size_t)(B * Hq * S_q);
   if ((double)rows * pl.NS > 1e13) return SIZE_MAX;
   return align_up(rows * pl.NS * 8) + align_up(rows * 4);
@@ -207,7 +492,7 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
   w.tiles = (int)((C + kColsKeys - 1) / kColsKeys);
 
   if (!lse) {
-    const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C);
+    const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C, D);
     const size_t rows = (size_t)(B * Hq * S_q);
     CacheParams p{};
     p.q = w.q;
@@ -220,6 +505,7 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
     p.Sq = w.Sq;
     p.D = w.D;
     p.scale_log2 = w.scale_log2;
+    p.seg[0].seqs = 1;
     set_seg(p.seg[1], k, k, lengths, C, B, 1, group * S_q, w.causal);
     p.seg[1].rtiles = pl.rtiles[1];
     p.seg[1].nsplit = pl.nsplit[1];
@@ -230,8 +516,15 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
                                            align_up(rows * pl.NS * 8));
     const long long items = (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1];
     if (items > 0x7fffffffll) return MI_ERR_SHAPE;
-    rc = bf ? launch_rows_dk<__nv_bfloat16, true>(p, pl.mt, items, st)
-            : launch_rows_dk<__half, true>(p, pl.mt, items, st);
+    if (pl.tile[1]) {
+      TileParams tp{};
+      tp.c = p;
+      tp.grp[1] = {1, 0, 1, pl.rtiles[1], pl.nsplit[1], pl.chunk[1] / 64, 0, items};
+      rc = launch_tiles<true>(tp, dtype, k, k, k, k, st);
+    } else {
+      rc = bf ? launch_rows_dk<__nv_bfloat16, true>(p, pl.mt, items, false, st)
+              : launch_rows_dk<__half, true>(p, pl.mt, items, false, st);
+    }
     if (rc != MI_OK) return rc;
     weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(p.ml, pl.NS, lse2,
                                                                       (long long)rows);
@@ -239,5 +532,5 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
     w.lse = lse2;
     w.lse_mul = 1.f;
   }
-  return bf ? launch_cols<__nv_bfloat16>(w, st) : launch_cols<__half>(w, st);
+  return bf ? launch_cols<__nv_bfloat16>(w, q, k, st) : launch_cols<__half>(w, q, k, st);
 }

@@ -46,10 +46,11 @@ def lengths_arg(name: str, x, n: int, cap: int, device: torch.device):
 
 
 def _aligned(x: torch.Tensor) -> bool:
-    """Rows that 16-byte loads can read (dimensions of one entry have no stride)."""
+    """Rows that 16-byte loads and tensor maps can read (dimensions of one entry
+    have no stride)."""
     if x.stride(-1) != 1 or x.data_ptr() % 16:
         return False
-    return all(x.shape[i] <= 1 or x.stride(i) % 8 == 0 for i in range(3))
+    return all(x.shape[i] <= 1 or (x.stride(i) > 0 and x.stride(i) % 8 == 0) for i in range(3))
 
 
 def rows_view(x: torch.Tensor, D: int) -> torch.Tensor:
