@@ -233,12 +233,19 @@ int mi_vs_convert_indexes(const int32_t* seqlens, const int32_t* v_idx, int64_t 
  * After the prefill: attention over a shared prefix and per-sequence caches,
  * the weight each cached key received, and eviction by weight.  No
  * counterpart functions in the reference, whose only cache attention is
- * decode_dense (minference/backend_npu/attention.py:274-293).  Views must have
- * no head table and no replicas; rows are read with 16-byte loads (unit dim
- * stride, other strides of dimensions longer than 1 multiples of 8 elements,
- * 16-byte aligned base, else MI_ERR_ALIGN; mi_evict_cache takes any
- * alignment).  Lengths are int32 device arrays, clamped to [0, capacity].
+ * decode_dense (minference/backend_npu/attention.py:274-293).  Arguments come
+ * in a struct, read by the host before the call returns; unset fields are 0.
+ * Lengths are int32 device arrays, clamped to [0, capacity].
  * ------------------------------------------------------------------------- */
+
+/* Rows of a [B, H, S, D] tensor of 16-bit elements with unit D stride: base
+ * and element strides.  The attention calls want a 16-byte aligned base and
+ * strides of dimensions longer than 1 that are positive multiples of 8
+ * elements, else MI_ERR_ALIGN; mi_evict_cache takes any. */
+typedef struct mi_rows {
+  void* ptr;
+  int64_t stride_b, stride_h, stride_s;
+} mi_rows;
 
 /* Attention of B sequences' S_q new tokens.  q/out [B, Hq, S_q, D]; prefix
  * keys and values [G, Hkv, P, D], entry b / (B/G) shared by the B/G sequences
@@ -248,16 +255,21 @@ int mi_vs_convert_indexes(const int32_t* seqlens, const int32_t* v_idx, int64_t 
  * j < lengths[b] - (S_q-1-s) if causal, j < lengths[b] otherwise (null: C).
  * A row that sees nothing gives 0 and lse -inf.  lse (null: not wanted) is
  * float [B, Hq, S_q], the natural logarithm of the sum of exp(scale q.k).
- * D is a multiple of 8, at most 128; P or C may be 0 (the views are then not
- * read).  What a cache holds past its length does not reach the result.
- * The workspace size is SIZE_MAX for sizes the call refuses. */
-size_t mi_shared_prefix_fwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t S_q,
-                                           int64_t G, int64_t P, int64_t C, int64_t D);
-int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor4 v_prefix, mi_tensor4 k,
-                         mi_tensor4 v, mi_tensor4 out, float* lse, int64_t B, int64_t Hq,
-                         int64_t Hkv, int64_t S_q, int64_t G, int64_t P, int64_t C, int64_t D,
-                         int dtype, const int32_t* prefix_lengths, const int32_t* lengths,
-                         int causal, float softmax_scale, void* workspace,
+ * D is a multiple of 8, at most 128; P or C may be 0 (the rows are then not
+ * read), P + C at most 2^30.  What a cache holds past its length does not
+ * reach the result.  The workspace (16-byte aligned) may be reused once the
+ * call's work has finished; its size is SIZE_MAX for sizes the call refuses. */
+typedef struct mi_shared_prefix_args {
+  mi_rows q, k_prefix, v_prefix, k, v, out;
+  float* lse;
+  const int32_t* prefix_lengths;
+  const int32_t* lengths;
+  int64_t B, Hq, Hkv, S_q, G, P, C, D;
+  int32_t dtype, causal;
+  float softmax_scale;
+} mi_shared_prefix_args;
+size_t mi_shared_prefix_fwd_workspace_size(const mi_shared_prefix_args* args);
+int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* workspace,
                          size_t workspace_bytes, void* stream);
 
 /* w_out[b,h,j] = w_in[b,h,j] + sum over the query heads of key/value head h and
@@ -267,13 +279,20 @@ int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor4 v_prefix,
  * whose lse is -inf adds nothing.  w_in null means 0; w_in and w_out
  * [B, Hkv, C] with unit key stride, and w_out may be w_in.  Entries past
  * lengths[b] take w_in (or 0). */
-size_t mi_attn_weights_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t S_q, int64_t C,
-                                      int64_t D, int have_lse);
-int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse, const int32_t* lengths,
-                    const float* w_in, int64_t w_in_stride_b, int64_t w_in_stride_h,
-                    float* w_out, int64_t w_out_stride_b, int64_t w_out_stride_h, int64_t B,
-                    int64_t Hq, int64_t Hkv, int64_t S_q, int64_t C, int64_t D, int dtype,
-                    int causal, float softmax_scale, void* workspace, size_t workspace_bytes,
+typedef struct mi_attn_weights_args {
+  mi_rows q, k;
+  const float* lse;
+  const int32_t* lengths;
+  const float* w_in;
+  int64_t w_in_stride_b, w_in_stride_h;
+  float* w_out;
+  int64_t w_out_stride_b, w_out_stride_h;
+  int64_t B, Hq, Hkv, S_q, C, D;
+  int32_t dtype, causal;
+  float softmax_scale;
+} mi_attn_weights_args;
+size_t mi_attn_weights_workspace_size(const mi_attn_weights_args* args);
+int mi_attn_weights(const mi_attn_weights_args* args, void* workspace, size_t workspace_bytes,
                     void* stream);
 
 /* Keeps min(n, keep) rows of every (b, h) of a cache with n = lengths[b]
@@ -284,13 +303,20 @@ int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse, const int32_t*
  * from and new_lengths [B] how many there are.  Past new_lengths, index is -1
  * and rows and weights are 0.  sink + recent <= keep.  Outputs must not overlap
  * the inputs.  16-bit elements of either type; D at most 1024. */
-size_t mi_evict_cache_workspace_size(int64_t B, int64_t H, int64_t C);
-int mi_evict_cache(mi_tensor4 k, mi_tensor4 v, const float* weights, int64_t weights_stride_b,
-                   int64_t weights_stride_h, mi_tensor4 k_out, mi_tensor4 v_out,
-                   float* weights_out, int64_t weights_out_stride_b,
-                   int64_t weights_out_stride_h, int32_t* index, int32_t* new_lengths, int64_t B,
-                   int64_t H, int64_t C, int64_t D, int64_t keep, int64_t sink, int64_t recent,
-                   const int32_t* lengths, void* workspace, size_t workspace_bytes,
+typedef struct mi_evict_args {
+  mi_rows k, v;
+  const float* weights;
+  int64_t weights_stride_b, weights_stride_h;
+  mi_rows k_out, v_out;
+  float* weights_out;
+  int64_t weights_out_stride_b, weights_out_stride_h;
+  int32_t* index;
+  int32_t* new_lengths;
+  const int32_t* lengths;
+  int64_t B, H, C, D, keep, sink, recent;
+} mi_evict_args;
+size_t mi_evict_cache_workspace_size(const mi_evict_args* args);
+int mi_evict_cache(const mi_evict_args* args, void* workspace, size_t workspace_bytes,
                    void* stream);
 
 #ifdef __cplusplus

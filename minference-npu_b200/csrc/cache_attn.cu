@@ -464,15 +464,14 @@ static bool cache_sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64
   return B <= lim && Hq <= lim && Sq <= lim && B * Hq <= lim && B * Hq * Sq <= lim;
 }
 
-// A view that 16-byte loads and tensor maps can read; the strides of dimensions
+// Rows that 16-byte loads and tensor maps can read; the strides of dimensions
 // of one entry are not looked at.
-static int cache_view_ok(const mi_tensor4& t, int64_t n0, int64_t n1, int64_t n2) {
-  if (t.head_index || t.n_replica) return MI_ERR_SHAPE;
-  if (t.stride_d != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15)) return MI_ERR_ALIGN;
+static bool rows_ok(const mi_rows& t, int64_t n0, int64_t n1, int64_t n2) {
+  if (!t.ptr || (reinterpret_cast<uintptr_t>(t.ptr) & 15)) return false;
   const int64_t n[3] = {n0, n1, n2}, s[3] = {t.stride_b, t.stride_h, t.stride_s};
   for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return MI_ERR_ALIGN;
-  return MI_OK;
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8)) return false;
+  return true;
 }
 
 template <typename K, typename... A>
@@ -496,11 +495,11 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
 template <typename DT, int DK, int MT, bool STATS>
 static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
   using L = RowsSmem<DK, STATS>;
-  auto kern = cache_rows_kernel<DT, DK, MT, STATS>;
+  constexpr auto kern = cache_rows_kernel<DT, DK, MT, STATS>;
   constexpr int kJoin = STATS ? 0 : kRowsWarps * 16 * MT * (DK + 4) * 4;
   constexpr int kQ = 16 * MT * L::kPitch;
   constexpr int bytes = L::kRing > kJoin ? (L::kRing > kQ ? L::kRing : kQ) : kJoin;
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, MT, STATS>>(bytes);
   if (err == cudaSuccess) {
     if (after) {
       err = launch_after(kern, dim3((unsigned)items), 32 * kRowsWarps, bytes, stream, p);
@@ -530,7 +529,7 @@ static int launch_rows_dk(const CacheParams& p, int mt, long long items, bool af
                  : launch_rows<DT, 128, 2, STATS>(p, items, after, st);
 }
 
-static void set_seg(CacheSeg& s, const mi_tensor4& k, const mi_tensor4& v, const int32_t* len,
+static void set_seg(CacheSeg& s, const mi_rows& k, const mi_rows& v, const int32_t* len,
                     int64_t cap, int64_t nb, int64_t seqs, int64_t rows, int causal) {
   s.k = static_cast<const uint16_t*>(k.ptr);
   s.v = static_cast<const uint16_t*>(v.ptr);
@@ -552,64 +551,55 @@ static void set_seg(CacheSeg& s, const mi_tensor4& k, const mi_tensor4& v, const
 
 using namespace mib200;
 
-extern "C" size_t mi_shared_prefix_fwd_workspace_size(int64_t B, int64_t Hq, int64_t Hkv,
-                                                      int64_t S_q, int64_t G, int64_t P,
-                                                      int64_t C, int64_t D) {
-  if (!cache_sizes_ok(B, Hq, Hkv, S_q, G, P, C, D)) return SIZE_MAX;
-  if (B == 0 || Hq == 0 || S_q == 0) return 0;
-  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, G, P, C, D);
+extern "C" size_t mi_shared_prefix_fwd_workspace_size(const mi_shared_prefix_args* a) {
+  if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, a->G, a->P, a->C, a->D)) return SIZE_MAX;
+  if (a->B == 0 || a->Hq == 0 || a->S_q == 0) return 0;
+  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C, a->D);
   if (pl.NS == 1) return 0;
-  const double need = (double)B * Hq * S_q * pl.NS * (D * 4 + 8);
+  const double need = (double)a->B * a->Hq * a->S_q * pl.NS * (a->D * 4 + 8);
   if (need > 1e15) return SIZE_MAX;
-  const size_t slots = (size_t)(B * Hq * S_q) * pl.NS;
-  return align_up(slots * D * 4) + align_up(slots * 8);
+  const size_t slots = (size_t)(a->B * a->Hq * a->S_q) * pl.NS;
+  return align_up(slots * a->D * 4) + align_up(slots * 8);
 }
 
-extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor4 v_prefix,
-                                    mi_tensor4 k, mi_tensor4 v, mi_tensor4 out, float* lse,
-                                    int64_t B, int64_t Hq, int64_t Hkv, int64_t S_q, int64_t G,
-                                    int64_t P, int64_t C, int64_t D, int dtype,
-                                    const int32_t* prefix_lengths, const int32_t* lengths,
-                                    int causal, float softmax_scale, void* workspace,
+extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* workspace,
                                     size_t workspace_bytes, void* stream) {
-  if (dtype != MI_F16 && dtype != MI_BF16) return MI_ERR_DTYPE;
+  if (!args) return MI_ERR_SHAPE;
+  const mi_shared_prefix_args& a = *args;
+  const int64_t B = a.B, Hq = a.Hq, Hkv = a.Hkv, S_q = a.S_q, G = a.G, P = a.P, C = a.C, D = a.D;
+  if (a.dtype != MI_F16 && a.dtype != MI_BF16) return MI_ERR_DTYPE;
   if (!cache_sizes_ok(B, Hq, Hkv, S_q, G, P, C, D)) return MI_ERR_SHAPE;
   if (B == 0 || Hq == 0 || S_q == 0) return MI_OK;
-  int rc;
-  if ((rc = cache_view_ok(q, B, Hq, S_q)) != MI_OK) return rc;
-  if ((rc = cache_view_ok(out, B, Hq, S_q)) != MI_OK) return rc;
-  if (P && ((rc = cache_view_ok(k_prefix, G, Hkv, P)) != MI_OK ||
-            (rc = cache_view_ok(v_prefix, G, Hkv, P)) != MI_OK))
-    return rc;
-  if (C && ((rc = cache_view_ok(k, B, Hkv, C)) != MI_OK ||
-            (rc = cache_view_ok(v, B, Hkv, C)) != MI_OK))
-    return rc;
+  if (!rows_ok(a.q, B, Hq, S_q) || !rows_ok(a.out, B, Hq, S_q)) return MI_ERR_ALIGN;
+  if (P && (!rows_ok(a.k_prefix, G, Hkv, P) || !rows_ok(a.v_prefix, G, Hkv, P)))
+    return MI_ERR_ALIGN;
+  if (C && (!rows_ok(a.k, B, Hkv, C) || !rows_ok(a.v, B, Hkv, C))) return MI_ERR_ALIGN;
   const int64_t group = Hq / Hkv;
   const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C, D);
-  const size_t need = mi_shared_prefix_fwd_workspace_size(B, Hq, Hkv, S_q, G, P, C, D);
+  const size_t need = mi_shared_prefix_fwd_workspace_size(args);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||
                (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return MI_ERR_WORKSPACE;
 
   CacheParams p{};
-  p.q = static_cast<const uint16_t*>(q.ptr);
-  p.qs_b = q.stride_b;
-  p.qs_h = q.stride_h;
-  p.qs_s = q.stride_s;
-  p.out = static_cast<uint16_t*>(out.ptr);
-  p.os_b = out.stride_b;
-  p.os_h = out.stride_h;
-  p.os_s = out.stride_s;
-  p.lse = lse;
+  p.q = static_cast<const uint16_t*>(a.q.ptr);
+  p.qs_b = a.q.stride_b;
+  p.qs_h = a.q.stride_h;
+  p.qs_s = a.q.stride_s;
+  p.out = static_cast<uint16_t*>(a.out.ptr);
+  p.os_b = a.out.stride_b;
+  p.os_h = a.out.stride_h;
+  p.os_s = a.out.stride_s;
+  p.lse = a.lse;
   p.Hq = (int)Hq;
   p.Hkv = (int)Hkv;
   p.group = (int)group;
   p.Sq = (int)S_q;
   p.D = (int)D;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  set_seg(p.seg[0], k_prefix, v_prefix, prefix_lengths, P, G, B / G, B / G * group * S_q, 0);
-  set_seg(p.seg[1], k, v, lengths, C, B, 1, group * S_q, causal ? 1 : 0);
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  set_seg(p.seg[0], a.k_prefix, a.v_prefix, a.prefix_lengths, P, G, B / G, B / G * group * S_q, 0);
+  set_seg(p.seg[1], a.k, a.v, a.lengths, C, B, 1, group * S_q, a.causal ? 1 : 0);
   for (int s = 0; s < 2; ++s) {
     p.seg[s].rtiles = pl.rtiles[s];
     p.seg[s].nsplit = pl.nsplit[s];
@@ -626,7 +616,7 @@ extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor
                               (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1]};
   if (items[0] + items[1] > 0x7fffffffll) return MI_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf = dtype == MI_BF16;
+  const bool bf = a.dtype == MI_BF16;
   TileParams tp{};
   long long rows_items = 0;
   for (int s = 0; s < 2; ++s) {
@@ -647,13 +637,13 @@ extern "C" int mi_shared_prefix_fwd(mi_tensor4 q, mi_tensor4 k_prefix, mi_tensor
   const bool tiles = pl.tile[0] || pl.tile[1];
   if (tiles) {
     tp.c = p;
-    rc = launch_tiles<false>(tp, dtype, k_prefix, v_prefix, k, v, st);
+    const int rc = launch_tiles<false>(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, st);
     if (rc != MI_OK) return rc;
   }
   if (rows_items) {
     p.items0 = pl.tile[0] ? 0 : items[0];
-    rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, rows_items, tiles, st)
-            : launch_rows_dk<__half, false>(p, pl.mt, rows_items, tiles, st);
+    const int rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, rows_items, tiles, st)
+                      : launch_rows_dk<__half, false>(p, pl.mt, rows_items, tiles, st);
     if (rc != MI_OK) return rc;
   }
   if (p.NS == 1) return MI_OK;

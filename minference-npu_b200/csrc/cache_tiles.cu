@@ -443,24 +443,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 }
 
 template <typename DT, int DK, bool STATS>
-static int launch_tiles_t(const TileParams& tp, const mi_tensor4& kp, const mi_tensor4& vp,
-                          const mi_tensor4& k, const mi_tensor4& v, cudaStream_t st) {
+static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows& vp,
+                          const mi_rows& k, const mi_rows& v, cudaStream_t st) {
   using L = TileSmem<DK, STATS>;
   const CacheParams& p = tp.c;
   CUtensorMap m[4];
   memset(m, 0, sizeof(m));
-  const mi_tensor4* t[4] = {&kp, &vp, &k, &v};
+  const mi_rows* t[4] = {&kp, &vp, &k, &v};
   const bool use0 = (tp.grp[0].items && tp.grp[0].use0) || (tp.grp[1].items && tp.grp[1].use0);
   const bool use1 = (tp.grp[0].items && tp.grp[0].use1) || (tp.grp[1].items && tp.grp[1].use1);
   for (int i = 0; i < 4; ++i) {
     if (!(i < 2 ? use0 : use1) || (STATS && (i & 1))) continue;
     const CacheSeg& s = p.seg[i / 2];
-    const int rc = make_bnsd_map(&m[i], *t[i], s.nb, p.Hkv, s.cap, p.D, 32, 64);
+    const int rc = make_rows4_map(&m[i], *t[i], s.nb, p.Hkv, s.cap, p.D, 32, 64);
     if (rc != MI_OK) return rc;
   }
-  auto kern = cache_tiles_kernel<DT, DK, STATS>;
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         L::kAlloc);
+  constexpr auto kern = cache_tiles_kernel<DT, DK, STATS>;
+  cudaError_t err = allow_smem<cache_tiles_kernel<DT, DK, STATS>>(L::kAlloc);
   if (err == cudaSuccess) {
     kern<<<(unsigned)(tp.grp[0].items + tp.grp[1].items), kTileThreads, L::kAlloc, st>>>(
         m[0], m[1], m[2], m[3], tp);
@@ -475,9 +474,8 @@ static int launch_tiles_t(const TileParams& tp, const mi_tensor4& kp, const mi_t
 }
 
 template <bool STATS>
-static int launch_tiles(const TileParams& tp, int dtype, const mi_tensor4& kp,
-                        const mi_tensor4& vp, const mi_tensor4& k, const mi_tensor4& v,
-                        cudaStream_t st) {
+static int launch_tiles(const TileParams& tp, int dtype, const mi_rows& kp, const mi_rows& vp,
+                        const mi_rows& k, const mi_rows& v, cudaStream_t st) {
   const bool bf = dtype == MI_BF16;
   const int D = tp.c.D;
   if (D <= 64)

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(192, 2)
 }
 
 template <typename DT, int DK>
-static int launch_weight_tiles(const WeightParams& w, const mi_tensor4& q, const mi_tensor4& k,
+static int launch_weight_tiles(const WeightParams& w, const mi_rows& q, const mi_rows& k,
                                cudaStream_t st) {
   using L = ColsSmem<DK>;
   ColsParams cp{};
@@ -390,12 +390,12 @@ static int launch_weight_tiles(const WeightParams& w, const mi_tensor4& q, const
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   CUtensorMap tk, tq;
   memset(&tq, 0, sizeof(tq));
-  int rc = make_bnsd_map(&tk, k, w.B, w.Hkv, w.C, w.D, 32, 128);
-  if (rc == MI_OK && !resq) rc = make_bnsd_map(&tq, q, w.B, w.Hq, w.Sq, w.D, 32, 64);
+  int rc = make_rows4_map(&tk, k, w.B, w.Hkv, w.C, w.D, 32, 128);
+  if (rc == MI_OK && !resq) rc = make_rows4_map(&tq, q, w.B, w.Hq, w.Sq, w.D, 32, 64);
   if (rc != MI_OK) return rc;
   auto kern = resq ? weight_tiles_kernel<DT, DK, true> : weight_tiles_kernel<DT, DK, false>;
-  cudaError_t err =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+  cudaError_t err = resq ? allow_smem<weight_tiles_kernel<DT, DK, true>>(L::kAlloc)
+                         : allow_smem<weight_tiles_kernel<DT, DK, false>>(L::kAlloc);
   if (err == cudaSuccess) {
     kern<<<(unsigned)items, 192, L::kAlloc, st>>>(tk, tq, cp);
     err = cudaGetLastError();
@@ -409,7 +409,7 @@ static int launch_weight_tiles(const WeightParams& w, const mi_tensor4& q, const
 }
 
 template <typename DT>
-static int launch_cols(const WeightParams& p, const mi_tensor4& q, const mi_tensor4& k,
+static int launch_cols(const WeightParams& p, const mi_rows& q, const mi_rows& k,
                        cudaStream_t st) {
   if ((long long)p.group * p.Sq > kRowsMost && p.D >= kTileMinDim) {
     if (p.D <= 64) return launch_weight_tiles<DT, 64>(p, q, k, st);
@@ -428,39 +428,39 @@ static int launch_cols(const WeightParams& p, const mi_tensor4& q, const mi_tens
 
 using namespace mib200;
 
-extern "C" size_t mi_attn_weights_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t S_q,
-                                                 int64_t C, int64_t D, int have_lse) {
-  if (!cache_sizes_ok(B, Hq, Hkv, S_q, 1, 0, C, D)) return SIZE_MAX;
-  if (B == 0 || Hq == 0 || S_q == 0 || C == 0 || have_lse) return 0;
-  const CachePlan pl = cache_plan(B, Hkv, Hq / Hkv, S_q, 1, 0, C, D);
-  const size_t rows = (size_t)(B * Hq * S_q);
+extern "C" size_t mi_attn_weights_workspace_size(const mi_attn_weights_args* a) {
+  if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, 1, 0, a->C, a->D)) return SIZE_MAX;
+  if (a->B == 0 || a->Hq == 0 || a->S_q == 0 || a->C == 0 || a->lse) return 0;
+  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, 1, 0, a->C, a->D);
+  const size_t rows = (size_t)(a->B * a->Hq * a->S_q);
   if ((double)rows * pl.NS > 1e13) return SIZE_MAX;
   return align_up(rows * pl.NS * 8) + align_up(rows * 4);
 }
 
-extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
-                               const int32_t* lengths, const float* w_in, int64_t w_in_stride_b,
-                               int64_t w_in_stride_h, float* w_out, int64_t w_out_stride_b,
-                               int64_t w_out_stride_h, int64_t B, int64_t Hq, int64_t Hkv,
-                               int64_t S_q, int64_t C, int64_t D, int dtype, int causal,
-                               float softmax_scale, void* workspace, size_t workspace_bytes,
-                               void* stream) {
+extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (!args) return MI_ERR_SHAPE;
+  const mi_attn_weights_args& a = *args;
+  const int64_t B = a.B, Hq = a.Hq, Hkv = a.Hkv, S_q = a.S_q, C = a.C, D = a.D;
+  const int dtype = a.dtype;
+  const float* lse = a.lse;
+  const int32_t* lengths = a.lengths;
+  const mi_rows &q = a.q, &k = a.k;
   if (dtype != MI_F16 && dtype != MI_BF16) return MI_ERR_DTYPE;
   if (!cache_sizes_ok(B, Hq, Hkv, S_q, 1, 0, C, D)) return MI_ERR_SHAPE;
   if (B == 0 || C == 0) return MI_OK;
   if (Hq == 0 || S_q == 0) return MI_ERR_SHAPE;  // no rows: nothing to add
-  if (!w_out) return MI_ERR_SHAPE;
-  int rc;
-  if ((rc = cache_view_ok(q, B, Hq, S_q)) != MI_OK) return rc;
-  if ((rc = cache_view_ok(k, B, Hkv, C)) != MI_OK) return rc;
+  if (!a.w_out) return MI_ERR_SHAPE;
+  if (!rows_ok(q, B, Hq, S_q) || !rows_ok(k, B, Hkv, C)) return MI_ERR_ALIGN;
   const int64_t group = Hq / Hkv;
-  const size_t need = mi_attn_weights_workspace_size(B, Hq, Hkv, S_q, C, D, lse != nullptr);
+  const size_t need = mi_attn_weights_workspace_size(args);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||
                (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return MI_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = dtype == MI_BF16;
+  int rc;
 
   WeightParams w{};
   w.q = static_cast<const uint16_t*>(q.ptr);
@@ -474,12 +474,12 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
   w.len = lengths;
   w.lse = lse;
   w.lse_mul = 1.4426950408889634f;
-  w.win = w_in;
-  w.wi_b = w_in_stride_b;
-  w.wi_h = w_in_stride_h;
-  w.wout = w_out;
-  w.wo_b = w_out_stride_b;
-  w.wo_h = w_out_stride_h;
+  w.win = a.w_in;
+  w.wi_b = a.w_in_stride_b;
+  w.wi_h = a.w_in_stride_h;
+  w.wout = a.w_out;
+  w.wo_b = a.w_out_stride_b;
+  w.wo_h = a.w_out_stride_h;
   w.B = (int)B;
   w.Hq = (int)Hq;
   w.Hkv = (int)Hkv;
@@ -487,8 +487,8 @@ extern "C" int mi_attn_weights(mi_tensor4 q, mi_tensor4 k, const float* lse,
   w.Sq = (int)S_q;
   w.C = (int)C;
   w.D = (int)D;
-  w.causal = causal ? 1 : 0;
-  w.scale_log2 = softmax_scale * 1.4426950408889634f;
+  w.causal = a.causal ? 1 : 0;
+  w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   w.tiles = (int)((C + kColsKeys - 1) / kColsKeys);
 
   if (!lse) {

@@ -127,8 +127,7 @@ static int launch_select(const EvictParams& p, int64_t BH, cudaStream_t st) {
   auto kern = evict_select_kernel<CL>;
   const int64_t seg = ((p.C + CL - 1) / CL + 31) & ~31ll;
   const int bytes = p.keys ? 0 : (int)(seg * 4);
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kEvictSegKeys * 4);
+  cudaError_t err = allow_smem<evict_select_kernel<CL>>(kEvictSegKeys * 4);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(BH * CL));
   cfg.blockDim = dim3(kEvictThreads);
@@ -151,7 +150,7 @@ static int launch_select(const EvictParams& p, int64_t BH, cudaStream_t st) {
 }
 
 // 16-byte rows: base and the strides of dimensions with more than one entry.
-static bool wide_rows(const mi_tensor4& t, int64_t n0, int64_t n1, int64_t n2) {
+static bool wide_rows(const mi_rows& t, int64_t n0, int64_t n1, int64_t n2) {
   return !(reinterpret_cast<uintptr_t>(t.ptr) & 15) && (n0 <= 1 || t.stride_b % 8 == 0) &&
          (n1 <= 1 || t.stride_h % 8 == 0) && (n2 <= 1 || t.stride_s % 8 == 0);
 }
@@ -160,45 +159,40 @@ static bool wide_rows(const mi_tensor4& t, int64_t n0, int64_t n1, int64_t n2) {
 
 using namespace mib200;
 
-extern "C" size_t mi_evict_cache_workspace_size(int64_t B, int64_t H, int64_t C) {
-  if (!evict_sizes_ok(B, H, C, 8, 1)) return SIZE_MAX;
-  return C > 8ll * kEvictSegKeys ? align_up((size_t)(B * H) * C * 4) : 0;
+extern "C" size_t mi_evict_cache_workspace_size(const mi_evict_args* a) {
+  if (!a || !evict_sizes_ok(a->B, a->H, a->C, a->D, a->keep)) return SIZE_MAX;
+  return a->C > 8ll * kEvictSegKeys ? align_up((size_t)(a->B * a->H) * a->C * 4) : 0;
 }
 
-extern "C" int mi_evict_cache(mi_tensor4 k, mi_tensor4 v, const float* weights,
-                              int64_t weights_stride_b, int64_t weights_stride_h,
-                              mi_tensor4 k_out, mi_tensor4 v_out, float* weights_out,
-                              int64_t weights_out_stride_b, int64_t weights_out_stride_h,
-                              int32_t* index, int32_t* new_lengths, int64_t B, int64_t H,
-                              int64_t C, int64_t D, int64_t keep, int64_t sink, int64_t recent,
-                              const int32_t* lengths, void* workspace, size_t workspace_bytes,
+extern "C" int mi_evict_cache(const mi_evict_args* args, void* workspace, size_t workspace_bytes,
                               void* stream) {
+  if (!args) return MI_ERR_SHAPE;
+  const mi_evict_args& a = *args;
+  const int64_t B = a.B, H = a.H, C = a.C, D = a.D, keep = a.keep;
   if (!evict_sizes_ok(B, H, C, D, keep)) return MI_ERR_SHAPE;
-  if (sink < 0 || recent < 0 || sink > keep || recent > keep || sink + recent > keep)
+  if (a.sink < 0 || a.recent < 0 || a.sink > keep || a.recent > keep || a.sink + a.recent > keep)
     return MI_ERR_SHAPE;
-  for (const mi_tensor4* t : {&k, &v, &k_out, &v_out}) {
-    if (t->head_index || t->n_replica) return MI_ERR_SHAPE;
-    if (t->stride_d != 1 && D > 1) return MI_ERR_ALIGN;
-  }
   if (B == 0 || H == 0) return MI_OK;
-  if (!index || !new_lengths || !weights_out || (C && !weights)) return MI_ERR_SHAPE;
-  const size_t need = mi_evict_cache_workspace_size(B, H, C);
+  if (!a.index || !a.new_lengths || !a.weights_out || !a.k_out.ptr || !a.v_out.ptr ||
+      (C && (!a.weights || !a.k.ptr || !a.v.ptr)))
+    return MI_ERR_SHAPE;
+  const size_t need = mi_evict_cache_workspace_size(args);
   if (need && (!workspace || workspace_bytes < need ||
                (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return MI_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   EvictParams p{};
-  p.w = weights;
-  p.w_b = weights_stride_b;
-  p.w_h = weights_stride_h;
-  p.len = lengths;
+  p.w = a.weights;
+  p.w_b = a.weights_stride_b;
+  p.w_h = a.weights_stride_h;
+  p.len = a.lengths;
   p.H = (int)H;
   p.C = (int)C;
   p.keep = (int)keep;
-  p.sink = (int)sink;
-  p.recent = (int)recent;
-  p.index = index;
-  p.new_len = new_lengths;
+  p.sink = (int)a.sink;
+  p.recent = (int)a.recent;
+  p.index = a.index;
+  p.new_len = a.new_lengths;
   p.keys = need ? static_cast<uint32_t*>(workspace) : nullptr;
   const int cl = evict_cluster(B * H, C);
   int rc = cl == 1   ? launch_select<1>(p, B * H, st)
@@ -208,27 +202,27 @@ extern "C" int mi_evict_cache(mi_tensor4 k, mi_tensor4 v, const float* weights,
   if (rc != MI_OK) return rc;
 
   MoveParams m{};
-  m.k = static_cast<const uint16_t*>(k.ptr);
-  m.v = static_cast<const uint16_t*>(v.ptr);
-  m.ks_b = k.stride_b, m.ks_h = k.stride_h, m.ks_s = k.stride_s;
-  m.vs_b = v.stride_b, m.vs_h = v.stride_h, m.vs_s = v.stride_s;
-  m.w = weights;
-  m.w_b = weights_stride_b, m.w_h = weights_stride_h;
-  m.ko = static_cast<uint16_t*>(k_out.ptr);
-  m.vo = static_cast<uint16_t*>(v_out.ptr);
-  m.ko_b = k_out.stride_b, m.ko_h = k_out.stride_h, m.ko_s = k_out.stride_s;
-  m.vo_b = v_out.stride_b, m.vo_h = v_out.stride_h, m.vo_s = v_out.stride_s;
-  m.wo = weights_out;
-  m.wo_b = weights_out_stride_b, m.wo_h = weights_out_stride_h;
-  m.index = index;
+  m.k = static_cast<const uint16_t*>(a.k.ptr);
+  m.v = static_cast<const uint16_t*>(a.v.ptr);
+  m.ks_b = a.k.stride_b, m.ks_h = a.k.stride_h, m.ks_s = a.k.stride_s;
+  m.vs_b = a.v.stride_b, m.vs_h = a.v.stride_h, m.vs_s = a.v.stride_s;
+  m.w = a.weights;
+  m.w_b = a.weights_stride_b, m.w_h = a.weights_stride_h;
+  m.ko = static_cast<uint16_t*>(a.k_out.ptr);
+  m.vo = static_cast<uint16_t*>(a.v_out.ptr);
+  m.ko_b = a.k_out.stride_b, m.ko_h = a.k_out.stride_h, m.ko_s = a.k_out.stride_s;
+  m.vo_b = a.v_out.stride_b, m.vo_h = a.v_out.stride_h, m.vo_s = a.v_out.stride_s;
+  m.wo = a.weights_out;
+  m.wo_b = a.weights_out_stride_b, m.wo_h = a.weights_out_stride_h;
+  m.index = a.index;
   m.H = (int)H;
   m.D = (int)D;
   m.keep = (int)keep;
   m.tiles = (int)((keep + kMoveRows - 1) / kMoveRows);
   const long long blocks = (long long)B * H * m.tiles;
   if (blocks > 0x7fffffffll) return MI_ERR_SHAPE;
-  const bool wide = D % 8 == 0 && wide_rows(k, B, H, C) && wide_rows(v, B, H, C) &&
-                    wide_rows(k_out, B, H, keep) && wide_rows(v_out, B, H, keep);
+  const bool wide = D % 8 == 0 && wide_rows(a.k, B, H, C) && wide_rows(a.v, B, H, C) &&
+                    wide_rows(a.k_out, B, H, keep) && wide_rows(a.v_out, B, H, keep);
   if (wide) evict_move_kernel<uint4><<<(unsigned)blocks, 256, 0, st>>>(m);
   else evict_move_kernel<uint16_t><<<(unsigned)blocks, 256, 0, st>>>(m);
   return cudaGetLastError() == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;

@@ -4,6 +4,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 
@@ -103,6 +104,32 @@ inline void debug_launch_failure(const char* name, const void* func, cudaError_t
           "max threads %d, static smem %zu, local %zu)\n",
           name, cudaGetErrorString(err), threads, smem_bytes, fa.numRegs, fa.maxThreadsPerBlock,
           fa.sharedSizeBytes, fa.localSizeBytes);
+}
+
+// Raises a kernel's shared-memory limit once per device (the call costs about
+// as much as a launch's arguments).
+template <auto Kern>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (err != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return err;
+  err = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
+}
+
+// 4-D map of a [B, H, S, D] tensor given by its rows (see make_bnsd_map).
+inline int make_rows4_map(CUtensorMap* map, const mi_rows& r, int64_t B, int64_t H, int64_t S,
+                          int64_t D, int box_d, int box_s) {
+  mi_tensor4 t{};
+  t.ptr = r.ptr;
+  t.stride_b = r.stride_b;
+  t.stride_h = r.stride_h;
+  t.stride_s = r.stride_s;
+  t.stride_d = 1;
+  return make_bnsd_map(map, t, B, H, S, D, box_d, box_s);
 }
 
 }  // namespace mib200

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -48,6 +49,14 @@ class mi_tensor4(ctypes.Structure):
         ("replica", ctypes.POINTER(ctypes.c_void_p)),
         ("n_replica", ctypes.c_int64),
     ]
+
+
+# Layouts of the argument structs of the cache entry points (include/minference_b200.h).
+# One packed bytes object costs a tenth of the ctypes structures it replaces,
+# which matters where a decode step takes a few microseconds.
+SHARED_PREFIX_ARGS = struct.Struct("=24q3q8qiif4x")
+ATTN_WEIGHTS_ARGS = struct.Struct("=8q3q2q1q2q6qiif4x")
+EVICT_ARGS = struct.Struct("=8q3q8q3q3q7q")
 
 
 def library_path() -> str:
@@ -104,20 +113,12 @@ def lib() -> ctypes.CDLL:
         L.mi_vs_sparse_fwd_rows.restype = I
         L.mi_vs_convert_indexes.argtypes = [P, P, I64, P, I64, I64, I64, I64, P, P, P, P, P]
         L.mi_vs_convert_indexes.restype = I
-        L.mi_shared_prefix_fwd_workspace_size.argtypes = [I64] * 8
-        L.mi_shared_prefix_fwd_workspace_size.restype = SZ
-        L.mi_shared_prefix_fwd.argtypes = [T4] * 6 + [P] + [I64] * 8 + [I, P, P, I, F, P, SZ, P]
-        L.mi_shared_prefix_fwd.restype = I
-        L.mi_attn_weights_workspace_size.argtypes = [I64] * 6 + [I]
-        L.mi_attn_weights_workspace_size.restype = SZ
-        L.mi_attn_weights.argtypes = ([T4, T4, P, P, P, I64, I64, P, I64, I64] + [I64] * 6
-                                      + [I, I, F, P, SZ, P])
-        L.mi_attn_weights.restype = I
-        L.mi_evict_cache_workspace_size.argtypes = [I64] * 3
-        L.mi_evict_cache_workspace_size.restype = SZ
-        L.mi_evict_cache.argtypes = ([T4, T4, P, I64, I64, T4, T4, P, I64, I64, P, P]
-                                     + [I64] * 7 + [P, P, SZ, P])
-        L.mi_evict_cache.restype = I
+        # argument structs (the *_ARGS layouts below), packed as bytes
+        for name in ("mi_shared_prefix_fwd", "mi_attn_weights", "mi_evict_cache"):
+            size = getattr(L, name + "_workspace_size")
+            size.argtypes, size.restype = [ctypes.c_char_p], SZ
+            getattr(L, name).argtypes = [ctypes.c_char_p, P, SZ, P]
+            getattr(L, name).restype = I
         _lib = L
     return _lib
 
@@ -164,6 +165,28 @@ def require_cuda(*ts: torch.Tensor) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_packed(name: str, args: bytes, device: torch.device) -> None:
+    """Workspace and launch of a cache entry point on the device's current stream."""
+    L = lib()
+    need = getattr(L, name + "_workspace_size")(args)
+    if need > 1 << 62:
+        raise ValueError(f"{name}: sizes not supported")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call_packed(name, args, device)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = getattr(L, name)(args, ws.data_ptr(), need, _raw_stream(device.index))
+    else:
+        rc = getattr(L, name)(args, None, 0, _raw_stream(device.index))
+    if rc != MI_OK:
+        check(rc, name)
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

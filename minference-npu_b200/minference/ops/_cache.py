@@ -10,55 +10,64 @@ from .. import _native
 MAX_HEAD_DIM = 128
 
 
+_DTYPES = {torch.float16: _native.MI_F16, torch.bfloat16: _native.MI_BF16}
+
+
 def check_same(name: str, x: torch.Tensor, like: torch.Tensor, shape: tuple) -> None:
     """`x` has the given shape and `like`'s dtype and device."""
-    if not isinstance(x, torch.Tensor) or tuple(x.shape) != tuple(shape):
+    if not isinstance(x, torch.Tensor) or x.shape != shape:
         got = tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__
         raise ValueError(f"{name} must be {tuple(shape)}, got {got}")
-    if x.dtype != like.dtype:
+    if x.dtype is not like.dtype:
         raise TypeError(f"{name} is {x.dtype}, expected {like.dtype}")
     if x.device != like.device:
         raise ValueError(f"{name} is on {x.device}, expected {like.device}")
 
 
-def check_query(q: torch.Tensor, Hkv: int) -> None:
+def check_query(q: torch.Tensor, Hkv: int) -> int:
+    """dtype code of q."""
     _native.require_cuda(q)
-    _native.dtype_code(q)
+    code = _DTYPES.get(q.dtype)
+    if code is None:
+        code = _native.dtype_code(q)  # raises
     if Hkv < 1 or q.shape[1] % Hkv:
         raise ValueError(f"{q.shape[1]} query heads over {Hkv} key/value heads")
-    if not 1 <= q.shape[-1] <= MAX_HEAD_DIM:
+    if not 1 <= q.shape[3] <= MAX_HEAD_DIM:
         raise NotImplementedError(
-            f"head_dim={q.shape[-1]}: the sm_100a kernels take 1 to {MAX_HEAD_DIM}")
+            f"head_dim={q.shape[3]}: the sm_100a kernels take 1 to {MAX_HEAD_DIM}")
+    return code
 
 
 def lengths_arg(name: str, x, n: int, cap: int, device: torch.device):
-    """int32 device tensor [n] of valid rows, or None (every row)."""
-    if x is None:
-        return None
+    """int32 device tensor [n] of valid rows."""
     if not isinstance(x, torch.Tensor) or x.dtype.is_floating_point or x.dtype.is_complex \
             or x.dtype == torch.bool:
         raise TypeError(f"{name} must be an integer tensor")
-    if tuple(x.shape) != (n,):
+    if x.shape != (n,):
         raise ValueError(f"{name} must be ({n},), got {tuple(x.shape)}")
-    if x.dtype != torch.int32:
+    if x.dtype is not torch.int32:
         x = x.clamp(0, cap).to(torch.int32)
-    return x.to(device).contiguous()
+    if x.device != device:
+        x = x.to(device)
+    return x.contiguous()
 
 
-def _aligned(x: torch.Tensor) -> bool:
-    """Rows that 16-byte loads and tensor maps can read (dimensions of one entry
-    have no stride)."""
-    if x.stride(-1) != 1 or x.data_ptr() % 16:
-        return False
-    return all(x.shape[i] <= 1 or (x.stride(i) > 0 and x.stride(i) % 8 == 0) for i in range(3))
-
-
-def rows_view(x: torch.Tensor, D: int) -> torch.Tensor:
-    """`x` with its head dim padded to D by zeros and 16-byte rows; `x` itself
-    where it has them already."""
-    if x.shape[-1] != D:
-        return F.pad(x, (0, D - x.shape[-1]))
-    return x if _aligned(x) else x.clone(memory_format=torch.contiguous_format)
+def rows_arg(x: torch.Tensor, D: int, hold: list) -> tuple[int, int, int, int]:
+    """(address, strides) of `x`'s rows for the C structs: the head dim padded to
+    D by zeros, rows that 16-byte loads and tensor maps can read.  A view without
+    them is copied; `hold` then keeps the copy until the launch."""
+    p = x.data_ptr()
+    b, h, s, d = x.stride()
+    if x.shape[3] == D and d == 1 and not (p | b * 2 | h * 2 | s * 2) & 15 \
+            and b > 0 and h > 0 and s > 0:
+        return p, b, h, s
+    if x.shape[3] != D:
+        x = F.pad(x, (0, D - x.shape[3]))
+    elif d != 1 or p & 15 or any(
+            n > 1 and (t <= 0 or t % 8) for n, t in zip(x.shape[:3], (b, h, s))):
+        x = x.clone(memory_format=torch.contiguous_format)
+    hold.append(x)
+    return x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)
 
 
 def span(x: torch.Tensor) -> tuple[int, int]:

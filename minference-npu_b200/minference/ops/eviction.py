@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _native
-from ._cache import check_output, check_query, check_same, lengths_arg, overlap, rows_view
+from ._cache import check_output, check_query, check_same, lengths_arg, overlap, rows_arg
 
 __all__ = ["accumulate_attention_weights", "evict_cache", "EvictedCache"]
 
@@ -32,10 +32,10 @@ class EvictedCache(NamedTuple):
 
 
 def _check_weights(name: str, w, shape: tuple, device: torch.device) -> None:
-    if not isinstance(w, torch.Tensor) or tuple(w.shape) != shape:
+    if not isinstance(w, torch.Tensor) or w.shape != shape:
         got = tuple(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__
         raise ValueError(f"{name} must be {shape}, got {got}")
-    if w.dtype != torch.float32:
+    if w.dtype is not torch.float32:
         raise TypeError(f"{name} must be float32, got {w.dtype}")
     if w.device != device:
         raise ValueError(f"{name} is on {w.device}, expected {device}")
@@ -66,27 +66,28 @@ def accumulate_attention_weights(q: torch.Tensor, k: torch.Tensor,
         raise ValueError("k must be [B,Hkv,C,D]")
     B, Hq, S_q, D = q.shape
     Hkv, C = k.shape[1], k.shape[2]
-    check_query(q, Hkv)
+    code = check_query(q, Hkv)
     check_same("k", k, q, (B, Hkv, C, D))
-    clen = lengths_arg("lengths", lengths, B, C, q.device)
+    dev = q.device
+    clen = None if lengths is None else lengths_arg("lengths", lengths, B, C, dev)
     if weights is not None:
-        _check_weights("weights", weights, (B, Hkv, C), q.device)
+        _check_weights("weights", weights, (B, Hkv, C), dev)
     if out is None:
         out = weights if weights is not None else \
-            torch.empty((B, Hkv, C), dtype=torch.float32, device=q.device)
+            torch.empty((B, Hkv, C), dtype=torch.float32, device=dev)
     else:
-        _check_weights("out", out, (B, Hkv, C), q.device)
+        _check_weights("out", out, (B, Hkv, C), dev)
+        if weights is not None and overlap(out, weights) and (
+                out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride()):
+            raise ValueError("out overlaps weights without being the same view")
     check_output("out", out)
-    if weights is not None and overlap(out, weights) and (
-            out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride()):
-        raise ValueError("out overlaps weights without being the same view")
     if overlap(out, q) or overlap(out, k):
         raise ValueError("out overlaps q or k")
     if lse is not None:
-        if not isinstance(lse, torch.Tensor) or tuple(lse.shape) != (B, Hq, S_q):
+        if not isinstance(lse, torch.Tensor) or lse.shape != (B, Hq, S_q):
             raise ValueError(f"lse must be {(B, Hq, S_q)}")
-        if lse.dtype != torch.float32 or lse.device != q.device:
-            raise TypeError(f"lse must be float32 on {q.device}")
+        if lse.dtype is not torch.float32 or lse.device != dev:
+            raise TypeError(f"lse must be float32 on {dev}")
         lse = lse.contiguous()
         if overlap(out, lse):
             raise ValueError("out overlaps lse")
@@ -96,24 +97,15 @@ def accumulate_attention_weights(q: torch.Tensor, k: torch.Tensor,
         if weights is None:
             return out.zero_()
         return out if out.data_ptr() == weights.data_ptr() else out.copy_(weights)
-    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    dk = -(-D // 8) * 8
-    qp, kp = rows_view(q, dk), rows_view(k, dk)
-    L = _native.lib()
-    need = L.mi_attn_weights_workspace_size(B, Hq, Hkv, S_q, C, dk, int(lse is not None))
-    if need > 1 << 62:
-        raise ValueError(f"sizes not supported: q {tuple(q.shape)}, k {tuple(k.shape)}")
-    with torch.cuda.device(q.device):
-        ws = _native.workspace(need, q.device) if need else None
-        rc = L.mi_attn_weights(
-            _native.t4(qp), _native.t4(kp), lse.data_ptr() if lse is not None else None,
-            clen.data_ptr() if clen is not None else None,
-            weights.data_ptr() if weights is not None else None,
-            *(weights.stride()[:2] if weights is not None else (0, 0)), out.data_ptr(),
-            *out.stride()[:2], B, Hq, Hkv, S_q, C, dk, _native.dtype_code(q), int(bool(causal)),
-            sc, ws.data_ptr() if need else None, ws.numel() if need else 0,
-            _native.stream_ptr(q.device))
-    _native.check(rc, "mi_attn_weights")
+    dk = (D + 7) & ~7
+    hold: list = []
+    args = _native.ATTN_WEIGHTS_ARGS.pack(
+        *rows_arg(q, dk, hold), *rows_arg(k, dk, hold), 0 if lse is None else lse.data_ptr(),
+        0 if clen is None else clen.data_ptr(),
+        *((weights.data_ptr(), *weights.stride()[:2]) if weights is not None else (0, 0, 0)),
+        out.data_ptr(), *out.stride()[:2], B, Hq, Hkv, S_q, C, dk, code, 1 if causal else 0,
+        1.0 / math.sqrt(D) if scale is None else scale)
+    _native.call_packed("mi_attn_weights", args, dev)
     return out
 
 
@@ -133,24 +125,26 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, keep: i
     _native.require_cuda(k)
     _native.dtype_code(k)
     B, H, C, D = k.shape
+    dev = k.device
     check_same("v", v, k, (B, H, C, D))
     if not 1 <= D <= 1024:
         raise NotImplementedError(f"head_dim={D}: evict_cache takes 1 to 1024")
-    _check_weights("weights", weights, (B, H, C), k.device)
+    _check_weights("weights", weights, (B, H, C), dev)
     keep, sink, recent = int(keep), int(sink), int(recent)
     if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError(f"need keep >= 1 and sink + recent <= keep; got keep={keep}, "
                          f"sink={sink}, recent={recent}")
-    clen = lengths_arg("lengths", lengths, B, C, k.device)
+    clen = None if lengths is None else lengths_arg("lengths", lengths, B, C, dev)
     shape = (B, H, keep, D)
     if out is None:
-        ko, vo = (torch.empty(shape, dtype=k.dtype, device=k.device) for _ in range(2))
-        wo = torch.empty(shape[:3], dtype=torch.float32, device=k.device)
+        ko = torch.empty(shape, dtype=k.dtype, device=dev)
+        vo = torch.empty(shape, dtype=k.dtype, device=dev)
+        wo = torch.empty(shape[:3], dtype=torch.float32, device=dev)
     else:
         ko, vo, wo = out
         check_same("out[0]", ko, k, shape)
         check_same("out[1]", vo, k, shape)
-        _check_weights("out[2]", wo, shape[:3], k.device)
+        _check_weights("out[2]", wo, shape[:3], dev)
         outs = (ko, vo, wo)
         for i, x in enumerate(outs):
             if i < 2 and D > 1 and x.stride(-1) != 1:
@@ -159,26 +153,21 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, keep: i
             if any(overlap(x, y) for y in (k, v, weights)) or any(
                     overlap(x, y) for y in outs[:i]):
                 raise ValueError(f"out[{i}] overlaps an input or another output")
-    index = torch.empty(shape[:3], dtype=torch.int32, device=k.device)
-    new_len = torch.empty((B,), dtype=torch.int32, device=k.device)
+    index = torch.empty(shape[:3], dtype=torch.int32, device=dev)
+    new_len = torch.empty((B,), dtype=torch.int32, device=dev)
     res = EvictedCache(ko, vo, wo, index, new_len)
     if B == 0 or H == 0:
         if B:  # no heads: the lengths alone
             n = clen.clamp(0, C) if clen is not None else torch.full_like(new_len, C)
             new_len.copy_(n.clamp_max(keep))
         return res
-    kp, vp = (x if D == 1 or x.stride(-1) == 1 else x.contiguous() for x in (k, v))
-    L = _native.lib()
-    need = L.mi_evict_cache_workspace_size(B, H, C)
-    if need > 1 << 62:
-        raise ValueError(f"sizes not supported: k {tuple(k.shape)}")
-    with torch.cuda.device(k.device):
-        ws = _native.workspace(need, k.device) if need else None
-        rc = L.mi_evict_cache(
-            _native.t4(kp), _native.t4(vp), weights.data_ptr(), *weights.stride()[:2],
-            _native.t4(ko), _native.t4(vo), wo.data_ptr(), *wo.stride()[:2], index.data_ptr(),
-            new_len.data_ptr(), B, H, C, D, keep, sink, recent,
-            clen.data_ptr() if clen is not None else None, ws.data_ptr() if need else None,
-            ws.numel() if need else 0, _native.stream_ptr(k.device))
-    _native.check(rc, "mi_evict_cache")
+    if D > 1:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        v = v if v.stride(-1) == 1 else v.contiguous()
+    args = _native.EVICT_ARGS.pack(
+        k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], weights.data_ptr(),
+        *weights.stride()[:2], ko.data_ptr(), *ko.stride()[:3], vo.data_ptr(), *vo.stride()[:3],
+        wo.data_ptr(), *wo.stride()[:2], index.data_ptr(), new_len.data_ptr(),
+        0 if clen is None else clen.data_ptr(), B, H, C, D, keep, sink, recent)
+    _native.call_packed("mi_evict_cache", args, dev)
     return res

@@ -16,12 +16,12 @@ import math
 import torch
 
 from .. import _native
-from ._cache import check_output, check_query, check_same, lengths_arg, overlap, rows_view
+from ._cache import check_output, check_query, check_same, lengths_arg, overlap, rows_arg
 from ._common import output as _common_out
 
 __all__ = ["shared_prefix_attention"]
 
-_NULL = _native.mi_tensor4(0, 0, 0, 0, 1)
+_NONE = (0, 0, 0, 0)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
@@ -60,59 +60,58 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
     if kv.dim() != 4:
         raise ValueError("keys must be [B,Hkv,C,D] and prefix keys [G,Hkv,P,D] or [Hkv,P,D]")
     Hkv = kv.shape[1]
-    check_query(q, Hkv)
-    G = P = C = 0
+    code = check_query(q, Hkv)
+    G, P, C = 1, 0, 0
+    plen = clen = None
     if k_prefix is not None:
         if k_prefix.dim() != 4:
             raise ValueError("prefix keys must be [G,Hkv,P,D] or [Hkv,P,D]")
         G, P = k_prefix.shape[0], k_prefix.shape[2]
-        for name, x in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
-            check_same(name, x, q, (G, Hkv, P, D))
+        shape = (G, Hkv, P, D)
+        check_same("k_prefix", k_prefix, q, shape)
+        check_same("v_prefix", v_prefix, q, shape)
         if G < 1 or B % G:
             raise ValueError(f"{B} sequences over {G} prefixes")
+        if prefix_lengths is not None:
+            plen = lengths_arg("prefix_lengths", prefix_lengths, G, P, q.device)
     elif prefix_lengths is not None:
         raise ValueError("prefix_lengths without a prefix")
     if k is not None:
         C = k.shape[2]
-        for name, x in (("k", k), ("v", v)):
-            check_same(name, x, q, (B, Hkv, C, D))
+        shape = (B, Hkv, C, D)
+        check_same("k", k, q, shape)
+        check_same("v", v, q, shape)
+        if lengths is not None:
+            clen = lengths_arg("lengths", lengths, B, C, q.device)
     elif lengths is not None:
         raise ValueError("lengths without own caches")
-    plen = lengths_arg("prefix_lengths", prefix_lengths, G, P, q.device)
-    clen = lengths_arg("lengths", lengths, B, C, q.device)
-    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
 
-    dk = -(-D // 8) * 8
-    if out is not None:
-        res = _common_out(out, (B, Hq, S_q, D), q) if dk == D else out
+    dk = (D + 7) & ~7
+    if out is None:
+        res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
+    else:
         check_same("out", out, q, (B, Hq, S_q, D))
         check_output("out", out)
         for name, x in (("q", q), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("k", k),
                         ("v", v)):
             if x is not None and overlap(out, x):
                 raise ValueError(f"out overlaps {name}")
-    if out is None or dk != D:
-        res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
+        if dk == D:
+            res = _common_out(out, (B, Hq, S_q, D), q)
+        else:
+            res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, Hq, S_q), dtype=torch.float32, device=q.device) if return_lse else None
-    qp = rows_view(q, dk)
-    pre = [rows_view(x, dk) for x in (k_prefix, v_prefix)] if P else None
-    cache = [rows_view(x, dk) for x in (k, v)] if C else None
-    L = _native.lib()
-    sizes = (B, Hq, Hkv, S_q, max(G, 1), P, C, dk)
-    need = L.mi_shared_prefix_fwd_workspace_size(*sizes)
-    if need > 1 << 62:
-        raise ValueError(f"sizes not supported: q {tuple(q.shape)}, prefix {P}, cache {C}")
-    with torch.cuda.device(q.device):
-        ws = _native.workspace(need, q.device) if need else None
-        rc = L.mi_shared_prefix_fwd(
-            _native.t4(qp), *([_native.t4(x) for x in pre] if pre else (_NULL, _NULL)),
-            *([_native.t4(x) for x in cache] if cache else (_NULL, _NULL)), _native.t4(res),
-            lse.data_ptr() if return_lse else None, *sizes, _native.dtype_code(q),
-            plen.data_ptr() if plen is not None and P else None,
-            clen.data_ptr() if clen is not None and C else None, int(bool(causal)), sc,
-            ws.data_ptr() if need else None, ws.numel() if need else 0,
-            _native.stream_ptr(q.device))
-    _native.check(rc, "mi_shared_prefix_fwd")
+    hold: list = []
+    args = _native.SHARED_PREFIX_ARGS.pack(
+        *rows_arg(q, dk, hold),
+        *(rows_arg(k_prefix, dk, hold) if P else _NONE),
+        *(rows_arg(v_prefix, dk, hold) if P else _NONE),
+        *(rows_arg(k, dk, hold) if C else _NONE), *(rows_arg(v, dk, hold) if C else _NONE),
+        res.data_ptr(), *res.stride()[:3], 0 if lse is None else lse.data_ptr(),
+        plen.data_ptr() if plen is not None and P else 0,
+        clen.data_ptr() if clen is not None and C else 0, B, Hq, Hkv, S_q, G, P, C, dk, code,
+        1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale)
+    _native.call_packed("mi_shared_prefix_fwd", args, q.device)
     if dk != D:
         res = res[..., :D] if out is None else out.copy_(res[..., :D])
     return (res, lse) if return_lse else res

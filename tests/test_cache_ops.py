@@ -760,60 +760,93 @@ def test_c_entry_points_refuse():
 
     build.build()
     L = _native.lib()
-    ok = _native.mi_tensor4(1 << 20, 4096, 1024, 64, 1)
-    null = _native.mi_tensor4(0, 0, 0, 0, 1)
+    ok = (1 << 20, 4096, 1024, 64)
+    odd = ((1 << 20) + 2, 4096, 1024, 64)    # not 16-byte aligned
+    step = (1 << 20, 4096, 1024, 60)         # rows not 16 bytes apart
+    flat = (1 << 20, 0, 1024, 64)            # one entry for all
+    null = (0, 4096, 1024, 64)
+    none = 2**64 - 1
 
-    def attn(q=ok, kp=ok, vp=ok, k=ok, v=ok, out=ok, B=2, Hq=4, Hkv=2, Sq=1, G=1, P=8, C=8, D=64,
-             dtype=1, ws=None, n=0):
-        return L.mi_shared_prefix_fwd(q, kp, vp, k, v, out, None, B, Hq, Hkv, Sq, G, P, C, D,
-                                      dtype, None, None, 1, 1.0, ws, n, None)
+    def attn(q=ok, kp=ok, vp=ok, k=ok, v=ok, out=ok, B=2, Hq=4, Hkv=2, Sq=1, G=2, P=8, C=8, D=64,
+             dtype=1, ws=None, n=0, size=False):
+        args = _native.SHARED_PREFIX_ARGS.pack(*q, *kp, *vp, *k, *v, *out, 0, 0, 0, B, Hq, Hkv,
+                                               Sq, G, P, C, D, dtype, 1, 1.0)
+        if size:
+            return L.mi_shared_prefix_fwd_workspace_size(args)
+        return L.mi_shared_prefix_fwd(args, ws, n, None)
 
+    assert L.mi_shared_prefix_fwd(None, None, 0, None) == 1
     assert attn(dtype=2) == 2
     for bad in (dict(Hq=3), dict(Hkv=0), dict(G=0), dict(B=3, G=2), dict(D=132), dict(D=60),
                 dict(D=0), dict(P=-1), dict(C=-1), dict(C=1 << 31), dict(Sq=-1),
-                dict(B=1 << 20, Hq=1 << 20)):
+                dict(P=1 << 30, C=64), dict(B=1 << 20, Hq=1 << 20)):
         assert attn(**bad) == 1, bad
+        assert attn(size=True, **bad) == none, bad
     assert attn(B=0) == 0 and attn(Sq=0) == 0
-    odd = _native.mi_tensor4((1 << 20) + 2, 4096, 1024, 64, 1)
-    step = _native.mi_tensor4(1 << 20, 4096, 1024, 60, 1)
-    wide = _native.mi_tensor4(1 << 20, 4096, 1024, 64, 2)
-    head = _native.mi_tensor4(1 << 20, 4096, 1024, 64, 1, 64, 4)
-    for x in (odd, wide):
+    for x in (odd, flat, null):
         for name in ("q", "kp", "vp", "k", "v", "out"):
             assert attn(**{name: x}) == 5, name
     assert attn(k=step) == 5 and attn(vp=step) == 5
-    assert attn(q=head) == 1 and attn(k=head) == 1
     assert attn() == 3 and attn(ws=1 << 20, n=64) == 3  # two segments need a workspace
     assert attn(ws=(1 << 20) + 4, n=1 << 30) == 3
-    assert L.mi_shared_prefix_fwd_workspace_size(2, 3, 2, 1, 1, 8, 8, 64) == 2**64 - 1
-    a = L.mi_shared_prefix_fwd_workspace_size(2, 4, 2, 1, 1, 1000, 8, 64)
-    b = L.mi_shared_prefix_fwd_workspace_size(2, 4, 2, 1, 1, 100000, 8, 64)
-    assert 0 < a < b
+    assert 0 < attn(G=1, P=1000, size=True) < attn(G=1, P=100000, size=True)
 
-    def weights(q=ok, k=ok, lse=None, wo=1 << 20, B=2, Hq=4, Hkv=2, Sq=1, C=8, D=64, dtype=1,
-                ws=None, n=0):
-        return L.mi_attn_weights(q, k, lse, None, None, 0, 0, wo, 16, 8, B, Hq, Hkv, Sq, C, D,
-                                 dtype, 1, 1.0, ws, n, None)
+    def weights(q=ok, k=ok, lse=0, wo=1 << 20, B=2, Hq=4, Hkv=2, Sq=1, C=8, D=64, dtype=1,
+                ws=None, n=0, size=False):
+        args = _native.ATTN_WEIGHTS_ARGS.pack(*q, *k, lse, 0, 0, 0, 0, wo, 16, 8, B, Hq, Hkv, Sq,
+                                              C, D, dtype, 1, 1.0)
+        if size:
+            return L.mi_attn_weights_workspace_size(args)
+        return L.mi_attn_weights(args, ws, n, None)
 
+    assert L.mi_attn_weights(None, None, 0, None) == 1
     assert weights(dtype=7) == 2
-    for bad in (dict(Hq=3), dict(D=136), dict(C=-1), dict(Hkv=0), dict(wo=None), dict(Sq=0)):
+    for bad in (dict(Hq=3), dict(D=136), dict(C=-1), dict(Hkv=0), dict(wo=0), dict(Sq=0)):
         assert weights(**bad) == 1, bad
-    assert weights(q=odd) == 5 and weights(k=step) == 5 and weights(k=head) == 1
+    assert weights(q=odd) == 5 and weights(k=step) == 5 and weights(k=null) == 5
     assert weights() == 3
     assert weights(B=0) == 0 and weights(C=0) == 0
-    assert L.mi_attn_weights_workspace_size(2, 4, 2, 1, 8, 64, 1) == 0
+    assert weights(lse=1 << 20, size=True) == 0 and weights(size=True) > 0
 
     def evict(k=ok, v=ok, w=1 << 20, ko=ok, vo=ok, wo=1 << 20, idx=1 << 20, nl=1 << 20, B=2, H=2,
-              C=8, D=64, keep=4, sink=0, recent=0, ws=None, n=0):
-        return L.mi_evict_cache(k, v, w, 16, 8, ko, vo, wo, 8, 4, idx, nl, B, H, C, D, keep, sink,
-                                recent, None, ws, n, None)
+              C=8, D=64, keep=4, sink=0, recent=0, ws=None, n=0, size=False):
+        args = _native.EVICT_ARGS.pack(*k, *v, w, 16, 8, *ko, *vo, wo, 8, 4, idx, nl, 0, B, H, C,
+                                       D, keep, sink, recent)
+        if size:
+            return L.mi_evict_cache_workspace_size(args)
+        return L.mi_evict_cache(args, ws, n, None)
 
+    assert L.mi_evict_cache(None, None, 0, None) == 1
     for bad in (dict(keep=0), dict(sink=3, recent=2), dict(sink=-1), dict(recent=-1), dict(D=0),
-                dict(D=2000), dict(C=-1), dict(idx=None), dict(nl=None), dict(wo=None),
-                dict(w=None), dict(k=head), dict(sink=2**62, recent=2**62)):
+                dict(D=2000), dict(C=-1), dict(idx=0), dict(nl=0), dict(wo=0), dict(w=0),
+                dict(k=null), dict(vo=null), dict(sink=2**62, recent=2**62)):
         assert evict(**bad) == 1, bad
-    assert evict(v=wide) == 5 and evict(ko=wide) == 5
     assert evict(C=400000) == 3  # keys past shared memory need a workspace
     assert evict(B=0) == 0 and evict(H=0) == 0
-    assert L.mi_evict_cache_workspace_size(1, 1, 65536) == 0
-    assert null.ptr in (None, 0)
+    assert evict(C=65536, size=True) == 0 and evict(C=400000, size=True) >= 4 * 400000 * 4
+    assert evict(keep=0, size=True) == none
+
+
+def test_argument_structs_match_the_header():
+    """The packed layouts have the sizes that a C compiler gives the structs."""
+    import subprocess
+    import tempfile
+
+    from minference import _native
+
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = (f'#include "{root}/include/minference_b200.h"\n#include <stdio.h>\n'
+           'int main(void){printf("%zu %zu %zu %zu %zu %zu", sizeof(mi_shared_prefix_args), '
+           'sizeof(mi_attn_weights_args), sizeof(mi_evict_args), '
+           'offsetof(mi_shared_prefix_args, dtype), offsetof(mi_attn_weights_args, dtype), '
+           'offsetof(mi_evict_args, B));return 0;}')
+    with tempfile.TemporaryDirectory() as d:
+        with open(d + "/a.c", "w") as f:
+            f.write(src)
+        subprocess.check_call(["gcc", "-o", d + "/a", d + "/a.c"])
+        got = [int(x) for x in subprocess.check_output([d + "/a"]).split()]
+    assert got[:3] == [_native.SHARED_PREFIX_ARGS.size, _native.ATTN_WEIGHTS_ARGS.size,
+                       _native.EVICT_ARGS.size]
+    assert got[3:] == [8 * 35, 8 * 22, 8 * 25]
