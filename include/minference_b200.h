@@ -255,7 +255,7 @@ typedef struct mi_rows {
  * j < lengths[b] - (S_q-1-s) if causal, j < lengths[b] otherwise (null: C).
  * A row that sees nothing gives 0 and lse -inf.  lse (null: not wanted) is
  * float [B, Hq, S_q], the natural logarithm of the sum of exp(scale q.k).
- * D is a multiple of 8, at most 128; P or C may be 0 (the rows are then not
+ * D is a multiple of 8 from 32 to 128; P or C may be 0 (the rows are then not
  * read), P + C at most 2^30.  What a cache holds past its length does not
  * reach the result.  The workspace (16-byte aligned) may be reused once the
  * call's work has finished; its size is SIZE_MAX for sizes the call refuses. */

@@ -9,38 +9,49 @@
 namespace mib200 {
 
 // ---------------------------------------------------------------------------
-// Few rows (1 to 32 per key/value head): a work item is one tile of 16*MT
-// rows against `chunk` keys.  Its four warps take groups of 16 keys in turn;
-// each warp streams its own groups through its own shared-memory ring
-// (cp.async) and keeps its own running maximum, sum and O, so there is no
-// barrier in the loop.  The four states are joined at the end.
-//   S (16 rows x 16 keys) = Q K^T     Q fragments stay in registers
-//   O (16 rows x D) += P V            P is S's registers, rounded to the
-//                                     inputs' type for the tensor core
+// Few rows (1 to 32 per key/value head): a work item is one tile of 8*NT rows
+// against `chunk` keys.  Its two warps take groups of 16 keys in turn; each
+// warp streams its own groups through its own shared-memory ring (cp.async)
+// and keeps its own running maximum, sum and O, so there is no barrier in the
+// loop.  The two states are joined at the end.  Keys are the M side of both
+// products, so that a single row costs an 8-wide tile, not a 16-wide one:
+//   S^T (16 keys x 8 rows) = K Q^T     Q fragments stay in registers
+//   O^T (D x 8 rows) += V^T P^T        P^T is S^T's registers rounded to the
+//                                      inputs' type and transposed in place
 // Rows of a ring stage are padded by 16 bytes, which makes the ldmatrix rows
 // of 128, 192 and 256 bytes fall into distinct banks.  Keys past the end of
 // the range are filled with zeros instead of being read, so whatever a cache
 // holds past its length cannot reach O through 0 * V.
+//
+// kStats: the rows' (maximum, sum) only; no V.
+// kWeights: given the rows' lse, a key's weight summed over the tile's rows
+// (all rows of the key/value head, at most 32) and added to win; no V.
 // ---------------------------------------------------------------------------
-constexpr int kRowsWarps = 4;
+enum RowsMode { kAttention, kStats, kWeights };
+constexpr int kRowsWarps = 2;
 
-template <int DK, bool STATS>
+template <int DK, RowsMode MODE>
 struct RowsSmem {
   static constexpr int kPitch = DK * 2 + 16;
-  static constexpr int kTile = 16 * kPitch;                   // 16 keys of K or V
-  static constexpr int kStage = (STATS ? 1 : 2) * kTile;      // one warp's stage
-  static constexpr int ST = DK == 64 ? 5 : (DK == 96 ? 4 : 3);  // ~100 KB a block: two per SM
+  static constexpr int kTile = 16 * kPitch;  // 16 keys of K or V
+  // one warp's stage; kWeights: and 16 of win
+  static constexpr int kStage = MODE == kAttention ? 2 * kTile
+                                                   : kTile + (MODE == kWeights ? 64 : 0);
+  // about 52 KB a block: four per SM
+  static constexpr int ST = (DK == 64 ? 6 : (DK == 96 ? 4 : 3)) * (MODE == kAttention ? 1 : 2) -
+                            (MODE == kAttention ? 0 : 1);
   static constexpr int kWarpRing = ST * kStage;
   static constexpr int kRing = kRowsWarps * kWarpRing;
 };
 
-template <typename DT, int DK, int MT, bool STATS>
-__global__ void __launch_bounds__(32 * kRowsWarps, 2)
+template <typename DT, int DK, int NT, RowsMode MODE>
+__global__ void __launch_bounds__(32 * kRowsWarps, 4)
     cache_rows_kernel(const __grid_constant__ CacheParams p) {
-  using L = RowsSmem<DK, STATS>;
-  constexpr int KS = DK / 16;
+  using L = RowsSmem<DK, MODE>;
+  constexpr int KS = DK / 16, R = 8 * NT, CPR = DK / 8;
+  constexpr bool kO = MODE == kAttention;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float sm_m[kRowsWarps][16 * MT], sm_l[kRowsWarps][16 * MT];
+  __shared__ float sm_m[kRowsWarps][R], sm_l[kRowsWarps][R];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
 
@@ -54,8 +65,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
   it /= sg.nsplit;
   const int h = (int)(it % p.Hkv);
   const int e = (int)(it / p.Hkv);
-  const int r0 = rt * 16 * MT;
-  const int nrows = min(16 * MT, sg.rows - r0);
+  const int r0 = rt * R;
+  const int nrows = min(R, sg.rows - r0);
   const int len = cache_len(sg, e);
   // Keys that the tile's last token sees (its rows cover tokens in order
   // unless they wrap into another head).
@@ -66,84 +77,133 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
     end = max(0, len - (p.Sq - 1 - smax));
   }
   const int kb = sp * sg.chunk;
-  const int ke = min(end, (int)min((long long)kb + sg.chunk, (long long)end));
+  const int ke = (int)min((long long)kb + sg.chunk, (long long)end);
   const int ngroups = ke > kb ? (ke - kb + 15) >> 4 : 0;
 
-  // ---- Q tile -> shared (ring area) -> fragments ----------------------------
-  constexpr int CPR = DK / 8;
-  for (int i = tid; i < 16 * MT * CPR; i += 32 * kRowsWarps) {
-    const int r = i / CPR, c = i - r * CPR;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < nrows && c * 8 < p.D) {
-      int b, hd, tk;
-      cache_row(p, sg, e, h, r0 + r, b, hd, tk);
-      x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b + hd * p.qs_h + tk * p.qs_s + c * 8);
-    }
-    *reinterpret_cast<uint4*>(smem + r * L::kPitch + c * 16) = x;
+  const float* win = nullptr;
+  float* wout = nullptr;
+  if constexpr (MODE == kWeights) {
+    win = p.win ? p.win + e * p.wi_b + h * p.wi_h : nullptr;
+    wout = p.wout + e * p.wo_b + h * p.wo_h;
   }
-  __syncthreads();
-  uint32_t qf[MT][KS][4];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      ldsm4(qf[i][ks], smem_u32(smem) + (i * 16 + (lane & 15)) * L::kPitch + ks * 32 +
-                           (lane >> 4) * 16);
-  __syncthreads();  // the ring reuses the Q area
-
-  // ---- per-thread rows: lane/4 and lane/4 + 8 of every 16-row tile ----------
-  int lim[MT][2];  // keys that the row sees
-  int minlim = ke;
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = i * 16 + (lane >> 2) + 8 * j;
-      lim[i][j] = 0;
-      if (r < nrows) lim[i][j] = sg.causal ? len - (p.Sq - 1 - (r0 + r) % p.Sq) : len;
-      if (r < nrows) minlim = min(minlim, lim[i][j]);
-    }
-  minlim = __reduce_min_sync(0xffffffffu, minlim);
 
   // ---- loader: lane l brings 16-byte pieces (l&3) + 4v of rows l/4 and l/4+8 -
   const uint32_t ring = smem_u32(smem) + warp * L::kWarpRing;
   const int lrow = lane >> 2, lcol = lane & 3;
   const uint32_t ldst = ring + lrow * L::kPitch + lcol * 16;
   const uint16_t* kbase = sg.k + e * sg.ks_b + h * sg.ks_h + lcol * 8;
-  const uint16_t* vbase = STATS ? nullptr : sg.v + e * sg.vs_b + h * sg.vs_h + lcol * 8;
+  const uint16_t* vbase = kO ? sg.v + e * sg.vs_b + h * sg.vs_h + lcol * 8 : nullptr;
   auto load = [&](int g) {
     if (g < ngroups) {
-      const uint32_t st = ldst + ((g / kRowsWarps) % L::ST) * L::kStage;
+      const uint32_t off = ((g / kRowsWarps) % L::ST) * L::kStage;
+      const uint32_t st = ldst + off;
       const int key = kb + g * 16 + lrow;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bool in = key + 8 * u < ke;
         const long long kk = in ? key + 8 * u : 0;
         const uint16_t* kr = kbase + kk * sg.ks_s;
-        const uint16_t* vr = STATS ? nullptr : vbase + kk * sg.vs_s;
+        const uint16_t* vr = kO ? vbase + kk * sg.vs_s : nullptr;
 #pragma unroll
         for (int v = 0; v < CPR / 4; ++v) {
           const bool ok = in && (lcol + 4 * v) * 8 < p.D;
           cp16(st + u * 8 * L::kPitch + v * 64, ok ? kr + v * 32 : kbase, ok);
-          if constexpr (!STATS)
+          if constexpr (kO)
             cp16(st + L::kTile + u * 8 * L::kPitch + v * 64, ok ? vr + v * 32 : vbase, ok);
         }
+      }
+      if constexpr (MODE == kWeights) {
+        const int j = kb + g * 16 + lane;
+        if (lane < 16 && win) cp4(ring + off + L::kTile + lane * 4, j < ke ? win + j : win, j < ke);
       }
     }
     cp_commit();
   };
+
+  // ---- Q tile -> shared (the last ring stage, loaded last) -> fragments ----------
+  // Every warp fetches the tile for itself, beside its first keys.
 #pragma unroll
   for (int s = 0; s < L::ST - 1; ++s) load(warp + s * kRowsWarps);
+  uint32_t qf[NT][KS][2];
+  int lim[NT][2];  // keys that row 8n + (lane&3)*2 + x sees
+  int minlim = 0x7fffffff;
+  {
+    uint8_t* qs = smem + warp * L::kWarpRing + (L::ST - 1) * L::kStage;
+    static_assert(16 * L::kPitch <= L::kStage, "16 rows of Q fit a stage");
+#pragma unroll
+    for (int half = 0; half < (NT + 1) / 2; ++half) {
+      const int hr = half * 16 + (lane & 15);  // row whose address this lane works out
+      const uint16_t* qp = p.q;
+      if (hr < nrows) {
+        int b, hd, tk;
+        cache_row(p, sg, e, h, r0 + hr, b, hd, tk);
+        qp += b * p.qs_b + hd * p.qs_h + tk * p.qs_s;
+      }
+      constexpr int kRows = NT == 1 ? 8 : 16;
+      constexpr int kIter = kRows * CPR / 32;
+      uint4 x[kIter];
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
+        const unsigned long long a =
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(qp), r);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (half * 16 + r < nrows && c * 8 < p.D)
+          x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + c * 8);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
+        *reinterpret_cast<uint4*>(qs + r * L::kPitch + c * 16) = x[i];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        if (half * 2 + n >= NT) break;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          uint32_t b[4];
+          ldsm4(b, smem_u32(qs) + (n * 8 + (lane & 7)) * L::kPitch + ks * 32 + (lane >> 3) * 16);
+          qf[half * 2 + n][ks][0] = b[0];
+          qf[half * 2 + n][ks][1] = b[1];
+          qf[half * 2 + n][ks + 1][0] = b[2];
+          qf[half * 2 + n][ks + 1][1] = b[3];
+        }
+      }
+      __syncwarp();
+    }
+  }
+  float nz[NT][2];  // kWeights: -lse (log2 units; -inf: the row adds nothing)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = n * 8 + (lane & 3) * 2 + x;
+      lim[n][x] = 0;
+      nz[n][x] = -INFINITY;
+      if (r < nrows) {
+        const int tok = (r0 + r) % p.Sq;
+        lim[n][x] = sg.causal ? len - (p.Sq - 1 - tok) : len;
+        minlim = min(minlim, lim[n][x]);
+        if constexpr (MODE == kWeights) {
+          const float z =
+              p.z[((long long)e * p.Hq + h * p.group + (r0 + r) / p.Sq) * p.Sq + tok];
+          if (z != -INFINITY) nz[n][x] = -z * p.z_mul;
+        }
+      }
+    }
+  minlim = __reduce_min_sync(0xffffffffu, minlim);
 
-  float m[MT][2], l[MT][2];
-  float o[MT][STATS ? 1 : DK / 8][4];
+  float m[NT][2], l[NT][2];
+  float o[kO ? DK / 16 : 1][NT][4];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    m[i][0] = m[i][1] = -INFINITY;
-    l[i][0] = l[i][1] = 0.f;
-    if constexpr (!STATS)
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+    if constexpr (kO)
 #pragma unroll
-      for (int d = 0; d < DK / 8; ++d) o[i][d][0] = o[i][d][1] = o[i][d][2] = o[i][d][3] = 0.f;
+      for (int d = 0; d < DK / 16; ++d) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.f;
   }
 
   for (int g = warp; g < ngroups; g += kRowsWarps) {
@@ -151,114 +211,137 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
     cp_wait<L::ST - 1>();
     __syncwarp();
     const uint32_t st = ring + ((g / kRowsWarps) % L::ST) * L::kStage;
-    float s[MT][2][4];
+    float s[NT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
-    // K: keys 0-7 / 8-15 (second pair of matrices) x dims 0-7 / 8-15 of the step
-    const uint32_t ka =
-        st + ((lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    const uint32_t ka = st + (lane & 15) * L::kPitch + (lane >> 4) * 16;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      uint32_t b[4];
-      ldsm4(b, ka + ks * 32);
+      uint32_t a[4];
+      ldsm4(a, ka + ks * 32);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        mma16816<DT>(s[i][0], qf[i][ks], b[0], b[1]);
-        mma16816<DT>(s[i][1], qf[i][ks], b[2], b[3]);
-      }
+      for (int n = 0; n < NT; ++n) mma16816<DT>(s[n], a, qf[n][ks][0], qf[n][ks][1]);
     }
     const int key0 = kb + g * 16;
-    const bool full = key0 + 16 <= minlim;
-    uint32_t pa[MT][4];
+    const bool full = key0 + 16 <= min(minlim, ke);
+    if constexpr (MODE == kWeights) {
+      float t0 = 0.f, t1 = 0.f;  // keys lane/4 and lane/4 + 8
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[i][n][c] *= p.scale_log2;
-      if (!full) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int key = key0 + n * 8 + (lane & 3) * 2 + (c & 1);
-            if (key >= min(lim[i][c >> 1], ke)) s[i][n][c] = -INFINITY;
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float t = fmaxf(fmaxf(s[i][0][2 * j], s[i][0][2 * j + 1]),
-                        fmaxf(s[i][1][2 * j], s[i][1][2 * j + 1]));
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        const float mn = fmaxf(m[i][j], t);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float f = fast_exp2(m[i][j] - base);
-        m[i][j] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float x0 = fast_exp2(s[i][n][2 * j] - base);
-          const float x1 = fast_exp2(s[i][n][2 * j + 1] - base);
-          sum += x0 + x1;
-          pa[i][n * 2 + j] = DType<DT>::pack2(x0, x1);
+        for (int x = 0; x < 2; ++x) {
+          const int key = key0 + (lane >> 2), lm = min(lim[n][x], ke);
+          const float p0 = fast_exp2(fmaf(s[n][x], p.scale_log2, nz[n][x]));
+          const float p1 = fast_exp2(fmaf(s[n][2 + x], p.scale_log2, nz[n][x]));
+          t0 += full || key < lm ? p0 : 0.f;
+          t1 += full || key + 8 < lm ? p1 : 0.f;
         }
-        l[i][j] = l[i][j] * f + sum;
-        if constexpr (!STATS) {
-          if (__any_sync(0xffffffffu, f != 1.f)) {
+      t0 += __shfl_xor_sync(0xffffffffu, t0, 1);
+      t1 += __shfl_xor_sync(0xffffffffu, t1, 1);
+      t0 += __shfl_xor_sync(0xffffffffu, t0, 2);
+      t1 += __shfl_xor_sync(0xffffffffu, t1, 2);
+      // lanes 4i and 4i+1 write keys i and i + 8
+      if ((lane & 3) < 2) {
+        const int i = (lane >> 2) + 8 * (lane & 1);
+        float w = (lane & 1) ? t1 : t0;
+        if (win)
+          w += *reinterpret_cast<const float*>(smem + (st - smem_u32(smem)) + L::kTile + i * 4);
+        if (key0 + i < ke) wout[key0 + i] = w;
+      }
+    } else {
+      uint32_t pb[NT][2];
+      bool grew = false;
+      float f[NT][2];
 #pragma unroll
-            for (int d = 0; d < DK / 8; ++d) {
-              o[i][d][2 * j] *= f;
-              o[i][d][2 * j + 1] *= f;
-            }
-          }
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[n][c] *= p.scale_log2;
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key0 + (lane >> 2) + 8 * (c >> 1) >= min(lim[n][c & 1], ke)) s[n][c] = -INFINITY;
+        }
+        float pr[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float t = fmaxf(s[n][x], s[n][2 + x]);
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+          const float mn = fmaxf(m[n][x], t);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          f[n][x] = fast_exp2(m[n][x] - base);
+          grew |= mn != m[n][x];
+          m[n][x] = mn;
+          pr[x] = fast_exp2(s[n][x] - base);
+          pr[2 + x] = fast_exp2(s[n][2 + x] - base);
+          l[n][x] = l[n][x] * f[n][x] + (pr[x] + pr[2 + x]);
+        }
+        if constexpr (kO) {
+          pb[n][0] = movm_t(DType<DT>::pack2(pr[0], pr[1]));
+          pb[n][1] = movm_t(DType<DT>::pack2(pr[2], pr[3]));
         }
       }
-    }
-    if constexpr (!STATS) {
-      // V (transposed by the load): keys 0-7 / 8-15 x dims 0-7 / 8-15
-      const uint32_t va = st + L::kTile + (lane & 15) * L::kPitch + (lane >> 4) * 16;
+      if constexpr (kO) {
+        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int d = 0; d < DK / 16; ++d) {
-        uint32_t b[4];
-        ldsm4_t(b, va + d * 32);
+          for (int d = 0; d < DK / 16; ++d)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          mma16816<DT>(o[i][2 * d], pa[i], b[0], b[1]);
-          mma16816<DT>(o[i][2 * d + 1], pa[i], b[2], b[3]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[d][n][c] *= f[n][c & 1];
+        }
+        const uint32_t va = st + L::kTile + ((lane & 7) + ((lane >> 4) << 3)) * L::kPitch +
+                            ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int d = 0; d < DK / 16; ++d) {
+          uint32_t a[4];
+          ldsm4_t(a, va + d * 32);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<DT>(o[d][n], a, pb[n][0], pb[n][1]);
         }
       }
     }
     __syncwarp();  // the stage is free for the load of the next step
   }
   cp_wait<0>();
-  __syncthreads();
 
-  // ---- join the four warps ---------------------------------------------------
+  if constexpr (MODE == kWeights) {
+    // keys of the range past the length: their weights pass through
+    const int last = (int)min((long long)kb + sg.chunk, (long long)sg.cap);
+    if (win != wout)
+      for (int j = max(kb, max(ke, 0)) + tid; j < last; j += 32 * kRowsWarps)
+        wout[j] = win ? win[j] : 0.f;
+    return;
+  }
+
+  // ---- join the two warps -----------------------------------------------------
+  constexpr int kOP = DK + 4;  // floats per row of O in shared memory
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 1);
-      l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 2);
-      const int r = i * 16 + (lane >> 2) + 8 * j;
-      if ((lane & 3) == 0) {
-        sm_m[warp][r] = m[i][j];
-        sm_l[warp][r] = l[i][j];
+    for (int x = 0; x < 2; ++x) {
+      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
+      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
+      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+      const int r = n * 8 + (lane & 3) * 2 + x;
+      if (lane < 4) {
+        sm_m[warp][r] = m[n][x];
+        sm_l[warp][r] = l[n][x];
       }
-      if constexpr (!STATS) {
-        float* row = reinterpret_cast<float*>(smem) + (warp * 16 * MT + r) * (DK + 4);
+      if constexpr (kO) {
+        float* row = reinterpret_cast<float*>(smem) + (warp * R + r) * kOP + (lane >> 2);
 #pragma unroll
-        for (int d = 0; d < DK / 8; ++d)
-          *reinterpret_cast<float2*>(row + d * 8 + (lane & 3) * 2) =
-              make_float2(o[i][d][2 * j], o[i][d][2 * j + 1]);
+        for (int d = 0; d < DK / 16; ++d) {
+          row[d * 16] = o[d][n][x];
+          row[d * 16 + 8] = o[d][n][2 + x];
+        }
       }
     }
   __syncthreads();
-  const int D4 = p.D >> 2;
-  const bool direct = !STATS && p.NS == 1;
+  const int D4 = kO ? p.D >> 2 : 1;
+  const bool direct = kO && p.NS == 1;
   for (int i = tid; i < nrows * D4; i += 32 * kRowsWarps) {
     const int r = i / D4, c = i - r * D4;
     float M = sm_m[0][r];
@@ -271,16 +354,15 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
     for (int w = 0; w < kRowsWarps; ++w) {
       const float f = fast_exp2(sm_m[w][r] - base);
       lt += f * sm_l[w][r];
-      if constexpr (!STATS) {
-        const float4 x = *reinterpret_cast<const float4*>(
-            reinterpret_cast<float*>(smem) + (w * 16 * MT + r) * (DK + 4) + c * 4);
+      if constexpr (kO) {
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) +
+                                                          (w * R + r) * kOP + c * 4);
         acc.x += f * x.x;
         acc.y += f * x.y;
         acc.z += f * x.z;
         acc.w += f * x.w;
       }
     }
-    if (STATS && c) continue;
     int b, hd, tk;
     cache_row(p, sg, e, h, r0 + r, b, hd, tk);
     const long long row = ((long long)b * p.Hq + hd) * p.Sq + tk;
@@ -294,7 +376,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
         p.lse[row] = M == -INFINITY ? M : (M + log2f(lt)) * 0.69314718055994531f;
     } else {
       const long long at = row * p.NS + sg.slot0 + sp;
-      if (!STATS && M != -INFINITY) *reinterpret_cast<float4*>(p.opart + at * p.D + c * 4) = acc;
+      if (kO && M != -INFINITY) *reinterpret_cast<float4*>(p.opart + at * p.D + c * 4) = acc;
       if (c == 0) p.ml[at] = make_float2(M, lt);
     }
   }
@@ -304,45 +386,63 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 2)
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partial results of a row: one warp per row, a lane per 4 dims.
-// Slots without a visible key have m = -inf and are not read.
+// Joins the partial results of a row: WPR warps per row, each with every
+// WPR-th slot, a lane per 4 dims.  Slots without a visible key have m = -inf
+// and are not read.
 // ---------------------------------------------------------------------------
-template <typename DT>
+template <typename DT, int WPR>
 __global__ void __launch_bounds__(128) cache_combine_kernel(const __grid_constant__ CacheParams p,
                                                             long long nrows) {
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  __shared__ float4 part[4][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = warp % WPR;
+  const long long row = (long long)blockIdx.x * (4 / WPR) + warp / WPR;
   pdl_wait();
-  if (row >= nrows) return;
-  const float2* ml = p.ml + row * p.NS;
-  float M = -INFINITY;
-  for (int i = lane; i < p.NS; i += 32) M = fmaxf(M, ml[i].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float base = M == -INFINITY ? 0.f : M;
-  float lt = 0.f;
+  const bool live = row < nrows;
+  float M = -INFINITY, lt = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool act = lane * 4 < p.D;
-  const float* op = p.opart + row * p.NS * p.D + lane * 4;
-  for (int s0 = 0; s0 < p.NS; s0 += 32) {
-    const float2 x = s0 + lane < p.NS ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
-    const float f = fast_exp2(x.x - base);
-    lt += f * x.y;
-    const int n = min(32, p.NS - s0);
+  if (live) {
+    const float2* ml = p.ml + row * p.NS;
+    for (int i = lane; i < p.NS; i += 32) M = fmaxf(M, ml[i].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float base = M == -INFINITY ? 0.f : M;
+    const float* op = p.opart + row * p.NS * p.D + lane * 4;
+    for (int s0 = 0; s0 < p.NS; s0 += 32) {
+      const float2 x = s0 + lane < p.NS ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+      const float f = fast_exp2(x.x - base);
+      lt += f * x.y;
+      const int n = min(32, p.NS - s0);
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (fi != 0.f && act) {
-        const float4 v = *reinterpret_cast<const float4*>(op + (long long)(s0 + i) * p.D);
-        acc.x += fi * v.x;
-        acc.y += fi * v.y;
-        acc.z += fi * v.z;
-        acc.w += fi * v.w;
+      for (int i = sub; i < n; i += WPR) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        if (fi != 0.f && act) {
+          const float4 v = *reinterpret_cast<const float4*>(op + (long long)(s0 + i) * p.D);
+          acc.x += fi * v.x;
+          acc.y += fi * v.y;
+          acc.z += fi * v.z;
+          acc.w += fi * v.w;
+        }
       }
     }
-  }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+    for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+  }
+  if constexpr (WPR > 1) {
+    part[warp][lane] = acc;
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+      const float4 x = part[warp + w][lane];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+    }
+  }
+  if (!live) return;
   const float inv = lt > 0.f ? 1.f / lt : 0.f;
   const int tk = (int)(row % p.Sq);
   const long long bh = row / p.Sq;
@@ -365,22 +465,38 @@ struct CachePlan {
   // fields below; ranges cover both)
   bool joint;
   bool tile[2];            // segment by cache_tiles_kernel, otherwise by cache_rows_kernel
-  int mt;                  // 16-row tiles per item of cache_rows_kernel
+  int nt;                  // 8-row tiles per item of cache_rows_kernel
   int rtiles[2], nsplit[2];
   int chunk[2];            // keys per range
   int NS;
 };
 
-// cache_rows_kernel: ranges of one length over its segments, so that about six
-// items per SM exist (two run at a time; the rest evens out ragged lengths)
-// but none is shorter than kMinChunk keys, below which an item's set-up and
-// its partial result cost more than its keys.
-constexpr long long kItemsWanted = 148 * 6;
-constexpr long long kMinChunk = 256;
+// cache_rows_kernel: keys per range.  Four items run on each of the 148 SMs;
+// an item costs its keys plus kRowsCost keys (set-up, first loads, the partial
+// result), and rounds of items are whole.  More than four rounds even out
+// nothing any more.
+constexpr int64_t kRowsSlots = 4 * 148, kRowsCost = 96, kRowsUnit = 32;
+static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
+  const double total = (double)tiles[0] * cap[0] + (double)tiles[1] * cap[1];
+  int64_t best = kRowsUnit;
+  double best_cost = 1e300;
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    // the shortest ranges that fit this many rounds
+    const int64_t slots = rounds * kRowsSlots;
+    int64_t ch = ((int64_t)(total / slots) / kRowsUnit + 1) * kRowsUnit, items = 0;
+    for (;; ch += (ch / 16 / kRowsUnit + 1) * kRowsUnit) {
+      items = tiles[0] * ((cap[0] + ch - 1) / ch) + tiles[1] * ((cap[1] + ch - 1) / ch);
+      if (items <= slots || (ch >= cap[0] && ch >= cap[1])) break;
+    }
+    const double cost = (double)((items + kRowsSlots - 1) / kRowsSlots) * (ch + kRowsCost);
+    if (cost < best_cost) best_cost = cost, best = ch;
+  }
+  return best;
+}
+
 // Most rows for which streaming the keys past warp-level tiles beats a 128-row
 // tcgen05 tile.
 constexpr int64_t kRowsMost = 32;
-constexpr int64_t kTileMinDim = 32;
 
 // cache_tiles_kernel: ranges per tile.  Two items run on each of the 148 SMs;
 // an item costs its blocks plus kItemCost (set-up, first loads, epilogue), and
@@ -390,7 +506,10 @@ static int tile_ranges(int64_t tiles, int64_t blocks) {
   const int64_t slots = 2 * 148;
   int best = 1;
   double best_cost = 1e300;
-  for (int64_t ns = 1; ns <= slots && ns <= blocks; ++ns) {
+  for (int64_t rounds = 0; rounds <= 6; ++rounds) {
+    int64_t ns = rounds * slots / tiles;  // as many ranges as fit these rounds
+    if (ns < 1) ns = 1;
+    if (ns > blocks) ns = blocks;
     const int64_t per = (blocks + ns - 1) / ns;
     const int64_t waves = (tiles * ns + slots - 1) / slots;
     const double cost = (double)waves * (per + kItemCost + (ns > 1 ? kJoinCost : 0));
@@ -400,13 +519,12 @@ static int tile_ranges(int64_t tiles, int64_t blocks) {
 }
 
 static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
-                            int64_t P, int64_t C, int64_t D) {
+                            int64_t P, int64_t C) {
   CachePlan pl{};
   const bool use[2] = {P > 0, C > 0 || P == 0};
   const int64_t rows[2] = {use[0] ? B / G * group * Sq : 0, use[1] ? group * Sq : 0};
   const int64_t cap[2] = {P, C}, nb[2] = {G, B};
-  const bool can = D >= kTileMinDim;
-  for (int s = 0; s < 2; ++s) pl.tile[s] = can && cap[s] > 0 && rows[s] > kRowsMost;
+  for (int s = 0; s < 2; ++s) pl.tile[s] = cap[s] > 0 && rows[s] > kRowsMost;
   // One walk over prefix and own keys where a sequence's rows fill tiles about
   // as well as all sequences' rows together do.
   const int64_t own_tiles = B * ((rows[1] + 127) / 128);
@@ -422,21 +540,19 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
     pl.NS = pl.nsplit[1];
     return pl;
   }
-  double total = 0;
   int64_t most = 0;
   for (int s = 0; s < 2; ++s)
     if (use[s] && !pl.tile[s] && rows[s] > most) most = rows[s];
-  pl.mt = most > 16 ? 2 : 1;
+  pl.nt = most > 16 ? 4 : (most > 8 ? 2 : 1);
+  int64_t tiles[2] = {0, 0};
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
-    const int per = pl.tile[s] ? 128 : 16 * pl.mt;
+    const int per = pl.tile[s] ? 128 : 8 * pl.nt;
     pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
-    if (!pl.tile[s]) total += (double)nb[s] * Hkv * pl.rtiles[s] * cap[s];
+    if (!pl.tile[s]) tiles[s] = nb[s] * Hkv * pl.rtiles[s];
   }
-  int64_t chunk = (int64_t)(total / kItemsWanted) + 1;
-  if (chunk < kMinChunk) chunk = kMinChunk;
-  if (chunk > (1 << 30)) chunk = 1 << 30;
-  chunk = (chunk + 63) & ~63ll;
+  const int64_t caps[2] = {tiles[0] ? cap[0] : 0, tiles[1] ? cap[1] : 0};
+  const int64_t chunk = rows_chunk(tiles, caps);
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
     int64_t ch = chunk;
@@ -456,7 +572,7 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
 static bool cache_sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t G, int64_t P,
                            int64_t C, int64_t D) {
   if (B < 0 || Hq < 0 || Hkv < 1 || Sq < 0 || G < 1 || P < 0 || C < 0) return false;
-  if (D < 8 || D > 128 || D % 8) return false;
+  if (D < 32 || D > 128 || D % 8) return false;
   if (P > (1 << 30) || C > (1 << 30) || P + C > (1 << 30)) return false;
   if (Hq % Hkv || B % G) return false;
   // rows are counted in 32 bits
@@ -492,14 +608,13 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <typename DT, int DK, int MT, bool STATS>
+template <typename DT, int DK, int NT, RowsMode MODE>
 static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
-  using L = RowsSmem<DK, STATS>;
-  constexpr auto kern = cache_rows_kernel<DT, DK, MT, STATS>;
-  constexpr int kJoin = STATS ? 0 : kRowsWarps * 16 * MT * (DK + 4) * 4;
-  constexpr int kQ = 16 * MT * L::kPitch;
-  constexpr int bytes = L::kRing > kJoin ? (L::kRing > kQ ? L::kRing : kQ) : kJoin;
-  cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, MT, STATS>>(bytes);
+  using L = RowsSmem<DK, MODE>;
+  constexpr auto kern = cache_rows_kernel<DT, DK, NT, MODE>;
+  constexpr int kJoin = MODE == kAttention ? kRowsWarps * 8 * NT * (DK + 4) * 4 : 0;
+  constexpr int bytes = L::kRing > kJoin ? L::kRing : kJoin;
+  cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, NT, MODE>>(bytes);
   if (err == cudaSuccess) {
     if (after) {
       err = launch_after(kern, dim3((unsigned)items), 32 * kRowsWarps, bytes, stream, p);
@@ -516,17 +631,24 @@ static int launch_rows(const CacheParams& p, long long items, bool after, cudaSt
   return MI_OK;
 }
 
-template <typename DT, bool STATS>
-static int launch_rows_dk(const CacheParams& p, int mt, long long items, bool after,
+template <RowsMode MODE>
+static int launch_rows_dk(const CacheParams& p, int dtype, int nt, long long items, bool after,
                           cudaStream_t st) {
-  if (p.D <= 64)
-    return mt == 1 ? launch_rows<DT, 64, 1, STATS>(p, items, after, st)
-                   : launch_rows<DT, 64, 2, STATS>(p, items, after, st);
-  if (p.D <= 96)
-    return mt == 1 ? launch_rows<DT, 96, 1, STATS>(p, items, after, st)
-                   : launch_rows<DT, 96, 2, STATS>(p, items, after, st);
-  return mt == 1 ? launch_rows<DT, 128, 1, STATS>(p, items, after, st)
-                 : launch_rows<DT, 128, 2, STATS>(p, items, after, st);
+#define MI_ROWS_CASE(DK)                                                                \
+  if (p.D <= DK) {                                                                      \
+    if (dtype == MI_BF16)                                                               \
+      return nt == 1   ? launch_rows<__nv_bfloat16, DK, 1, MODE>(p, items, after, st)   \
+             : nt == 2 ? launch_rows<__nv_bfloat16, DK, 2, MODE>(p, items, after, st)   \
+                       : launch_rows<__nv_bfloat16, DK, 4, MODE>(p, items, after, st);  \
+    return nt == 1   ? launch_rows<__half, DK, 1, MODE>(p, items, after, st)            \
+           : nt == 2 ? launch_rows<__half, DK, 2, MODE>(p, items, after, st)            \
+                     : launch_rows<__half, DK, 4, MODE>(p, items, after, st);           \
+  }
+  MI_ROWS_CASE(64)
+  MI_ROWS_CASE(96)
+  MI_ROWS_CASE(128)
+#undef MI_ROWS_CASE
+  return MI_ERR_SHAPE;
 }
 
 static void set_seg(CacheSeg& s, const mi_rows& k, const mi_rows& v, const int32_t* len,
@@ -554,7 +676,7 @@ using namespace mib200;
 extern "C" size_t mi_shared_prefix_fwd_workspace_size(const mi_shared_prefix_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, a->G, a->P, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0) return 0;
-  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C, a->D);
+  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C);
   if (pl.NS == 1) return 0;
   const double need = (double)a->B * a->Hq * a->S_q * pl.NS * (a->D * 4 + 8);
   if (need > 1e15) return SIZE_MAX;
@@ -575,7 +697,7 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
     return MI_ERR_ALIGN;
   if (C && (!rows_ok(a.k, B, Hkv, C) || !rows_ok(a.v, B, Hkv, C))) return MI_ERR_ALIGN;
   const int64_t group = Hq / Hkv;
-  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C, D);
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C);
   const size_t need = mi_shared_prefix_fwd_workspace_size(args);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||
@@ -642,15 +764,20 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
   }
   if (rows_items) {
     p.items0 = pl.tile[0] ? 0 : items[0];
-    const int rc = bf ? launch_rows_dk<__nv_bfloat16, false>(p, pl.mt, rows_items, tiles, st)
-                      : launch_rows_dk<__half, false>(p, pl.mt, rows_items, tiles, st);
+    const int rc = launch_rows_dk<kAttention>(p, a.dtype, pl.nt, rows_items, tiles, st);
     if (rc != MI_OK) return rc;
   }
   if (p.NS == 1) return MI_OK;
   const long long nrows = B * Hq * S_q;
-  const dim3 grid((unsigned)((nrows + 3) / 4));
-  const cudaError_t err =
-      bf ? launch_after(cache_combine_kernel<__nv_bfloat16>, grid, 128, 0, st, p, nrows)
-         : launch_after(cache_combine_kernel<__half>, grid, 128, 0, st, p, nrows);
+  // many slots: four warps share a row's
+  const bool wide = p.NS > 8;
+  const dim3 grid((unsigned)(wide ? nrows : (nrows + 3) / 4));
+  cudaError_t err;
+  if (bf)
+    err = wide ? launch_after(cache_combine_kernel<__nv_bfloat16, 4>, grid, 128, 0, st, p, nrows)
+               : launch_after(cache_combine_kernel<__nv_bfloat16, 1>, grid, 128, 0, st, p, nrows);
+  else
+    err = wide ? launch_after(cache_combine_kernel<__half, 4>, grid, 128, 0, st, p, nrows)
+               : launch_after(cache_combine_kernel<__half, 1>, grid, 128, 0, st, p, nrows);
   return err == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

@@ -44,6 +44,13 @@ struct CacheParams {
   int NS;            // partial slots per row (both segments); 1: items write out / lse themselves
   float* opart;      // [rows][NS][D] unnormalised
   float2* ml;        // [rows][NS] (m, l), log2 units
+  // weights of the own caches' keys (cache_rows_kernel, kWeights)
+  const float* z;    // lse of the rows [B, Hq, Sq], times z_mul in log2 units
+  float z_mul;
+  const float* win;  // or null: 0
+  long long wi_b, wi_h;
+  float* wout;
+  long long wo_b, wo_h;
 };
 
 // (sequence, query head, token) of row r of (entry e, kv head h).

@@ -46,14 +46,17 @@ struct TileSmem {
   static constexpr int kKOff = kQBytes;
   static constexpr int kVOff = kKOff + KS * kBlock;
   static constexpr int kBarOff = kVOff + VS * kBlock;
-  // k_full[KS] k_empty[KS] v_full[VS] v_empty[VS] s_full[2] p_full[2] pv_done[2]
-  static constexpr int kNumBars = 2 * KS + 2 * VS + 6;
+  // k_full[KS] k_empty[KS] v_full[VS] v_empty[VS] s_full[2] p_full[2] pv_done[2] q_full
+  static constexpr int kNumBars = 2 * KS + 2 * VS + 7;
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kBytes = kSlotOff + 8;
   static constexpr int kAlloc = kBytes + 512;  // the base is aligned to a swizzle atom
   static constexpr uint32_t kTmemCols = STATS ? 128 : 256;
   static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
   static_assert(STATS || 128 + DK <= 256, "TMEM");
+  // The epilogue stages O in the ring, a padded row per thread.
+  static constexpr int kOPitch = DK * 4 + 16;
+  static_assert(STATS || 128 * kOPitch <= (KS + VS) * kBlock, "O rows fit the ring");
 };
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -62,6 +65,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=l"(reinterpret_cast<uint64_t&>(r))
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return r;
+}
+
+// Untiled bulk copy shared -> global: both 16-byte aligned, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_wait0() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 constexpr int kTileThreads = 192;
@@ -88,6 +101,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   uint64_t* s_full = v_empty + VS;
   uint64_t* p_full = s_full + 2;
   uint64_t* pv_done = p_full + 2;
+  uint64_t* q_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlotOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kSlotOff + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -121,12 +135,13 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int j0 = min(n0 + n1, (int)min((long long)sp * gr.blocks, (long long)(n0 + n1)));
   const int nent = min(n0 + n1 - j0, gr.blocks);
 
-  // ---- set-up: barriers, TMEM, Q (64-byte swizzled chunks of 32 dims) -----------
+  // ---- set-up: barriers, TMEM --------------------------------------------------
   if (threadIdx.x == 0) {
     for (int s = 0; s < KS; ++s) mbar_init(&k_full[s], 1), mbar_init(&k_empty[s], 1);
     for (int s = 0; s < VS; ++s) mbar_init(&v_full[s], 1), mbar_init(&v_empty[s], 1);
     for (int i = 0; i < 2; ++i)
       mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128), mbar_init(&pv_done[i], 1);
+    mbar_init(q_full, 128);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -134,24 +149,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
-  // A negative scale is taken into Q (its sign bits), so that the largest
-  // score is the largest product.
-  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-  if (nent > 0) {
-    for (int i = threadIdx.x; i < 128 * (DK / 8); i += kTileThreads) {
-      const int r = i / (DK / 8), u = i - r * (DK / 8);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < nrows && u * 8 < p.D) {
-        int b, hd, tk;
-        cache_row(p, rs, e, h, r0 + r, b, hd, tk);
-        x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b + hd * p.qs_h + tk * p.qs_s + u * 8);
-        x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
-      }
-      *reinterpret_cast<uint4*>(smem + (u >> 2) * (128 * 64) + r * 64 +
-                                (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x;
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -211,8 +208,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       __syncwarp();
       return true;
     };
-    bool ok = true;
-    if (nent > 0) ok = issue_qk(0);
+    bool ok = __all_sync(0xffffffffu, nent == 0 || mbar_wait(q_full, 0, 130));
+    if (ok && nent > 0) ok = issue_qk(0);
     if (STATS && ok && nent > 1) ok = issue_qk(1);
     for (int j = 0; ok && j < nent; ++j) {
       if (*abort_flag) { ok = false; break; }
@@ -250,8 +247,41 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   } else {
     // ---- softmax: thread = row ---------------------------------------------------
     const int row = threadIdx.x;
-    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
     const bool live = row < nrows;
+    int b = 0, hd = 0, tk = 0;
+    if (live) cache_row(p, rs, e, h, r0 + row, b, hd, tk);
+    // Q: each warp gathers its 32 rows (a lane per 16 bytes, addresses passed
+    // around by shuffle), into chunks of 32 dims with the 64-byte swizzle.  A
+    // negative scale is taken into Q (its sign bits), so that the largest score
+    // is the largest product.
+    if (nent > 0) {
+      constexpr int U = DK / 8, kBatch = U / 2;
+      const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+      const unsigned long long mine = reinterpret_cast<unsigned long long>(
+          p.q + (live ? b * p.qs_b + hd * p.qs_h + tk * p.qs_s : 0));
+#pragma unroll
+      for (int i0 = 0; i0 < U; i0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int idx = (i0 + i) * 32 + lane, r = idx / U, u = idx % U;
+          const unsigned long long a = __shfl_sync(0xffffffffu, mine, r);
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (warp * 32 + r < nrows && u * 8 < p.D)
+            x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + u * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int idx = (i0 + i) * 32 + lane, r = warp * 32 + idx / U, u = idx % U;
+          x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
+          *reinterpret_cast<uint4*>(smem + (u >> 2) * (128 * 64) + r * 64 +
+                                    (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x[i];
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
     int lim0 = len0, lim1 = len1;  // keys that the row sees
     if (live && causal) lim1 = len1 - (p.Sq - 1 - (r0 + row) % p.Sq);
     // Blocks below `full` are whole for every row of the warp, blocks from
@@ -389,14 +419,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       tc_fence_after();
     }
     if (!ok) *abort_flag = 1;
-    int b = 0, hd = 0, tk = 0;
-    if (live) cache_row(p, rs, e, h, r0 + row, b, hd, tk);
     const long long grow = ((long long)b * p.Hq + hd) * p.Sq + tk;
     const bool direct = !STATS && p.NS == 1;
     const bool seen = m != -INFINITY && ok;
-    const float inv = direct ? (seen && l > 0.f ? 1.f / l : 0.f) : 1.f;
     const long long at = grow * p.NS + gr.slot0 + sp;
     if constexpr (!STATS) {
+      // Every product has run, so the ring is free: each thread lays its row
+      // there (padded, so that 16-byte stores of a warp do not collide) and
+      // sends it off with one bulk copy.
+      const float inv = seen && l > 0.f ? 1.f / l : 0.f;
+      uint8_t* orow = smem + L::kKOff + row * L::kOPitch;
       if (nent > 0 || direct) {
 #pragma unroll
         for (int c = 0; c < DK / 32; ++c) {
@@ -406,11 +438,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tmem_ld32(lane_base + 128 + c * 32, o);
             tmem_wait_ld();
           }
+          if (direct) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int d = c * 32 + u * 8;
-            if (d >= p.D || !live || (!direct && !seen)) continue;
-            if (direct) {
+            for (int u = 0; u < 4; ++u) {
               uint4 x = make_uint4(0, 0, 0, 0);
               if (seen) {
                 x.x = DType<DT>::pack2(o[u * 8] * inv, o[u * 8 + 1] * inv);
@@ -418,13 +448,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 x.z = DType<DT>::pack2(o[u * 8 + 4] * inv, o[u * 8 + 5] * inv);
                 x.w = DType<DT>::pack2(o[u * 8 + 6] * inv, o[u * 8 + 7] * inv);
               }
-              *reinterpret_cast<uint4*>(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s + d) = x;
-            } else {
-              float4* dst = reinterpret_cast<float4*>(p.opart + at * p.D + d);
-              dst[0] = make_float4(o[u * 8], o[u * 8 + 1], o[u * 8 + 2], o[u * 8 + 3]);
-              dst[1] = make_float4(o[u * 8 + 4], o[u * 8 + 5], o[u * 8 + 6], o[u * 8 + 7]);
+              *reinterpret_cast<uint4*>(orow + c * 64 + u * 16) = x;
             }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<float4*>(orow + c * 128 + u * 16) =
+                  make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
           }
+        }
+        fence_proxy_async_smem();
+        if (live && ok && (direct || seen)) {
+          if (direct)
+            bulk_store(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s, orow, p.D * 2);
+          else
+            bulk_store(p.opart + at * p.D, orow, p.D * 4);
+          bulk_commit();
+          bulk_wait0();
         }
       }
     }

@@ -23,7 +23,6 @@ struct WeightParams {
   long long wo_b, wo_h;
   int B, Hq, Hkv, group, Sq, C, D, causal;
   float scale_log2;
-  int tiles;  // key tiles per (b, h)
 };
 
 // log-sum-exp (log2 units) of every row from its ranges' (m, l).
@@ -38,95 +37,6 @@ __global__ void weight_lse_kernel(const float2* ml, int NS, float* lse, long lon
       l += x.y * fast_exp2(x.x - M);
     }
   lse[row] = M == -INFINITY ? M : M + log2f(l);
-}
-
-// Few rows: a warp keeps 16 keys (the A operand, so a thread's results belong
-// to two keys and the sum over rows stays in its registers) and walks the
-// query rows eight at a time.  Bound by the bytes of K.
-constexpr int kColsKeys = 64;
-
-template <typename DT, int DK>
-__global__ void __launch_bounds__(128) weight_cols_kernel(const __grid_constant__ WeightParams p) {
-  constexpr int kPitch = DK * 2 + 16, KS = DK / 16, CPR = DK / 8;
-  __shared__ __align__(16) uint8_t sk[kColsKeys * kPitch];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  long long it = blockIdx.x;
-  const int tile = (int)(it % p.tiles);
-  it /= p.tiles;
-  const int h = (int)(it % p.Hkv), b = (int)(it / p.Hkv);
-  const int len = p.len ? min(max(p.len[b], 0), p.C) : p.C;
-  const int k0 = tile * kColsKeys + warp * 16;
-  const float* win = p.win ? p.win + b * p.wi_b + h * p.wi_h : nullptr;
-  float* wout = p.wout + b * p.wo_b + h * p.wo_h;
-  if (k0 >= p.C) return;
-  if (k0 >= len) {  // stale keys: their weights pass through
-    const int j = k0 + lane;
-    if (lane < 16 && j < p.C && (win != wout)) wout[j] = win ? win[j] : 0.f;
-    return;
-  }
-  const uint16_t* kb = p.k + b * p.ks_b + h * p.ks_h;
-  const uint32_t sw = smem_u32(sk) + warp * 16 * kPitch;
-  for (int i = lane; i < 16 * CPR; i += 32) {
-    const int r = i / CPR, c = i - r * CPR;
-    const bool ok = k0 + r < len && c * 8 < p.D;
-    cp16(sw + r * kPitch + c * 16, ok ? kb + (long long)(k0 + r) * p.ks_s + c * 8 : kb, ok);
-  }
-  cp_commit();
-  cp_wait<0>();
-  __syncwarp();
-  uint32_t a[KS][4];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-    ldsm4(a[ks], sw + (lane & 15) * kPitch + ks * 32 + (lane >> 4) * 16);
-
-  const int rows = p.group * p.Sq;
-  // First token that sees this warp's first key, and the row limit of a key.
-  const int slo = p.causal ? max(0, k0 - len + p.Sq) : 0;
-  float tot[2] = {0.f, 0.f};
-  for (int rb = 0; rb < rows; rb += 256) {
-    float part[2] = {0.f, 0.f};  // two-level sums: 32 steps, then the total
-    for (int r0 = rb; r0 < min(rows, rb + 256); r0 += 8) {
-      if (r0 / p.Sq == (r0 + 7) / p.Sq && (r0 + 7) % p.Sq < slo) continue;
-      const int rq = r0 + (lane >> 2);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      const int rr = min(rq, rows - 1);
-      const uint16_t* qp = p.q + b * p.qs_b + (long long)(h * p.group + rr / p.Sq) * p.qs_h +
-                           (long long)(rr % p.Sq) * p.qs_s + (lane & 3) * 2;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const uint32_t b0 = ks * 16 < p.D ? *reinterpret_cast<const uint32_t*>(qp + ks * 16) : 0u;
-        const uint32_t b1 =
-            ks * 16 + 8 < p.D ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + 8) : 0u;
-        mma16816<DT>(c, a[ks], b0, b1);
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = r0 + (lane & 3) * 2 + x;
-        if (r >= rows) continue;
-        const int s = r % p.Sq;
-        const float z = p.lse[((long long)b * p.Hq + h * p.group + r / p.Sq) * p.Sq + s];
-        const float nz = z == -INFINITY ? -INFINITY : -z * p.lse_mul;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int j = k0 + (lane >> 2) + 8 * y;
-          const bool vis = j < len && (!p.causal || j < len - (p.Sq - 1 - s));
-          if (vis) part[y] += fast_exp2(fmaf(c[2 * y + x], p.scale_log2, nz));
-        }
-      }
-    }
-    tot[0] += part[0];
-    tot[1] += part[1];
-  }
-#pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    tot[y] += __shfl_xor_sync(0xffffffffu, tot[y], 1);
-    tot[y] += __shfl_xor_sync(0xffffffffu, tot[y], 2);
-    const int j = k0 + (lane >> 2) + 8 * y;
-    if ((lane & 3) == 0 && j < p.C) {
-      if (j < len) wout[j] = (win ? win[j] : 0.f) + tot[y];
-      else if (win != wout) wout[j] = win ? win[j] : 0.f;
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -408,20 +318,17 @@ static int launch_weight_tiles(const WeightParams& w, const mi_rows& q, const mi
   return MI_OK;
 }
 
-template <typename DT>
-static int launch_cols(const WeightParams& p, const mi_rows& q, const mi_rows& k,
-                       cudaStream_t st) {
-  if ((long long)p.group * p.Sq > kRowsMost && p.D >= kTileMinDim) {
-    if (p.D <= 64) return launch_weight_tiles<DT, 64>(p, q, k, st);
-    if (p.D <= 96) return launch_weight_tiles<DT, 96>(p, q, k, st);
-    return launch_weight_tiles<DT, 128>(p, q, k, st);
-  }
-  const long long items = (long long)p.tiles * p.Hkv * p.B;
-  if (items > 0x7fffffffll) return MI_ERR_SHAPE;
-  if (p.D <= 64) weight_cols_kernel<DT, 64><<<(unsigned)items, 128, 0, st>>>(p);
-  else if (p.D <= 96) weight_cols_kernel<DT, 96><<<(unsigned)items, 128, 0, st>>>(p);
-  else weight_cols_kernel<DT, 128><<<(unsigned)items, 128, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;
+static int launch_weights_many(const WeightParams& p, int dtype, const mi_rows& q,
+                               const mi_rows& k, cudaStream_t st) {
+  const bool bf = dtype == MI_BF16;
+  if (p.D <= 64)
+    return bf ? launch_weight_tiles<__nv_bfloat16, 64>(p, q, k, st)
+              : launch_weight_tiles<__half, 64>(p, q, k, st);
+  if (p.D <= 96)
+    return bf ? launch_weight_tiles<__nv_bfloat16, 96>(p, q, k, st)
+              : launch_weight_tiles<__half, 96>(p, q, k, st);
+  return bf ? launch_weight_tiles<__nv_bfloat16, 128>(p, q, k, st)
+            : launch_weight_tiles<__half, 128>(p, q, k, st);
 }
 
 }  // namespace mib200
@@ -431,7 +338,7 @@ using namespace mib200;
 extern "C" size_t mi_attn_weights_workspace_size(const mi_attn_weights_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, 1, 0, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0 || a->C == 0 || a->lse) return 0;
-  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, 1, 0, a->C, a->D);
+  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, 1, 0, a->C);
   const size_t rows = (size_t)(a->B * a->Hq * a->S_q);
   if ((double)rows * pl.NS > 1e13) return SIZE_MAX;
   return align_up(rows * pl.NS * 8) + align_up(rows * 4);
@@ -459,7 +366,6 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
                (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return MI_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf = dtype == MI_BF16;
   int rc;
 
   WeightParams w{};
@@ -489,41 +395,40 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   w.D = (int)D;
   w.causal = a.causal ? 1 : 0;
   w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  w.tiles = (int)((C + kColsKeys - 1) / kColsKeys);
 
+  // the rows' split, for their statistics and for the few-row form of the weights
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C);
+  const size_t rows = (size_t)(B * Hq * S_q);
+  CacheParams p{};
+  p.q = w.q;
+  p.qs_b = w.qs_b;
+  p.qs_h = w.qs_h;
+  p.qs_s = w.qs_s;
+  p.Hq = w.Hq;
+  p.Hkv = w.Hkv;
+  p.group = w.group;
+  p.Sq = w.Sq;
+  p.D = w.D;
+  p.scale_log2 = w.scale_log2;
+  p.seg[0].seqs = 1;
+  set_seg(p.seg[1], k, k, lengths, C, B, 1, group * S_q, w.causal);
+  p.seg[1].rtiles = pl.rtiles[1];
+  p.seg[1].nsplit = pl.nsplit[1];
+  p.seg[1].chunk = pl.chunk[1];
+  p.NS = pl.NS;
+  const long long items = (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1];
+  if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   if (!lse) {
-    const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C, D);
-    const size_t rows = (size_t)(B * Hq * S_q);
-    CacheParams p{};
-    p.q = w.q;
-    p.qs_b = w.qs_b;
-    p.qs_h = w.qs_h;
-    p.qs_s = w.qs_s;
-    p.Hq = w.Hq;
-    p.Hkv = w.Hkv;
-    p.group = w.group;
-    p.Sq = w.Sq;
-    p.D = w.D;
-    p.scale_log2 = w.scale_log2;
-    p.seg[0].seqs = 1;
-    set_seg(p.seg[1], k, k, lengths, C, B, 1, group * S_q, w.causal);
-    p.seg[1].rtiles = pl.rtiles[1];
-    p.seg[1].nsplit = pl.nsplit[1];
-    p.seg[1].chunk = pl.chunk[1];
-    p.NS = pl.NS;
     p.ml = static_cast<float2*>(workspace);
     float* lse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                            align_up(rows * pl.NS * 8));
-    const long long items = (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1];
-    if (items > 0x7fffffffll) return MI_ERR_SHAPE;
     if (pl.tile[1]) {
       TileParams tp{};
       tp.c = p;
       tp.grp[1] = {1, 0, 1, pl.rtiles[1], pl.nsplit[1], pl.chunk[1] / 64, 0, items};
       rc = launch_tiles<true>(tp, dtype, k, k, k, k, st);
     } else {
-      rc = bf ? launch_rows_dk<__nv_bfloat16, true>(p, pl.mt, items, false, st)
-              : launch_rows_dk<__half, true>(p, pl.mt, items, false, st);
+      rc = launch_rows_dk<kStats>(p, dtype, pl.nt, items, false, st);
     }
     if (rc != MI_OK) return rc;
     weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(p.ml, pl.NS, lse2,
@@ -532,5 +437,14 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
     w.lse = lse2;
     w.lse_mul = 1.f;
   }
-  return bf ? launch_cols<__nv_bfloat16>(w, q, k, st) : launch_cols<__half>(w, q, k, st);
+  if (pl.tile[1]) return launch_weights_many(w, dtype, q, k, st);
+  p.z = w.lse;
+  p.z_mul = w.lse_mul;
+  p.win = w.win;
+  p.wi_b = w.wi_b;
+  p.wi_h = w.wi_h;
+  p.wout = w.wout;
+  p.wo_b = w.wo_b;
+  p.wo_h = w.wo_h;
+  return launch_rows_dk<kWeights>(p, dtype, pl.nt, items, false, st);
 }

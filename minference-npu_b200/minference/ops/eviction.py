@@ -97,7 +97,7 @@ def accumulate_attention_weights(q: torch.Tensor, k: torch.Tensor,
         if weights is None:
             return out.zero_()
         return out if out.data_ptr() == weights.data_ptr() else out.copy_(weights)
-    dk = (D + 7) & ~7
+    dk = max(32, (D + 7) & ~7)
     hold: list = []
     args = _native.ATTN_WEIGHTS_ARGS.pack(
         *rows_arg(q, dk, hold), *rows_arg(k, dk, hold), 0 if lse is None else lse.data_ptr(),

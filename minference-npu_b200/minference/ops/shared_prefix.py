@@ -86,7 +86,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
     elif lengths is not None:
         raise ValueError("lengths without own caches")
 
-    dk = (D + 7) & ~7
+    dk = max(32, (D + 7) & ~7)
     if out is None:
         res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
     else:

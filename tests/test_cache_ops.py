@@ -777,7 +777,7 @@ def test_c_entry_points_refuse():
 
     assert L.mi_shared_prefix_fwd(None, None, 0, None) == 1
     assert attn(dtype=2) == 2
-    for bad in (dict(Hq=3), dict(Hkv=0), dict(G=0), dict(B=3, G=2), dict(D=132), dict(D=60),
+    for bad in (dict(Hq=3), dict(Hkv=0), dict(G=0), dict(B=3, G=2), dict(D=132), dict(D=60), dict(D=24),
                 dict(D=0), dict(P=-1), dict(C=-1), dict(C=1 << 31), dict(Sq=-1),
                 dict(P=1 << 30, C=64), dict(B=1 << 20, Hq=1 << 20)):
         assert attn(**bad) == 1, bad
