@@ -10,10 +10,10 @@ namespace mib200 {
 
 // ---------------------------------------------------------------------------
 // Few rows (1 to 32 per key/value head): a work item is one tile of 8*NT rows
-// against `chunk` keys.  Its two warps take groups of 16 keys in turn; each
+// against `chunk` keys.  Its warps take groups of 16 keys in turn; each
 // warp streams its own groups through its own shared-memory ring (cp.async)
 // and keeps its own running maximum, sum and O, so there is no barrier in the
-// loop.  The two states are joined at the end.  Keys are the M side of both
+// loop.  Their states are joined at the end.  Keys are the M side of both
 // products, so that a single row costs an 8-wide tile, not a 16-wide one:
 //   S^T (16 keys x 8 rows) = K Q^T     Q fragments stay in registers
 //   O^T (D x 8 rows) += V^T P^T        P^T is S^T's registers rounded to the
@@ -28,26 +28,33 @@ namespace mib200 {
 // (all rows of the key/value head, at most 32) and added to win; no V.
 // ---------------------------------------------------------------------------
 enum RowsMode { kAttention, kStats, kWeights };
-constexpr int kRowsWarps = 2;
 
-template <int DK, RowsMode MODE>
+template <int DK, int NT, RowsMode MODE>
 struct RowsSmem {
+  // Four blocks per SM either way: with one 8-row tile a warp waits on its own
+  // instruction latencies more than on memory, so four warps share the bytes in
+  // flight; taller tiles have the work, and the registers, of two.
+  static constexpr int W = NT == 1 ? 4 : 2;
   static constexpr int kPitch = DK * 2 + 16;
   static constexpr int kTile = 16 * kPitch;  // 16 keys of K or V
   // one warp's stage; kWeights: and 16 of win
   static constexpr int kStage = MODE == kAttention ? 2 * kTile
                                                    : kTile + (MODE == kWeights ? 64 : 0);
-  // about 52 KB a block: four per SM
-  static constexpr int ST = (DK == 64 ? 6 : (DK == 96 ? 4 : 3)) * (MODE == kAttention ? 1 : 2) -
-                            (MODE == kAttention ? 0 : 1);
+  // about 52 KB a block (70 KB and three blocks per SM for D = 128, NT = 1)
+  static constexpr int kFit =
+      (MODE == kAttention && DK == 128 && W == 4 ? 70 * 1024 : 55 * 1024) / (W * kStage);
+  static constexpr int ST = kFit > 8 ? 8 : kFit;
+  static_assert(ST >= 2, "a stage to load beside the one in use");
   static constexpr int kWarpRing = ST * kStage;
-  static constexpr int kRing = kRowsWarps * kWarpRing;
+  static constexpr int kRing = W * kWarpRing;
 };
 
 template <typename DT, int DK, int NT, RowsMode MODE>
-__global__ void __launch_bounds__(32 * kRowsWarps, 4)
+__global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
+                                  MODE == kAttention && DK == 128 && NT == 1 ? 3 : 4)
     cache_rows_kernel(const __grid_constant__ CacheParams p) {
-  using L = RowsSmem<DK, MODE>;
+  using L = RowsSmem<DK, NT, MODE>;
+  constexpr int kRowsWarps = L::W;
   constexpr int KS = DK / 16, R = 8 * NT, CPR = DK / 8;
   constexpr bool kO = MODE == kAttention;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -55,16 +62,13 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
 
-  long long it = blockIdx.x;
+  int it = blockIdx.x, rt, sp, h;
   const bool own = it >= p.items0;
   if (own) it -= p.items0;
   const CacheSeg& sg = p.seg[own ? 1 : 0];
-  const int rt = (int)(it % sg.rtiles);
-  it /= sg.rtiles;
-  const int sp = (int)(it % sg.nsplit);
-  it /= sg.nsplit;
-  const int h = (int)(it % p.Hkv);
-  const int e = (int)(it / p.Hkv);
+  it = sg.rtiles.divmod(it, rt);
+  it = sg.nsplit.divmod(it, sp);
+  const int e = p.div_hkv.divmod(it, h);
   const int r0 = rt * R;
   const int nrows = min(R, sg.rows - r0);
   const int len = cache_len(sg, e);
@@ -73,7 +77,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
   int end = len;
   if (sg.causal) {
     const int last = r0 + nrows - 1;
-    const int smax = (r0 / p.Sq != last / p.Sq) ? p.Sq - 1 : last % p.Sq;
+    int smax;
+    if (p.div_sq.divmod(last, smax) != p.div_sq.div(r0)) smax = p.Sq - 1;
     end = max(0, len - (p.Sq - 1 - smax));
   }
   const int kb = sp * sg.chunk;
@@ -120,60 +125,61 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
     cp_commit();
   };
 
-  // ---- Q tile -> shared (the last ring stage, loaded last) -> fragments ----------
-  // Every warp fetches the tile for itself, beside its first keys.
+  // ---- Q tile: every warp fetches it for itself, ahead of its first keys (whose
+  // loads would otherwise queue before it), through the ring stage that is
+  // loaded last, 16 rows at a time, into fragments ------------------------------
+  uint32_t qf[NT][KS][2];
+  uint8_t* qs = smem + warp * L::kWarpRing + (L::ST - 1) * L::kStage;
+  static_assert(16 * L::kPitch <= L::kStage, "16 rows of Q fit a stage");
+  constexpr int kQRows = NT == 1 ? 8 : 16, kQIter = kQRows * CPR / 32;
+  uint4 qx[kQIter];
+  auto fetch_q = [&](int half) {
+    const int hr = half * 16 + (lane & 15);  // row whose address this lane works out
+    const uint16_t* qp = p.q;
+    if (hr < nrows) {
+      int b, hd, tk;
+      cache_row(p, sg, e, h, r0 + hr, b, hd, tk);
+      qp += b * p.qs_b + hd * p.qs_h + tk * p.qs_s;
+    }
+#pragma unroll
+    for (int i = 0; i < kQIter; ++i) {
+      const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
+      const unsigned long long a =
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(qp), r);
+      qx[i] = make_uint4(0, 0, 0, 0);
+      if (half * 16 + r < nrows && c * 8 < p.D)
+        qx[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + c * 8);
+    }
+  };
+  fetch_q(0);
 #pragma unroll
   for (int s = 0; s < L::ST - 1; ++s) load(warp + s * kRowsWarps);
-  uint32_t qf[NT][KS][2];
+#pragma unroll
+  for (int half = 0; half < (NT + 1) / 2; ++half) {
+    if (half) fetch_q(half);
+#pragma unroll
+    for (int i = 0; i < kQIter; ++i) {
+      const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
+      *reinterpret_cast<uint4*>(qs + r * L::kPitch + c * 16) = qx[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if (half * 2 + n >= NT) break;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks += 2) {
+        uint32_t b[4];
+        ldsm4(b, smem_u32(qs) + (n * 8 + (lane & 7)) * L::kPitch + ks * 32 + (lane >> 3) * 16);
+        qf[half * 2 + n][ks][0] = b[0];
+        qf[half * 2 + n][ks][1] = b[1];
+        qf[half * 2 + n][ks + 1][0] = b[2];
+        qf[half * 2 + n][ks + 1][1] = b[3];
+      }
+    }
+    __syncwarp();
+  }
   int lim[NT][2];  // keys that row 8n + (lane&3)*2 + x sees
   int minlim = 0x7fffffff;
-  {
-    uint8_t* qs = smem + warp * L::kWarpRing + (L::ST - 1) * L::kStage;
-    static_assert(16 * L::kPitch <= L::kStage, "16 rows of Q fit a stage");
-#pragma unroll
-    for (int half = 0; half < (NT + 1) / 2; ++half) {
-      const int hr = half * 16 + (lane & 15);  // row whose address this lane works out
-      const uint16_t* qp = p.q;
-      if (hr < nrows) {
-        int b, hd, tk;
-        cache_row(p, sg, e, h, r0 + hr, b, hd, tk);
-        qp += b * p.qs_b + hd * p.qs_h + tk * p.qs_s;
-      }
-      constexpr int kRows = NT == 1 ? 8 : 16;
-      constexpr int kIter = kRows * CPR / 32;
-      uint4 x[kIter];
-#pragma unroll
-      for (int i = 0; i < kIter; ++i) {
-        const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
-        const unsigned long long a =
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(qp), r);
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (half * 16 + r < nrows && c * 8 < p.D)
-          x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + c * 8);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kIter; ++i) {
-        const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
-        *reinterpret_cast<uint4*>(qs + r * L::kPitch + c * 16) = x[i];
-      }
-      __syncwarp();
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        if (half * 2 + n >= NT) break;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks += 2) {
-          uint32_t b[4];
-          ldsm4(b, smem_u32(qs) + (n * 8 + (lane & 7)) * L::kPitch + ks * 32 + (lane >> 3) * 16);
-          qf[half * 2 + n][ks][0] = b[0];
-          qf[half * 2 + n][ks][1] = b[1];
-          qf[half * 2 + n][ks + 1][0] = b[2];
-          qf[half * 2 + n][ks + 1][1] = b[3];
-        }
-      }
-      __syncwarp();
-    }
-  }
   float nz[NT][2];  // kWeights: -lse (log2 units; -inf: the row adds nothing)
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -183,12 +189,13 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
       lim[n][x] = 0;
       nz[n][x] = -INFINITY;
       if (r < nrows) {
-        const int tok = (r0 + r) % p.Sq;
+        int tok;
+        const int g = p.div_sq.divmod(r0 + r, tok);
         lim[n][x] = sg.causal ? len - (p.Sq - 1 - tok) : len;
         minlim = min(minlim, lim[n][x]);
         if constexpr (MODE == kWeights) {
           const float z =
-              p.z[((long long)e * p.Hq + h * p.group + (r0 + r) / p.Sq) * p.Sq + tok];
+              p.z[((long long)e * p.Hq + h * p.group + g) * p.Sq + tok];
           if (z != -INFINITY) nz[n][x] = -z * p.z_mul;
         }
       }
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
     return;
   }
 
-  // ---- join the two warps -----------------------------------------------------
+  // ---- join the warps ---------------------------------------------------------
   constexpr int kOP = DK + 4;  // floats per row of O in shared memory
   __syncthreads();
 #pragma unroll
@@ -380,54 +387,71 @@ __global__ void __launch_bounds__(32 * kRowsWarps, 4)
       if (c == 0) p.ml[at] = make_float2(M, lt);
     }
   }
-  // The tile kernel of the same call may still run: end after it, so that what
-  // waits for this kernel waits for both.
+  // The kernel that this call launched before may still run: end after it, so
+  // that what waits for this kernel waits for both.
   pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
 // Joins the partial results of a row: WPR warps per row, each with every
-// WPR-th slot, a lane per 4 dims.  Slots without a visible key have m = -inf
-// and are not read.
+// WPR-th slot, a lane per 4 dims.  Bound by latency, so a warp asks for its
+// first eight slots before it knows their weights.  Slots without a visible
+// key have m = -inf; what lies there is not used.
 // ---------------------------------------------------------------------------
 template <typename DT, int WPR>
-__global__ void __launch_bounds__(128) cache_combine_kernel(const __grid_constant__ CacheParams p,
-                                                            long long nrows) {
-  __shared__ float4 part[4][32];
+__global__ void __launch_bounds__(WPR > 4 ? 32 * WPR : 128)
+    cache_combine_kernel(const __grid_constant__ CacheParams p, long long nrows) {
+  constexpr int kWarps = WPR > 4 ? WPR : 4, kBatch = 8;
+  __shared__ float4 part[kWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = warp % WPR;
-  const long long row = (long long)blockIdx.x * (4 / WPR) + warp / WPR;
+  const long long row = (long long)blockIdx.x * (kWarps / WPR) + warp / WPR;
   pdl_wait();
   const bool live = row < nrows;
+  const bool act = lane * 4 < p.D;
   float M = -INFINITY, lt = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const bool act = lane * 4 < p.D;
   if (live) {
     const float2* ml = p.ml + row * p.NS;
-    for (int i = lane; i < p.NS; i += 32) M = fmaxf(M, ml[i].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float base = M == -INFINITY ? 0.f : M;
     const float* op = p.opart + row * p.NS * p.D + lane * 4;
-    for (int s0 = 0; s0 < p.NS; s0 += 32) {
-      const float2 x = s0 + lane < p.NS ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
-      const float f = fast_exp2(x.x - base);
-      lt += f * x.y;
-      const int n = min(32, p.NS - s0);
-#pragma unroll 8
-      for (int i = sub; i < n; i += WPR) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        if (fi != 0.f && act) {
-          const float4 v = *reinterpret_cast<const float4*>(op + (long long)(s0 + i) * p.D);
-          acc.x += fi * v.x;
-          acc.y += fi * v.y;
-          acc.z += fi * v.z;
-          acc.w += fi * v.w;
+    float4 v[kBatch];
+    float2 x[kBatch];
+    auto fetch = [&](int s0) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + i * WPR;
+        x[i] = s < p.NS ? ml[s] : make_float2(-INFINITY, 0.f);
+        if (s < p.NS && act) v[i] = *reinterpret_cast<const float4*>(op + (long long)s * p.D);
+      }
+    };
+    fetch(sub);
+    for (int i = lane; i < p.NS; i += 32) {
+      const float2 y = ml[i];
+      const float mn = fmaxf(M, y.x);
+      if (mn != -INFINITY) lt = lt * fast_exp2(M - mn) + y.y * fast_exp2(y.x - mn);
+      M = mn;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, M, o);
+      const float l2 = __shfl_xor_sync(0xffffffffu, lt, o);
+      const float mn = fmaxf(M, m2);
+      if (mn != -INFINITY) lt = lt * fast_exp2(M - mn) + l2 * fast_exp2(m2 - mn);
+      M = mn;
+    }
+    for (int s0 = sub; s0 < p.NS; s0 += kBatch * WPR) {
+      if (s0 != sub) fetch(s0);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (x[i].x != -INFINITY) {
+          const float f = fast_exp2(x[i].x - M);
+          acc.x += f * v[i].x;
+          acc.y += f * v[i].y;
+          acc.z += f * v[i].z;
+          acc.w += f * v[i].w;
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
   }
   if constexpr (WPR > 1) {
     part[warp][lane] = acc;
@@ -435,11 +459,11 @@ __global__ void __launch_bounds__(128) cache_combine_kernel(const __grid_constan
     if (sub) return;
 #pragma unroll
     for (int w = 1; w < WPR; ++w) {
-      const float4 x = part[warp + w][lane];
-      acc.x += x.x;
-      acc.y += x.y;
-      acc.z += x.z;
-      acc.w += x.w;
+      const float4 y = part[warp + w][lane];
+      acc.x += y.x;
+      acc.y += y.y;
+      acc.z += y.z;
+      acc.w += y.w;
     }
   }
   if (!live) return;
@@ -465,22 +489,27 @@ struct CachePlan {
   // fields below; ranges cover both)
   bool joint;
   bool tile[2];            // segment by cache_tiles_kernel, otherwise by cache_rows_kernel
-  int nt;                  // 8-row tiles per item of cache_rows_kernel
+  int nt[2];               // 8-row tiles per item of cache_rows_kernel
   int rtiles[2], nsplit[2];
   int chunk[2];            // keys per range
   int NS;
 };
 
-// cache_rows_kernel: keys per range.  Four items run on each of the 148 SMs;
-// an item costs its keys plus kRowsCost keys (set-up, first loads, the partial
-// result), and rounds of items are whole.  More than four rounds even out
-// nothing any more.
-constexpr int64_t kRowsSlots = 4 * 148, kRowsCost = 96, kRowsUnit = 32;
-static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
+// cache_rows_kernel: keys per range.  Four items run on each of the 148 SMs.
+// An item costs its keys plus `extra` keys (set-up, first loads, the partial
+// result: 1 us for an 8-row tile, 4 us for taller ones, at 27 keys a
+// microsecond and block).  Items of several rounds start as others end, so
+// they fill the device but for a third of an item at the end; those of a
+// single round all wait for the slowest (15 % behind).  The join costs 4 us.  Measured on a 16384-key prefix of 32 heads:
+// 16 rows 42 us at 1024 keys a range (one round), 47 at 512, 54 at 256; 8 rows
+// 39, 39, 41; two 65536-key caches 218, 215, 216.
+constexpr int64_t kRowsSlots = 4 * 148, kRowsUnit = 32;
+static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2], int nt) {
+  const int64_t extra = nt == 1 ? 32 : 108;
   const double total = (double)tiles[0] * cap[0] + (double)tiles[1] * cap[1];
   int64_t best = kRowsUnit;
   double best_cost = 1e300;
-  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+  for (int64_t rounds = 1; rounds <= 16; rounds += rounds < 4 ? 1 : 4) {
     // the shortest ranges that fit this many rounds
     const int64_t slots = rounds * kRowsSlots;
     int64_t ch = ((int64_t)(total / slots) / kRowsUnit + 1) * kRowsUnit, items = 0;
@@ -488,7 +517,9 @@ static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
       items = tiles[0] * ((cap[0] + ch - 1) / ch) + tiles[1] * ((cap[1] + ch - 1) / ch);
       if (items <= slots || (ch >= cap[0] && ch >= cap[1])) break;
     }
-    const double cost = (double)((items + kRowsSlots - 1) / kRowsSlots) * (ch + kRowsCost);
+    const double fill = (double)items / kRowsSlots;
+    double cost = (fill <= 1 ? 1.15 : fill + 0.3) * (ch + extra);
+    if (ch < cap[0] || ch < cap[1]) cost += 110;
     if (cost < best_cost) best_cost = cost, best = ch;
   }
   return best;
@@ -540,19 +571,17 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
     pl.NS = pl.nsplit[1];
     return pl;
   }
-  int64_t most = 0;
-  for (int s = 0; s < 2; ++s)
-    if (use[s] && !pl.tile[s] && rows[s] > most) most = rows[s];
-  pl.nt = most > 16 ? 4 : (most > 8 ? 2 : 1);
   int64_t tiles[2] = {0, 0};
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
-    const int per = pl.tile[s] ? 128 : 8 * pl.nt;
+    pl.nt[s] = rows[s] > 16 ? 4 : (rows[s] > 8 ? 2 : 1);
+    const int per = pl.tile[s] ? 128 : 8 * pl.nt[s];
     pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
     if (!pl.tile[s]) tiles[s] = nb[s] * Hkv * pl.rtiles[s];
   }
   const int64_t caps[2] = {tiles[0] ? cap[0] : 0, tiles[1] ? cap[1] : 0};
-  const int64_t chunk = rows_chunk(tiles, caps);
+  const int nt = tiles[0] && pl.nt[0] > pl.nt[1] ? pl.nt[0] : pl.nt[1];
+  const int64_t chunk = rows_chunk(tiles, caps, nt);
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
     int64_t ch = chunk;
@@ -610,7 +639,8 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
 
 template <typename DT, int DK, int NT, RowsMode MODE>
 static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
-  using L = RowsSmem<DK, MODE>;
+  using L = RowsSmem<DK, NT, MODE>;
+  constexpr int kRowsWarps = L::W;
   constexpr auto kern = cache_rows_kernel<DT, DK, NT, MODE>;
   constexpr int kJoin = MODE == kAttention ? kRowsWarps * 8 * NT * (DK + 4) * 4 : 0;
   constexpr int bytes = L::kRing > kJoin ? L::kRing : kJoin;
@@ -669,6 +699,17 @@ static void set_seg(CacheSeg& s, const mi_rows& k, const mi_rows& v, const int32
   s.causal = causal;
 }
 
+static void set_heads(CacheParams& p, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.group = (int)(Hq / Hkv);
+  p.Sq = (int)Sq;
+  p.D = (int)D;
+  p.div_hkv = FastDiv(Hkv);
+  p.div_sq = FastDiv(Sq);
+  p.div_rows = FastDiv(Hq / Hkv * Sq);
+}
+
 }  // namespace mib200
 
 using namespace mib200;
@@ -714,17 +755,13 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
   p.os_h = a.out.stride_h;
   p.os_s = a.out.stride_s;
   p.lse = a.lse;
-  p.Hq = (int)Hq;
-  p.Hkv = (int)Hkv;
-  p.group = (int)group;
-  p.Sq = (int)S_q;
-  p.D = (int)D;
+  set_heads(p, Hq, Hkv, S_q, D);
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   set_seg(p.seg[0], a.k_prefix, a.v_prefix, a.prefix_lengths, P, G, B / G, B / G * group * S_q, 0);
   set_seg(p.seg[1], a.k, a.v, a.lengths, C, B, 1, group * S_q, a.causal ? 1 : 0);
   for (int s = 0; s < 2; ++s) {
-    p.seg[s].rtiles = pl.rtiles[s];
-    p.seg[s].nsplit = pl.nsplit[s];
+    p.seg[s].rtiles = FastDiv(pl.rtiles[s]);
+    p.seg[s].nsplit = FastDiv(pl.nsplit[s]);
     p.seg[s].chunk = pl.chunk[s];
   }
   p.seg[1].slot0 = pl.nsplit[0];
@@ -740,44 +777,47 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a.dtype == MI_BF16;
   TileParams tp{};
-  long long rows_items = 0;
   for (int s = 0; s < 2; ++s) {
-    if (!pl.tile[s]) {
-      rows_items += items[s];
-      continue;
-    }
+    if (!pl.tile[s]) continue;
     TileGroup& g = tp.grp[s];
     g.rows_of = s;
     g.use0 = s == 0 || pl.joint;
     g.use1 = s == 1;
-    g.rtiles = pl.rtiles[s];
-    g.nsplit = pl.nsplit[s];
+    g.rtiles = FastDiv(pl.rtiles[s]);
+    g.nsplit = FastDiv(pl.nsplit[s]);
     g.blocks = pl.chunk[s] / 64;
     g.slot0 = p.seg[s].slot0;
-    g.items = items[s];
+    g.items = (int)items[s];
   }
   const bool tiles = pl.tile[0] || pl.tile[1];
   if (tiles) {
     tp.c = p;
-    const int rc = launch_tiles<false>(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, st);
+    const int rc = launch_tiles(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, st);
     if (rc != MI_OK) return rc;
   }
-  if (rows_items) {
-    p.items0 = pl.tile[0] ? 0 : items[0];
-    const int rc = launch_rows_dk<kAttention>(p, a.dtype, pl.nt, rows_items, tiles, st);
+  // Both segments in one launch where they take tiles of the same height,
+  // else one after the other (the second starts as the first's blocks end).
+  bool after = tiles;
+  for (int s = 0; s < 2; ++s) {
+    if (pl.tile[s] || !items[s]) continue;
+    const bool both = s == 0 && !pl.tile[1] && items[1] && pl.nt[0] == pl.nt[1];
+    p.items0 = s == 0 ? (int)items[0] : 0;
+    const int rc = launch_rows_dk<kAttention>(p, a.dtype, pl.nt[s],
+                                              items[s] + (both ? items[1] : 0), after, st);
     if (rc != MI_OK) return rc;
+    if (both) break;
+    after = true;
   }
   if (p.NS == 1) return MI_OK;
   const long long nrows = B * Hq * S_q;
-  // many slots: four warps share a row's
-  const bool wide = p.NS > 8;
-  const dim3 grid((unsigned)(wide ? nrows : (nrows + 3) / 4));
-  cudaError_t err;
-  if (bf)
-    err = wide ? launch_after(cache_combine_kernel<__nv_bfloat16, 4>, grid, 128, 0, st, p, nrows)
-               : launch_after(cache_combine_kernel<__nv_bfloat16, 1>, grid, 128, 0, st, p, nrows);
-  else
-    err = wide ? launch_after(cache_combine_kernel<__half, 4>, grid, 128, 0, st, p, nrows)
-               : launch_after(cache_combine_kernel<__half, 1>, grid, 128, 0, st, p, nrows);
+  // a warp joins up to eight slots at once; many rows need fewer warps each
+  const int wpr = p.NS <= 8 || nrows >= 16384 ? 1 : (p.NS <= 32 || nrows >= 4096 ? 4 : 8);
+  const dim3 grid((unsigned)(wpr == 1 ? (nrows + 3) / 4 : nrows));
+#define MI_JOIN(W)                                                                            \
+  (bf ? launch_after(cache_combine_kernel<__nv_bfloat16, W>, grid, W > 4 ? 32 * W : 128, 0,   \
+                     st, p, nrows)                                                            \
+      : launch_after(cache_combine_kernel<__half, W>, grid, W > 4 ? 32 * W : 128, 0, st, p, nrows))
+  const cudaError_t err = wpr == 1 ? MI_JOIN(1) : (wpr == 4 ? MI_JOIN(4) : MI_JOIN(8));
+#undef MI_JOIN
   return err == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

@@ -16,6 +16,33 @@
 
 namespace mib200 {
 
+// Division of 0 <= n < 2^31 by a divisor known on the host: one multiplication
+// and a shift.  With 2^(s-1) < d <= 2^s and m = floor(2^(31+s) / d) + 1, the
+// product n m exceeds 2^(31+s) n / d by at most n 2^s / d < 2^(31+s) / d, too
+// little to reach the next quotient.
+struct FastDiv {
+  uint32_t d, m;
+  int shift;
+  FastDiv() = default;
+  __host__ explicit FastDiv(int64_t v) {
+    d = (uint32_t)(v < 1 ? 1 : v);
+    int s = 0;
+    while ((1ull << s) < d) ++s;
+    shift = 31 + s;
+    m = (uint32_t)((1ull << shift) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)(((uint64_t)(uint32_t)n * m) >> shift);
+  }
+  // n / d and n % d
+  __device__ __forceinline__ int divmod(int n, int& rem) const {
+    const int q = div(n);
+    rem = n - q * (int)d;
+    return q;
+  }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
+
 struct CacheSeg {
   const uint16_t* k;
   const uint16_t* v;
@@ -25,8 +52,8 @@ struct CacheSeg {
   int nb;      // batch entries (prefixes, or sequences)
   int seqs;    // sequences per batch entry
   int rows;    // query rows per (entry, kv head): seqs * group * Sq
-  int rtiles;  // row tiles
-  int nsplit, chunk;
+  FastDiv rtiles, nsplit;  // row tiles; key ranges
+  int chunk;               // keys per range
   int slot0;   // first partial slot
   int causal;  // rows see keys < len - (Sq - 1 - s); otherwise every valid key
 };
@@ -38,9 +65,10 @@ struct CacheParams {
   long long os_b, os_h, os_s;
   float* lse;  // [B, Hq, Sq] natural logarithm, or null
   int Hq, Hkv, group, Sq, D;
+  FastDiv div_hkv, div_sq, div_rows;  // by Hkv, Sq and group * Sq
   float scale_log2;
   CacheSeg seg[2];
-  long long items0;  // work items of segment 0
+  int items0;        // work items of segment 0
   int NS;            // partial slots per row (both segments); 1: items write out / lse themselves
   float* opart;      // [rows][NS][D] unnormalised
   float2* ml;        // [rows][NS] (m, l), log2 units
@@ -56,16 +84,53 @@ struct CacheParams {
 // (sequence, query head, token) of row r of (entry e, kv head h).
 __device__ __forceinline__ void cache_row(const CacheParams& p, const CacheSeg& s, int e, int h,
                                           int r, int& b, int& head, int& tok) {
-  const int per = p.group * p.Sq;
-  const int i = r / per, rem = r - i * per;
-  const int g = rem / p.Sq;
+  int rem;
+  const int i = p.div_rows.divmod(r, rem);
+  const int g = p.div_sq.divmod(rem, tok);
   b = e * s.seqs + i;
   head = h * p.group + g;
-  tok = rem - g * p.Sq;
 }
 
 __device__ __forceinline__ int cache_len(const CacheSeg& s, int e) {
   return s.len ? min(max(s.len[e], 0), s.cap) : s.cap;
+}
+
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe; x is held to [-126, 126].
+// x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low
+// bits), 2^f by a polynomial of degree 5, the minimax one for the relative
+// error over [-1/2, 1/2] found by Remez exchange (7.5e-8), n into the exponent.
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  x.x = fminf(fmaxf(x.x, -126.f), 126.f);
+  x.y = fminf(fmaxf(x.y, -126.f), 126.f);
+  const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
+  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 r = make_float2(1.3276472e-3f, 1.3276472e-3f);
+  r = fma2(r, f, make_float2(9.6755413e-3f, 9.6755413e-3f));
+  r = fma2(r, f, make_float2(5.5507133e-2f, 5.5507133e-2f));
+  r = fma2(r, f, make_float2(2.4022120e-1f, 2.4022120e-1f));
+  r = fma2(r, f, make_float2(6.9314697e-1f, 6.9314697e-1f));
+  r = fma2(r, f, make_float2(1.0000001f, 1.0000001f));
+  r.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
+  r.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
+  return r;
 }
 
 }  // namespace mib200

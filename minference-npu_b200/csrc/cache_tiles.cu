@@ -11,8 +11,6 @@
 // gathered with plain loads; row sums are kept in registers, because at
 // D = 128 O fills what the two S buffers leave of half the TMEM; O leaves
 // unnormalised (or finished, when the item has the whole row).
-//
-// STATS computes the rows' (maximum, sum) only: no V, no P, no O.
 #include <cstring>
 
 #include "cache_attn.cuh"
@@ -25,9 +23,10 @@ namespace mib200 {
 struct TileGroup {
   int rows_of;
   int use0, use1;
-  int rtiles, nsplit, blocks;  // blocks: key blocks per range
+  FastDiv rtiles, nsplit;
+  int blocks;  // key blocks per range
   int slot0;
-  long long items;
+  int items;
 };
 
 struct TileParams {
@@ -35,14 +34,14 @@ struct TileParams {
   TileGroup grp[2];
 };
 
-template <int DK, bool STATS>
+template <int DK>
 struct TileSmem {
   static constexpr int NC = DK / 32;
   static constexpr int kQBytes = NC * 128 * 64;
   static constexpr int kBlock = NC * 64 * 64;  // 64 keys of K or V
   // two blocks per SM: 113 KB each at most
-  static constexpr int KS = STATS ? (DK == 128 ? 4 : 5) : (DK == 128 ? 2 : (DK == 96 ? 3 : 5));
-  static constexpr int VS = STATS ? 0 : (DK == 128 ? 3 : (DK == 96 ? 4 : 5));
+  static constexpr int KS = DK == 128 ? 2 : (DK == 96 ? 3 : 5);
+  static constexpr int VS = DK == 128 ? 3 : (DK == 96 ? 4 : 5);
   static constexpr int kKOff = kQBytes;
   static constexpr int kVOff = kKOff + KS * kBlock;
   static constexpr int kBarOff = kVOff + VS * kBlock;
@@ -51,21 +50,13 @@ struct TileSmem {
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kBytes = kSlotOff + 8;
   static constexpr int kAlloc = kBytes + 512;  // the base is aligned to a swizzle atom
-  static constexpr uint32_t kTmemCols = STATS ? 128 : 256;
+  static constexpr uint32_t kTmemCols = 256;
   static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
-  static_assert(STATS || 128 + DK <= 256, "TMEM");
+  static_assert(128 + DK <= 256, "TMEM");
   // The epilogue stages O in the ring, a padded row per thread.
   static constexpr int kOPitch = DK * 4 + 16;
-  static_assert(STATS || 128 * kOPitch <= (KS + VS) * kBlock, "O rows fit the ring");
+  static_assert(128 * kOPitch <= (KS + VS) * kBlock, "O rows fit the ring");
 };
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(r))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return r;
-}
 
 // Untiled bulk copy shared -> global: both 16-byte aligned, a multiple of 16 bytes.
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
@@ -80,14 +71,14 @@ __device__ __forceinline__ void bulk_wait0() {
 constexpr int kTileThreads = 192;
 constexpr float kTileRescale = 12.0f;  // log2 growth of a row's maximum that rescales O
 
-template <typename DT, int DK, bool STATS>
+template <typename DT, int DK>
 __global__ void __launch_bounds__(kTileThreads, 2)
     cache_tiles_kernel(const __grid_constant__ CUtensorMap tm_kp,
                        const __grid_constant__ CUtensorMap tm_vp,
                        const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v,
                        const __grid_constant__ TileParams tp) {
-  using L = TileSmem<DK, STATS>;
+  using L = TileSmem<DK>;
   constexpr int NC = L::NC, KS = L::KS, VS = L::VS;
   constexpr bool kBF16 = DType<DT>::kBF16;
   const CacheParams& p = tp.c;
@@ -108,17 +99,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   pdl_launch();
 
   // ---- the item ---------------------------------------------------------------
-  long long it = blockIdx.x;
+  int it = blockIdx.x, rt, sp, h;
   const bool second = it >= tp.grp[0].items;
   if (second) it -= tp.grp[0].items;
   const TileGroup& gr = tp.grp[second ? 1 : 0];
   const CacheSeg& rs = p.seg[gr.rows_of];
-  const int rt = (int)(it % gr.rtiles);
-  it /= gr.rtiles;
-  const int sp = (int)(it % gr.nsplit);
-  it /= gr.nsplit;
-  const int h = (int)(it % p.Hkv);
-  const int e = (int)(it / p.Hkv);                        // entry of the row segment
+  it = gr.rtiles.divmod(it, rt);
+  it = gr.nsplit.divmod(it, sp);
+  const int e = p.div_hkv.divmod(it, h);                         // entry of the row segment
   const int e0 = gr.rows_of == 0 ? e : e / p.seg[0].seqs;  // prefix
   const int r0 = rt * 128;
   const int nrows = min(128, rs.rows - r0);
@@ -128,7 +116,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   int end1 = len1;  // own keys that the tile's last token sees
   if (gr.use1 && causal) {
     const int last = r0 + nrows - 1;
-    const int smax = (r0 / p.Sq != last / p.Sq) ? p.Sq - 1 : last % p.Sq;
+    int smax;
+    if (p.div_sq.divmod(last, smax) != p.div_sq.div(r0)) smax = p.Sq - 1;
     end1 = max(0, len1 - (p.Sq - 1 - smax));
   }
   const int n0 = (len0 + 63) >> 6, n1 = (end1 + 63) >> 6;
@@ -166,19 +155,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         for (int c = 0; c < NC; ++c) tma_load_4d(dst + c * (64 * 64), map, full, c * 32, key, h, ent);
       };
       bool ok = true;
-      for (int j = 0; ok && j < nent + (STATS ? 0 : 1); ++j) {
+      for (int j = 0; ok && j < nent + 1; ++j) {
         if (*abort_flag) break;
         if (j < nent) {
           const int st = j % KS, use = j / KS;
           if (use > 0 && !mbar_wait(&k_empty[st], (use - 1) & 1, 131)) { ok = false; break; }
           load(smem + L::kKOff + st * L::kBlock, &k_full[st], j, false);
         }
-        if constexpr (!STATS) {
-          if (j >= 1) {
-            const int st = (j - 1) % VS, use = (j - 1) / VS;
-            if (use > 0 && !mbar_wait(&v_empty[st], (use - 1) & 1, 132)) { ok = false; break; }
-            load(smem + L::kVOff + st * L::kBlock, &v_full[st], j - 1, true);
-          }
+        if (j >= 1) {
+          const int st = (j - 1) % VS, use = (j - 1) / VS;
+          if (use > 0 && !mbar_wait(&v_empty[st], (use - 1) & 1, 132)) { ok = false; break; }
+          load(smem + L::kVOff + st * L::kBlock, &v_full[st], j - 1, true);
         }
       }
       if (!ok) *abort_flag = 1;
@@ -210,38 +197,31 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     };
     bool ok = __all_sync(0xffffffffu, nent == 0 || mbar_wait(q_full, 0, 130));
     if (ok && nent > 0) ok = issue_qk(0);
-    if (STATS && ok && nent > 1) ok = issue_qk(1);
     for (int j = 0; ok && j < nent; ++j) {
       if (*abort_flag) { ok = false; break; }
       // S buffer (j+1)&1 last held P(j-1), which PV(j-1) has read: products of
       // one thread run in issue order.
-      if (!STATS && j + 1 < nent && !issue_qk(j + 1)) { ok = false; break; }
-      if (STATS && j + 2 >= nent) continue;
+      if (j + 1 < nent && !issue_qk(j + 1)) { ok = false; break; }
       if (!__all_sync(0xffffffffu, mbar_wait(&p_full[j & 1], (j >> 1) & 1, 134))) {
         ok = false;
         break;
       }
-      if constexpr (STATS) {
-        tc_fence_after();
-        if (!issue_qk(j + 2)) { ok = false; break; }  // its S buffer has been read
-      } else {
-        const int st = j % VS;
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / VS) & 1, 135))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (elect_one_sync()) {
-          const uint64_t vd = vd0 + (uint64_t)((st * L::kBlock) >> 4);
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f16_ts(tmem_base + 128, tmem_base + (j & 1) * 64 + ks * 8,
-                        vd + (uint64_t)((ks * 1024) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&pv_done[j & 1]);
-          umma_commit(&v_empty[st]);
-        }
-        __syncwarp();
+      const int st = j % VS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / VS) & 1, 135))) {
+        ok = false;
+        break;
       }
+      tc_fence_after();
+      if (elect_one_sync()) {
+        const uint64_t vd = vd0 + (uint64_t)((st * L::kBlock) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma_f16_ts(tmem_base + 128, tmem_base + (j & 1) * 64 + ks * 8,
+                      vd + (uint64_t)((ks * 1024) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+        umma_commit(&pv_done[j & 1]);
+        umma_commit(&v_empty[st]);
+      }
+      __syncwarp();
     }
     if (!ok && lane == 0) *abort_flag = 1;
   } else {
@@ -283,7 +263,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     }
     const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
     int lim0 = len0, lim1 = len1;  // keys that the row sees
-    if (live && causal) lim1 = len1 - (p.Sq - 1 - (r0 + row) % p.Sq);
+    if (live && causal) lim1 = len1 - (p.Sq - 1 - p.div_sq.mod(r0 + row));
     // Blocks below `full` are whole for every row of the warp, blocks from
     // `none` on empty.  Rows past the tile's last (Q = 0) take what the others
     // see; a warp of such rows only sees nothing.
@@ -306,18 +286,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const uint32_t tmem_s = lane_base + (j & 1) * 64;
       const bool empty = key0 >= (own ? none1 : none0);
       const bool whole = key0 + 64 <= (own ? full1 : full0);
-      if constexpr (!STATS) {
-        // a cache's stale rows: 0 * V must not let them through
-        const int held = own ? len1 : len0;
-        if (key0 + 64 > held) {
-          if (!all(mbar_wait(&v_full[j % VS], (j / VS) & 1, 137))) { ok = false; break; }
-          uint8_t* vb = smem + L::kVOff + (j % VS) * L::kBlock;
-          for (int i = threadIdx.x; i < NC * 64 * 4; i += 128)
-            if (((i >> 2) & 63) >= held - key0)
-              *reinterpret_cast<uint4*>(vb + i * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+      // a cache's stale rows: 0 * V must not let them through
+      const int held = own ? len1 : len0;
+      if (key0 + 64 > held) {
+        if (!all(mbar_wait(&v_full[j % VS], (j / VS) & 1, 137))) { ok = false; break; }
+        uint8_t* vb = smem + L::kVOff + (j % VS) * L::kBlock;
+        for (int i = threadIdx.x; i < NC * 64 * 4; i += 128)
+          if (((i >> 2) & 63) >= held - key0)
+            *reinterpret_cast<uint4*>(vb + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
       }
       float s[64];
       uint32_t pk[32];
@@ -351,7 +329,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
           const float x1 = fast_exp2(__fmaf_rn(s[2 * c + 1], sc, nm));
           if (c & 1) t1 = add2(t1, make_float2(x0, x1));
           else t0 = add2(t0, make_float2(x0, x1));
-          if constexpr (!STATS) pk[c] = DType<DT>::pack2(x0, x1);
+          pk[c] = DType<DT>::pack2(x0, x1);
         }
         t0 = add2(t0, t1);
         return t0.x + t0.y;
@@ -366,30 +344,26 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const bool need = mn > m + kTileRescale;
       bool again = !spec;
       if (__any_sync(0xffffffffu, need)) {
-        if constexpr (!STATS) {
-          if (j > 0) {
-            if (!all(mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, 138))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+        if (j > 0) {
+          if (!all(mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, 138))) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
         }
         const float f = need ? (m == -INFINITY ? 0.f : fast_exp2(m - mn)) : 1.f;
         l *= f;
-        if constexpr (!STATS) {
-          if (j > 0) {
+        if (j > 0) {
 #pragma unroll
-            for (int c = 0; c < DK / 16; ++c) {
-              float o[16];
-              tmem_ld16(lane_base + 128 + c * 16, o);
-              tmem_wait_ld();
+          for (int c = 0; c < DK / 16; ++c) {
+            float o[16];
+            tmem_ld16(lane_base + 128 + c * 16, o);
+            tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] *= f;
-              tmem_st16(lane_base + 128 + c * 16, o);
-            }
-            tmem_wait_st();
+            for (int x = 0; x < 16; ++x) o[x] *= f;
+            tmem_st16(lane_base + 128 + c * 16, o);
           }
+          tmem_wait_st();
         }
         if (need) m = mn;
         again = true;
@@ -397,75 +371,70 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       if (again) {
         if (empty || m == -INFINITY) {  // nothing seen yet
           sum = 0.f;
-          if constexpr (!STATS)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) pk[c] = 0u;
+          for (int c = 0; c < 32; ++c) pk[c] = 0u;
         } else {
           sum = exp_block(-m);
         }
       }
       l += sum;
-      if constexpr (!STATS) {
-        tmem_st32u(tmem_s, pk);
-        tmem_wait_st();
-      }
+      tmem_st32u(tmem_s, pk);
+      tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[j & 1]);
     }
 
     // ---- epilogue ------------------------------------------------------------
-    if (!STATS && ok && nent > 0) {
+    if (ok && nent > 0) {
       ok = all(mbar_wait(&pv_done[(nent - 1) & 1], ((nent - 1) >> 1) & 1, 139));
       tc_fence_after();
     }
     if (!ok) *abort_flag = 1;
     const long long grow = ((long long)b * p.Hq + hd) * p.Sq + tk;
-    const bool direct = !STATS && p.NS == 1;
+    const bool direct = p.NS == 1;
     const bool seen = m != -INFINITY && ok;
     const long long at = grow * p.NS + gr.slot0 + sp;
-    if constexpr (!STATS) {
-      // Every product has run, so the ring is free: each thread lays its row
-      // there (padded, so that 16-byte stores of a warp do not collide) and
-      // sends it off with one bulk copy.
-      const float inv = seen && l > 0.f ? 1.f / l : 0.f;
-      uint8_t* orow = smem + L::kKOff + row * L::kOPitch;
-      if (nent > 0 || direct) {
+    // Every product has run, so the ring is free: each thread lays its row
+    // there (padded, so that 16-byte stores of a warp do not collide) and
+    // sends it off with one bulk copy.
+    const float inv = seen && l > 0.f ? 1.f / l : 0.f;
+    uint8_t* orow = smem + L::kKOff + row * L::kOPitch;
+    if (nent > 0 || direct) {
 #pragma unroll
-        for (int c = 0; c < DK / 32; ++c) {
-          float o[32];
-          __syncwarp();
-          if (nent > 0 && ok) {
-            tmem_ld32(lane_base + 128 + c * 32, o);
-            tmem_wait_ld();
-          }
-          if (direct) {
+      for (int c = 0; c < DK / 32; ++c) {
+        float o[32];
+        __syncwarp();
+        if (nent > 0 && ok) {
+          tmem_ld32(lane_base + 128 + c * 32, o);
+          tmem_wait_ld();
+        }
+        if (direct) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (seen) {
-                x.x = DType<DT>::pack2(o[u * 8] * inv, o[u * 8 + 1] * inv);
-                x.y = DType<DT>::pack2(o[u * 8 + 2] * inv, o[u * 8 + 3] * inv);
-                x.z = DType<DT>::pack2(o[u * 8 + 4] * inv, o[u * 8 + 5] * inv);
-                x.w = DType<DT>::pack2(o[u * 8 + 6] * inv, o[u * 8 + 7] * inv);
-              }
-              *reinterpret_cast<uint4*>(orow + c * 64 + u * 16) = x;
+          for (int u = 0; u < 4; ++u) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (seen) {
+              x.x = DType<DT>::pack2(o[u * 8] * inv, o[u * 8 + 1] * inv);
+              x.y = DType<DT>::pack2(o[u * 8 + 2] * inv, o[u * 8 + 3] * inv);
+              x.z = DType<DT>::pack2(o[u * 8 + 4] * inv, o[u * 8 + 5] * inv);
+              x.w = DType<DT>::pack2(o[u * 8 + 6] * inv, o[u * 8 + 7] * inv);
             }
-          } else {
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<float4*>(orow + c * 128 + u * 16) =
-                  make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
+            *reinterpret_cast<uint4*>(orow + c * 64 + u * 16) = x;
           }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<float4*>(orow + c * 128 + u * 16) =
+                make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
         }
-        fence_proxy_async_smem();
-        if (live && ok && (direct || seen)) {
-          if (direct)
-            bulk_store(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s, orow, p.D * 2);
-          else
-            bulk_store(p.opart + at * p.D, orow, p.D * 4);
-          bulk_commit();
-          bulk_wait0();
-        }
+      }
+      fence_proxy_async_smem();
+      if (live && ok && (direct || seen)) {
+        if (direct)
+          bulk_store(p.out + b * p.os_b + hd * p.os_h + tk * p.os_s, orow, p.D * 2);
+        else
+          bulk_store(p.opart + at * p.D, orow, p.D * 4);
+        bulk_commit();
+        bulk_wait0();
       }
     }
     if (live) {
@@ -482,10 +451,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   }
 }
 
-template <typename DT, int DK, bool STATS>
+template <typename DT, int DK>
 static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows& vp,
                           const mi_rows& k, const mi_rows& v, cudaStream_t st) {
-  using L = TileSmem<DK, STATS>;
+  using L = TileSmem<DK>;
   const CacheParams& p = tp.c;
   CUtensorMap m[4];
   memset(m, 0, sizeof(m));
@@ -493,13 +462,13 @@ static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows
   const bool use0 = (tp.grp[0].items && tp.grp[0].use0) || (tp.grp[1].items && tp.grp[1].use0);
   const bool use1 = (tp.grp[0].items && tp.grp[0].use1) || (tp.grp[1].items && tp.grp[1].use1);
   for (int i = 0; i < 4; ++i) {
-    if (!(i < 2 ? use0 : use1) || (STATS && (i & 1))) continue;
+    if (!(i < 2 ? use0 : use1)) continue;
     const CacheSeg& s = p.seg[i / 2];
     const int rc = make_rows4_map(&m[i], *t[i], s.nb, p.Hkv, s.cap, p.D, 32, 64);
     if (rc != MI_OK) return rc;
   }
-  constexpr auto kern = cache_tiles_kernel<DT, DK, STATS>;
-  cudaError_t err = allow_smem<cache_tiles_kernel<DT, DK, STATS>>(L::kAlloc);
+  constexpr auto kern = cache_tiles_kernel<DT, DK>;
+  cudaError_t err = allow_smem<cache_tiles_kernel<DT, DK>>(L::kAlloc);
   if (err == cudaSuccess) {
     kern<<<(unsigned)(tp.grp[0].items + tp.grp[1].items), kTileThreads, L::kAlloc, st>>>(
         m[0], m[1], m[2], m[3], tp);
@@ -513,19 +482,18 @@ static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows
   return MI_OK;
 }
 
-template <bool STATS>
 static int launch_tiles(const TileParams& tp, int dtype, const mi_rows& kp, const mi_rows& vp,
                         const mi_rows& k, const mi_rows& v, cudaStream_t st) {
   const bool bf = dtype == MI_BF16;
   const int D = tp.c.D;
   if (D <= 64)
-    return bf ? launch_tiles_t<__nv_bfloat16, 64, STATS>(tp, kp, vp, k, v, st)
-              : launch_tiles_t<__half, 64, STATS>(tp, kp, vp, k, v, st);
+    return bf ? launch_tiles_t<__nv_bfloat16, 64>(tp, kp, vp, k, v, st)
+              : launch_tiles_t<__half, 64>(tp, kp, vp, k, v, st);
   if (D <= 96)
-    return bf ? launch_tiles_t<__nv_bfloat16, 96, STATS>(tp, kp, vp, k, v, st)
-              : launch_tiles_t<__half, 96, STATS>(tp, kp, vp, k, v, st);
-  return bf ? launch_tiles_t<__nv_bfloat16, 128, STATS>(tp, kp, vp, k, v, st)
-            : launch_tiles_t<__half, 128, STATS>(tp, kp, vp, k, v, st);
+    return bf ? launch_tiles_t<__nv_bfloat16, 96>(tp, kp, vp, k, v, st)
+              : launch_tiles_t<__half, 96>(tp, kp, vp, k, v, st);
+  return bf ? launch_tiles_t<__nv_bfloat16, 128>(tp, kp, vp, k, v, st)
+            : launch_tiles_t<__half, 128>(tp, kp, vp, k, v, st);
 }
 
 }  // namespace mib200

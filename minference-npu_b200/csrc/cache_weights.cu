@@ -40,45 +40,334 @@ __global__ void weight_lse_kernel(const float2* ml, int NS, float* lse, long lon
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: S^T = K Q^T on tcgen05, a tile of 128 keys (the M rows, one per
-// thread) against blocks of 64 query rows.  A key's weight is then a sum along
-// its own TMEM lane: 64 exponentials and adds per block and thread, no exchange
-// between threads, nothing written back.  Bound by the exponentials (16 per
-// clock and SM).  What a cache holds past its length stays in its own lanes,
-// whose sums are dropped.
-//
-// RESQ: all rows of the key/value head (at most QS blocks, packed over its
-// query heads) stay in shared memory while key tiles stream; otherwise a key
-// tile stays while the blocks of each head's rows that see it stream.
+// Many rows (more than kRowsMost per key/value head): two tcgen05 passes over
+// Q K^T that keep nothing of it, row statistics and key sums.  Both are bound
+// by the exponentials, one per (row, key) and pass: 16 per clock and SM on the
+// MUFU unit.  Every fourth pair is computed on the FMA pipe instead
+// (poly_exp2), and eight epilogue warps (two per TMEM lane quadrant, each with
+// half of a step's columns) on each of two blocks per SM hide the latencies of
+// either.  Warp 8 issues TMA, warp 9 the products.
+// ---------------------------------------------------------------------------
+#ifndef MI_POLY_EVERY
+#define MI_POLY_EVERY 4
+#endif
+constexpr int kScanThreads = 320;
+
+// acc += sum over 32 columns of 2^(s * sc + z[c]); z per column in shared memory.
+__device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, const float* z,
+                                             float2& a0, float2& a1) {
+  const float2 sc2 = make_float2(sc, sc);
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const float4 zz = *reinterpret_cast<const float4*>(z + c);
+    const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(zz.x, zz.y));
+    const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(zz.z, zz.w));
+    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0 ? poly_exp2(x0)
+                                               : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
+    a1 = add2(a1, (c / 2 + 1) % MI_POLY_EVERY == 0
+                      ? poly_exp2(x1)
+                      : make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
+  }
+}
+// The same with one addend for all columns.
+__device__ __forceinline__ void exp_sum_row(const float (&s)[32], float sc, float z, float2& a0,
+                                            float2& a1) {
+  const float2 sc2 = make_float2(sc, sc), z2 = make_float2(z, z);
+#pragma unroll
+  for (int c = 0; c < 32; c += 4) {
+    const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, z2);
+    const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, z2);
+    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0 ? poly_exp2(x0)
+                                               : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
+    a1 = add2(a1, (c / 2 + 1) % MI_POLY_EVERY == 0
+                      ? poly_exp2(x1)
+                      : make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
+  }
+}
+
+// Gathers query rows [r0, r0 + 16) of a tile into 64-byte swizzled chunks of 32
+// dims (`chunk` bytes apart), by one warp.  Row r of the key/value head is token
+// r % Sq of its query head r / Sq; rows from `rows` on are zero.
+template <int DK>
+__device__ __forceinline__ void gather_rows16(const WeightParams& p, const FastDiv& div_sq, int b,
+                                              int h, int row0, int r0, int rows, uint32_t flip,
+                                              uint8_t* dst, int chunk) {
+  constexpr int U = DK / 8, kIter = U / 2;
+  const int lane = threadIdx.x & 31;
+  int tok;
+  const int g = div_sq.divmod(min(row0 + r0 + (lane & 15), rows - 1), tok);
+  const unsigned long long mine = reinterpret_cast<unsigned long long>(
+      p.q + b * p.qs_b + (long long)(h * p.group + g) * p.qs_h + (long long)tok * p.qs_s);
+  uint4 x[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int r = (i * 32 + lane) / U, u = (i * 32 + lane) % U;
+    const unsigned long long a = __shfl_sync(0xffffffffu, mine, r);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row0 + r0 + r < rows && u * 8 < p.D)
+      x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + u * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int r = r0 + (i * 32 + lane) / U, u = (i * 32 + lane) % U;
+    x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
+    *reinterpret_cast<uint4*>(dst + (u >> 2) * chunk + r * 64 + (((u & 3) ^ ((r >> 1) & 3)) << 4)) =
+        x[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Row statistics: an item is a tile of 128 query rows of a key/value head (the
+// M rows) against a range of 128-key blocks.  A row's exponentials are taken
+// against its maximum so far without looking for a larger one: only a sum that
+// passes 2^40 (or none so far) makes the warp look, so the maximum costs
+// nothing in between.  Leaves (maximum, sum), or the log-sum-exp where the item
+// has the whole row.
 // ---------------------------------------------------------------------------
 template <int DK>
+struct StatSmem {
+  static constexpr int NC = DK / 32;
+  static constexpr int KS = DK == 128 ? 2 : (DK == 96 ? 3 : 5);
+  static constexpr int kQTile = NC * 128 * 64, kKBlock = NC * 128 * 64;
+  static constexpr int kKOff = kQTile;
+  static constexpr int kJoinOff = kKOff + KS * kKBlock;
+  static constexpr int kBarOff = kJoinOff + 128 * 8;
+  // k_full[KS] k_empty[KS] s_full[2] s_empty[2] q_full
+  static constexpr int kSlotOff = kBarOff + (2 * KS + 5) * 8;
+  static constexpr int kAlloc = kSlotOff + 8 + 512;
+  static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
+};
+
+struct StatParams {
+  WeightParams w;
+  FastDiv rtiles, nsplit, div_hkv, div_sq;
+  int blocks;  // 128-key blocks per range
+  float2* ml;  // [rows][nsplit], or null
+  float* lse;  // [rows], log2 units, where nsplit is 1
+};
+
+template <typename DT, int DK>
+__global__ void __launch_bounds__(kScanThreads, 2)
+    row_stats_kernel(const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ StatParams sp) {
+  using L = StatSmem<DK>;
+  constexpr int NC = L::NC, KS = L::KS;
+  const WeightParams& p = sp.w;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~static_cast<uintptr_t>(511));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* s_full = k_empty + KS;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* q_full = s_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlotOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kSlotOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+  pdl_launch();
+
+  int rt, split, h;
+  // late row tiles first: a causal prompt's last rows see the most keys
+  const int b = sp.div_hkv.divmod(
+      sp.rtiles.divmod(sp.nsplit.divmod(blockIdx.x, split), rt), h);
+  const int r0 = ((int)sp.rtiles.d - 1 - rt) * 128;
+  const int rows = p.group * p.Sq;
+  const int nrows = min(128, rows - r0);
+  const int len = p.len ? min(max(p.len[b], 0), p.C) : p.C;
+  int end = len;  // keys that the tile's last token sees
+  if (p.causal) {
+    const int last = r0 + nrows - 1;
+    int smax;
+    if (sp.div_sq.divmod(last, smax) != sp.div_sq.div(r0)) smax = p.Sq - 1;
+    end = max(0, len - (p.Sq - 1 - smax));
+  }
+  const int nblk = (end + 127) >> 7;
+  const int j0 = (int)min((long long)split * sp.blocks, (long long)nblk);
+  const int nent = min(nblk - j0, sp.blocks);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 256);
+    mbar_init(q_full, 256);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int j = 0; j < nent; ++j) {
+        if (*abort_flag) break;
+        const int st = j % KS, use = j / KS;
+        if (use > 0 && !mbar_wait(&k_empty[st], (use - 1) & 1, 151)) {
+          *abort_flag = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&k_full[st], L::kKBlock);
+        for (int c = 0; c < NC; ++c)
+          tma_load_4d(smem + L::kKOff + st * L::kKBlock + c * (128 * 64), &tm_k, &k_full[st],
+                      c * 32, (j0 + j) * 128, h, b);
+      }
+    }
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = make_idesc_f16(DType<DT>::kBF16, 128, 128, false, false);
+    const uint64_t qd = make_desc_sw64(smem_u32(smem), 16, 512);
+    const uint64_t kd0 = make_desc_sw64(smem_u32(smem + L::kKOff), 16, 512);
+    bool ok = all(nent == 0 || mbar_wait(q_full, 0, 152));
+    for (int j = 0; ok && j < nent; ++j) {
+      const int st = j % KS;
+      if (*abort_flag) break;
+      ok = all(mbar_wait(&k_full[st], (j / KS) & 1, 153));
+      if (ok && j >= 2) ok = all(mbar_wait(&s_empty[j & 1], ((j >> 1) - 1) & 1, 154));
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one_sync()) {
+        const uint64_t kd = kd0 + (uint64_t)((st * L::kKBlock) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ++ks) {
+          const uint64_t off = ((ks >> 1) * (128 * 64) + (ks & 1) * 32) >> 4;
+          umma_f16_ss(tmem_base + (j & 1) * 128, qd + off, kd + off, idesc, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[j & 1]);
+        umma_commit(&k_empty[st]);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+  } else {
+    // thread = row (warp & 3) * 32 + lane, columns half * 64 ...
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const bool live = row < nrows;
+    int tok;
+    const int g = sp.div_sq.divmod(r0 + min(row, nrows - 1), tok);
+    if (nent > 0) {
+      gather_rows16<DK>(p, sp.div_sq, b, h, r0, warp * 16, rows,
+                        p.scale_log2 < 0.f ? 0x80008000u : 0u, smem, 128 * 64);
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const int lim = p.causal ? len - (p.Sq - 1 - tok) : len;  // keys that the row sees
+    const int wlo = __reduce_min_sync(0xffffffffu, live ? lim : 0x7fffffff);
+    const int whi = __reduce_max_sync(0xffffffffu, live ? lim : 0);
+    // not 0: a hidden score of -inf has to stay -inf when it is scaled
+    const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nent; ++j) {
+      if (!all(mbar_wait(&s_full[j & 1], (j >> 1) & 1, 155))) { ok = false; break; }
+      tc_fence_after();
+      const int key0 = (j0 + j) * 128 + half * 64;
+      if (key0 < whi) {
+        const bool whole = key0 + 64 <= wlo;
+        const uint64_t vis = bits_below((long long)lim - key0);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float s[32];
+          tmem_ld32(tcol + (j & 1) * 128 + q * 32, s);
+          tmem_wait_ld();
+          if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c] = ((vis >> (q * 32 + c)) & 1ull) ? s[c] : -INFINITY;
+          }
+          float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+          exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1);
+          a0 = add2(a0, a1);
+          float sum = a0.x + a0.y;
+          const bool bad = m == -INFINITY || !(sum < 1.1e12f);
+          if (__any_sync(0xffffffffu, bad)) {
+            float t = s[0];
+#pragma unroll
+            for (int c = 1; c < 31; c += 2) t = fmax3(t, s[c], s[c + 1]);
+            t = fmaxf(t, s[31]) * sc;
+            if (bad) {
+              const float mn = fmaxf(m, t);
+              if (m != -INFINITY) l *= fast_exp2(m - mn);
+              m = mn;
+            }
+            a0 = a1 = make_float2(0.f, 0.f);
+            exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1);
+            a0 = add2(a0, a1);
+            sum = m == -INFINITY ? 0.f : a0.x + a0.y;
+          }
+          l += sum;
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&s_empty[j & 1]);
+    }
+    if (!all(ok)) *abort_flag = 1;
+    float2* join = reinterpret_cast<float2*>(smem + L::kJoinOff);
+    if (half) join[row] = make_float2(m, l);
+    named_barrier(1, 256);
+    if (!half && live) {
+      const float2 o = join[row];
+      const float mn = fmaxf(m, o.x);
+      const float lt = mn == -INFINITY ? 0.f : l * fast_exp2(m - mn) + o.y * fast_exp2(o.x - mn);
+      const long long at = ((long long)b * p.Hq + h * p.group + g) * p.Sq + tok;
+      if (sp.lse) sp.lse[at] = mn == -INFINITY ? mn : mn + log2f(lt);
+      else sp.ml[at * sp.nsplit.d + split] = make_float2(mn, lt);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 256);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Key sums: S^T = K Q^T, a tile of 128 keys (the M rows, one per thread)
+// against blocks of NB query rows.  A key's weight is a sum along its own TMEM
+// lane, so nothing crosses threads (but the two halves of a step's columns, once
+// per tile) and nothing is written back.  What a cache holds past its length
+// stays in its own lanes, whose sums are dropped.
+//
+// RES: the rows of the key/value head are one block (NB = 64 or 128, packed
+// over its query heads), which stays in shared memory while key tiles stream;
+// otherwise a key tile stays while the blocks of each head's rows that see it
+// stream.
+// ---------------------------------------------------------------------------
+template <int DK, int NB, bool RES>
 struct ColsSmem {
   static constexpr int NC = DK / 32;
-  static constexpr int KS = 2, QS = DK == 128 ? 2 : (DK == 96 ? 4 : 6), SB = 4;
-  static constexpr int kKTile = NC * 128 * 64, kQBlock = NC * 64 * 64;
+  static constexpr int kKTile = NC * 128 * 64, kQBlock = NC * NB * 64;
+  static constexpr int QS = RES ? 1 : (DK == 64 ? 4 : 2);
+  static constexpr int KS = RES ? (104 * 1024 - kQBlock) / kKTile : (DK == 128 ? 1 : 2);
+  static constexpr int SB = 256 / NB;  // S buffers
   static constexpr int kQOff = KS * kKTile;
-  static constexpr int kRowOff = kQOff + QS * kQBlock;  // per warp: 64 x (-lse), 64 x token
-  static constexpr int kBarOff = kRowOff + 4 * 2 * 512;
+  static constexpr int kRowOff = kQOff + QS * kQBlock;  // per warp: 2 x (NB/2 x (-lse, token))
+  static constexpr int kJoinOff = kRowOff + 8 * 2 * NB * 4;
+  static constexpr int kBarOff = kJoinOff + 128 * 4;
   // k_full[KS] k_empty[KS] q_full[QS] q_empty[QS] s_full[SB] s_empty[SB]
   static constexpr int kSlotOff = kBarOff + (2 * KS + 2 * QS + 2 * SB) * 8;
   static constexpr int kAlloc = kSlotOff + 8 + 512;
-  static constexpr uint32_t kTmemCols = SB * 64;
   static_assert(kAlloc <= 113 * 1024, "two blocks per SM");
 };
 
 struct ColsParams {
   WeightParams w;
-  int tiles, per;    // key tiles of a (b, h); tiles per item
-  int ranges;        // items per (b, h)
+  int tiles, per;  // key tiles of a (b, h); tiles per item
+  FastDiv ranges;  // items per (b, h)
+  FastDiv div_hkv, div_sq;
 };
 
-template <typename DT, int DK, bool RESQ>
-__global__ void __launch_bounds__(192, 2)
+template <typename DT, int DK, int NB, bool RES>
+__global__ void __launch_bounds__(kScanThreads, 2)
     weight_tiles_kernel(const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ ColsParams cp) {
-  using L = ColsSmem<DK>;
-  constexpr int NC = L::NC, KS = L::KS, QS = L::QS, SB = L::SB;
+  using L = ColsSmem<DK, NB, RES>;
+  constexpr int NC = L::NC, KS = L::KS, QS = L::QS, SB = L::SB, NH = NB / 2;
   const WeightParams& p = cp.w;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -92,54 +381,38 @@ __global__ void __launch_bounds__(192, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlotOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kSlotOff + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
 
-  long long it = blockIdx.x;
-  const int range = (int)(it % cp.ranges);
-  it /= cp.ranges;
-  const int h = (int)(it % p.Hkv), b = (int)(it / p.Hkv);
+  int range, h;
+  const int b = cp.div_hkv.divmod(cp.ranges.divmod(blockIdx.x, range), h);
   const int len = p.len ? min(max(p.len[b], 0), p.C) : p.C;
   const int t0 = range * cp.per, t1 = min(cp.tiles, t0 + cp.per);
   const int tv = min(t1, (len + 127) >> 7);  // tiles from tv on hold no valid key
   const int rows = p.group * p.Sq;
-  const int nsb = RESQ ? (rows + 63) >> 6 : (p.Sq + 63) >> 6;
-  // First 64-row block of a head that sees key tile t.
+  const int nsb = RES ? 1 : (p.Sq + NB - 1) / NB;
+  const int heads = RES ? 1 : p.group;
+  // First block of a head's rows that sees key tile t.
   auto first_block = [&](int t) {
-    return !RESQ && p.causal ? max(0, t * 128 - len + p.Sq) >> 6 : 0;
+    return !RES && p.causal ? max(0, t * 128 - len + p.Sq) / NB : 0;
   };
-  const int heads = RESQ ? 1 : p.group;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < QS; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < SB; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 128);
+    for (int i = 0; i < QS; ++i) mbar_init(&q_full[i], RES ? 256 : 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < SB; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 256);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, L::kTmemCols);
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
-  if constexpr (RESQ) {
-    if (tv > t0) {
-      for (int i = threadIdx.x; i < nsb * 64 * (DK / 8); i += 192) {
-        const int r = i / (DK / 8), u = i - r * (DK / 8);
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && u * 8 < p.D)
-          x = *reinterpret_cast<const uint4*>(p.q + b * p.qs_b +
-                                              (long long)(h * p.group + r / p.Sq) * p.qs_h +
-                                              (long long)(r % p.Sq) * p.qs_s + u * 8);
-        *reinterpret_cast<uint4*>(smem + L::kQOff + (r >> 6) * L::kQBlock + (u >> 2) * (64 * 64) +
-                                  (r & 63) * 64 + (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x;
-      }
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
       bool ok = true;
       int nq = 0;
@@ -151,26 +424,25 @@ __global__ void __launch_bounds__(192, 2)
         for (int c = 0; c < NC; ++c)
           tma_load_4d(smem + st * L::kKTile + c * (128 * 64), &tm_k, &k_full[st], c * 32, t * 128,
                       h, b);
-        if constexpr (!RESQ) {
+        if constexpr (!RES) {
           for (int g = 0; ok && g < heads; ++g)
             for (int sb = first_block(t); sb < nsb; ++sb, ++nq) {
               const int qs = nq % QS, qu = nq / QS;
               if (qu > 0 && !mbar_wait(&q_empty[qs], (qu - 1) & 1, 142)) { ok = false; break; }
               mbar_arrive_expect_tx(&q_full[qs], L::kQBlock);
               for (int c = 0; c < NC; ++c)
-                tma_load_4d(smem + L::kQOff + qs * L::kQBlock + c * (64 * 64), &tm_q, &q_full[qs],
-                            c * 32, sb * 64, h * p.group + g, b);
+                tma_load_4d(smem + L::kQOff + qs * L::kQBlock + c * (NB * 64), &tm_q, &q_full[qs],
+                            c * 32, sb * NB, h * p.group + g, b);
             }
         }
       }
       if (!ok) *abort_flag = 1;
     }
-  } else if (warp == 5) {
-    constexpr uint32_t idesc = make_idesc_f16(DType<DT>::kBF16, 128, 64, false, false);
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = make_idesc_f16(DType<DT>::kBF16, 128, NB, false, false);
     const uint64_t kd0 = make_desc_sw64(smem_u32(smem), 16, 512);
     const uint64_t qd0 = make_desc_sw64(smem_u32(smem + L::kQOff), 16, 512);
-    auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-    bool ok = true;
+    bool ok = all(!RES || tv <= t0 || mbar_wait(&q_full[0], 0, 144));
     int n = 0;
     for (int t = t0; ok && t < tv; ++t) {
       const int st = (t - t0) % KS;
@@ -179,8 +451,8 @@ __global__ void __launch_bounds__(192, 2)
       const int f = first_block(t);
       for (int g = 0; ok && g < heads; ++g)
         for (int sb = f; sb < nsb; ++sb, ++n) {
-          const int qs = RESQ ? sb : n % QS, buf = n % SB;
-          if (!RESQ && !all(mbar_wait(&q_full[qs], (n / QS) & 1, 144))) { ok = false; break; }
+          const int qs = n % QS, buf = n % SB;
+          if (!RES && !all(mbar_wait(&q_full[qs], (n / QS) & 1, 144))) { ok = false; break; }
           if (n >= SB && !all(mbar_wait(&s_empty[buf], (n / SB - 1) & 1, 145))) {
             ok = false;
             break;
@@ -188,15 +460,15 @@ __global__ void __launch_bounds__(192, 2)
           tc_fence_after();
           if (elect_one_sync()) {
             const uint64_t kd = kd0 + (uint64_t)((st * L::kKTile) >> 4);
-            const uint64_t qd = qd0 + (uint64_t)((qs * L::kQBlock) >> 4);
+            const uint64_t qd = qd0 + (uint64_t)((RES ? 0 : qs * L::kQBlock) >> 4);
 #pragma unroll
             for (int ks = 0; ks < DK / 16; ++ks) {
               const uint32_t off = (ks & 1) * 32;
-              umma_f16_ss(tmem_base + buf * 64, kd + (((ks >> 1) * (128 * 64) + off) >> 4),
-                          qd + (((ks >> 1) * (64 * 64) + off) >> 4), idesc, ks > 0 ? 1u : 0u);
+              umma_f16_ss(tmem_base + buf * NB, kd + (((ks >> 1) * (128 * 64) + off) >> 4),
+                          qd + (((ks >> 1) * (NB * 64) + off) >> 4), idesc, ks > 0 ? 1u : 0u);
             }
             umma_commit(&s_full[buf]);
-            if constexpr (!RESQ) umma_commit(&q_empty[qs]);
+            if constexpr (!RES) umma_commit(&q_empty[qs]);
             if (g == heads - 1 && sb == nsb - 1) umma_commit(&k_empty[st]);
           }
           __syncwarp();
@@ -204,144 +476,237 @@ __global__ void __launch_bounds__(192, 2)
     }
     if (!ok && lane == 0) *abort_flag = 1;
   } else {
-    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
-    float* srow = reinterpret_cast<float*>(smem + L::kRowOff) + warp * 256;
+    // thread = key (warp & 3) * 32 + lane of the tile, columns half * NH ...
+    const int key = (warp & 3) * 32 + lane, half = warp >> 2;
+    if constexpr (RES) {
+      if (tv > t0) {
+        if (warp * 16 < NB)
+          gather_rows16<DK>(p, cp.div_sq, b, h, 0, warp * 16, rows, 0u, smem + L::kQOff, NB * 64);
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[0]);
+      }
+    }
+    pdl_wait();  // lse may come from the kernel before
+    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * NH;
+    float* srow = reinterpret_cast<float*>(smem + L::kRowOff) + warp * (2 * NB);
+    float* join = reinterpret_cast<float*>(smem + L::kJoinOff);
     const float* win = p.win ? p.win + b * p.wi_b + h * p.wi_h : nullptr;
     float* wout = p.wout + b * p.wo_b + h * p.wo_h;
+    const float* lse = p.lse + ((long long)b * p.Hq + h * p.group) * p.Sq;
+    // -lse (log2 units; -inf: adds nothing) and tokens of this warp's columns of
+    // a block of rows, to shared memory; fetched a block ahead
+    float zn[NH / 32];
+    auto fetch = [&](int g, int sb) {
+#pragma unroll
+      for (int x = 0; x < NH / 32; ++x) {
+        const int r = sb * NB + half * NH + x * 32 + lane;
+        zn[x] = r < (RES ? rows : p.Sq) ? lse[(long long)g * p.Sq + r] : -INFINITY;
+      }
+    };
+    auto lay = [&](int sb, float* nz) {
+#pragma unroll
+      for (int x = 0; x < NH / 32; ++x) {
+        const int r = sb * NB + half * NH + x * 32 + lane;
+        nz[x * 32 + lane] = zn[x] == -INFINITY ? zn[x] : -zn[x] * p.lse_mul;
+        reinterpret_cast<int*>(nz)[NH + x * 32 + lane] = RES ? cp.div_sq.mod(r) : r;
+      }
+    };
+    if (RES && tv > t0) {
+      fetch(0, 0);
+      lay(0, srow);
+      __syncwarp();
+    }
     bool ok = true;
-    auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
     int n = 0;
     for (int t = t0; t < t1; ++t) {
-      const int j = t * 128 + threadIdx.x;
+      const int j = t * 128 + key;
+      const float w0 = !half && win && j < min(len, p.C) ? win[j] : 0.f;
       float tot = 0.f;
-      // token from which a row sees the key; whole: every row of the block does
+      // token from which a row sees the key
       const int smin = p.causal ? j - len + p.Sq : 0;
       const int wmin = __shfl_sync(0xffffffffu, smin, 31);
       if (ok && t < tv) {
         const int f = first_block(t);
+        if (!RES) fetch(0, f);
         for (int g = 0; ok && g < heads; ++g)
           for (int sb = f; sb < nsb; ++sb, ++n) {
-            // this block's rows: -lse (log2 units; -inf: adds nothing) and tokens
-            float* nz = srow + (n & 1) * 128;
-            int* tok = reinterpret_cast<int*>(nz) + 64;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int r = sb * 64 + lane + 32 * x;
-              const int hd = RESQ ? r / p.Sq : g, s = RESQ ? r - hd * p.Sq : r;
-              float z = -INFINITY;
-              if (RESQ ? r < rows : s < p.Sq)
-                z = p.lse[((long long)b * p.Hq + h * p.group + hd) * p.Sq + s];
-              nz[lane + 32 * x] = z == -INFINITY ? z : -z * p.lse_mul;
-              tok[lane + 32 * x] = s;
+            float* nz = RES ? srow : srow + (n & 1) * NB;
+            if constexpr (!RES) {
+              lay(sb, nz);
+              __syncwarp();
+              if (sb + 1 < nsb) fetch(g, sb + 1);
+              else if (g + 1 < heads) fetch(g + 1, f);
             }
-            __syncwarp();
             const int buf = n % SB;
             if (!all(mbar_wait(&s_full[buf], (n / SB) & 1, 146))) { ok = false; break; }
             tc_fence_after();
-            float s[64];
-            tmem_ld32(lane_base + buf * 64, *reinterpret_cast<float(*)[32]>(&s[0]));
-            tmem_ld32(lane_base + buf * 64 + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
-            tmem_wait_ld();
-            tc_fence_before();
-            mbar_arrive(&s_empty[buf]);
-            const bool whole = RESQ ? wmin <= 0 : wmin <= sb * 64;
+            const bool whole = RES ? wmin <= 0 : wmin <= sb * NB + half * NH;
             float2 a0 = make_float2(0.f, 0.f), a1 = a0;
-            if (whole) {
 #pragma unroll
-              for (int c = 0; c < 64; c += 4) {
-                const float4 z = *reinterpret_cast<const float4*>(nz + c);
-                a0 = add2(a0, make_float2(fast_exp2(fmaf(s[c], p.scale_log2, z.x)),
-                                          fast_exp2(fmaf(s[c + 1], p.scale_log2, z.y))));
-                a1 = add2(a1, make_float2(fast_exp2(fmaf(s[c + 2], p.scale_log2, z.z)),
-                                          fast_exp2(fmaf(s[c + 3], p.scale_log2, z.w))));
+            for (int q = 0; q < NH / 32; ++q) {
+              float s[32];
+              tmem_ld32(tcol + buf * NB + q * 32, s);
+              tmem_wait_ld();
+              if (q == NH / 32 - 1) {
+                tc_fence_before();
+                mbar_arrive(&s_empty[buf]);
               }
-            } else {
+              if (whole) {
+                exp_sum_cols(s, p.scale_log2, nz + q * 32, a0, a1);
+              } else {
+                const int* tok = reinterpret_cast<const int*>(nz) + NH + q * 32;
 #pragma unroll
-              for (int c = 0; c < 64; ++c)
-                if (tok[c] >= smin) a0.x += fast_exp2(fmaf(s[c], p.scale_log2, nz[c]));
+                for (int c = 0; c < 32; ++c)
+                  if (tok[c] >= smin) a0.x += fast_exp2(fmaf(s[c], p.scale_log2, nz[q * 32 + c]));
+              }
             }
             a0 = add2(a0, a1);
             tot += a0.x + a0.y;  // two-level sum: a block, then the blocks
           }
       }
-      if (j < len) {
-        if (ok) wout[j] = (win ? win[j] : 0.f) + tot;
-      } else if (j < p.C && win != wout) {
-        wout[j] = win ? win[j] : 0.f;
+      // the two halves of the columns meet once per tile
+      if (half) join[key] = tot;
+      named_barrier(1, 256);
+      if (!half) {
+        tot += join[key];
+        if (j < len) {
+          if (ok) wout[j] = w0 + tot;
+        } else if (j < p.C && win != wout) {
+          wout[j] = win ? win[j] : 0.f;
+        }
       }
+      named_barrier(2, 256);
     }
-    if (!ok) *abort_flag = 1;
+    if (!all(ok)) *abort_flag = 1;
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, L::kTmemCols);
+    tmem_dealloc(tmem_base, 256);
   }
 }
 
+// Ranges per row tile of the statistics (two items per SM run at a time; see
+// tile_ranges), in 128-key blocks.
+static int stat_ranges(int64_t B, int64_t Hkv, int64_t rows, int64_t C) {
+  return tile_ranges(B * Hkv * ((rows + 127) / 128), (C + 127) / 128);
+}
+
 template <typename DT, int DK>
-static int launch_weight_tiles(const WeightParams& w, const mi_rows& q, const mi_rows& k,
-                               cudaStream_t st) {
-  using L = ColsSmem<DK>;
+static int launch_stats(const WeightParams& w, const mi_rows& k, float2* ml, float* lse,
+                        cudaStream_t st) {
+  using L = StatSmem<DK>;
+  StatParams sp{};
+  const int64_t rows = (int64_t)w.group * w.Sq, rtiles = (rows + 127) / 128;
+  const int64_t blocks = (w.C + 127) / 128;
+  const int ns = stat_ranges(w.B, w.Hkv, rows, w.C);
+  const long long items = (long long)w.B * w.Hkv * rtiles * ns;
+  if (items > 0x7fffffffll) return MI_ERR_SHAPE;
+  sp.w = w;
+  sp.rtiles = FastDiv(rtiles);
+  sp.nsplit = FastDiv(ns);
+  sp.div_hkv = FastDiv(w.Hkv);
+  sp.div_sq = FastDiv(w.Sq);
+  sp.blocks = (int)((blocks + ns - 1) / ns);
+  sp.ml = ml;
+  sp.lse = ns == 1 ? lse : nullptr;
+  CUtensorMap tk;
+  const int rc = make_rows4_map(&tk, k, w.B, w.Hkv, w.C, w.D, 32, 128);
+  if (rc != MI_OK) return rc;
+  cudaError_t err = allow_smem<row_stats_kernel<DT, DK>>(L::kAlloc);
+  if (err == cudaSuccess) {
+    row_stats_kernel<DT, DK><<<(unsigned)items, kScanThreads, L::kAlloc, st>>>(tk, sp);
+    err = cudaGetLastError();
+  }
+  if (err == cudaSuccess && ns > 1) {
+    const long long n = (long long)w.B * w.Hq * w.Sq;
+    weight_lse_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(ml, ns, lse, n);
+    err = cudaGetLastError();
+  }
+  return err == cudaSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+template <typename DT, int DK, int NB, bool RES>
+static int launch_cols_t(const WeightParams& w, const mi_rows& q, const mi_rows& k, bool after,
+                         cudaStream_t st) {
+  using L = ColsSmem<DK, NB, RES>;
   ColsParams cp{};
   cp.w = w;
   cp.tiles = (w.C + 127) / 128;
-  const long long rows = (long long)w.group * w.Sq;
-  const bool resq = rows <= 64 * L::QS;
   const long long all = (long long)w.B * w.Hkv * cp.tiles;
-  // tiles per item: with resident rows, three rounds of two items per SM;
+  // tiles per item: with resident rows, two rounds of two items per SM;
   // otherwise enough that an item has 16 blocks
-  const long long steps = (long long)w.group * ((w.Sq + 63) / 64);
-  long long per = resq ? (all + 148 * 6 - 1) / (148 * 6) : (16 + steps - 1) / steps;
+  const long long steps = (long long)w.group * ((w.Sq + NB - 1) / NB);
+  const long long per = RES ? (all + 148 * 4 - 1) / (148 * 4) : (16 + steps - 1) / steps;
   cp.per = (int)(per < 1 ? 1 : (per > cp.tiles ? cp.tiles : per));
-  cp.ranges = (cp.tiles + cp.per - 1) / cp.per;
-  const long long items = (long long)w.B * w.Hkv * cp.ranges;
+  const int ranges = (cp.tiles + cp.per - 1) / cp.per;
+  cp.ranges = FastDiv(ranges);
+  cp.div_hkv = FastDiv(w.Hkv);
+  cp.div_sq = FastDiv(w.Sq);
+  const long long items = (long long)w.B * w.Hkv * ranges;
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   CUtensorMap tk, tq;
   memset(&tq, 0, sizeof(tq));
   int rc = make_rows4_map(&tk, k, w.B, w.Hkv, w.C, w.D, 32, 128);
-  if (rc == MI_OK && !resq) rc = make_rows4_map(&tq, q, w.B, w.Hq, w.Sq, w.D, 32, 64);
+  if (rc == MI_OK && !RES) rc = make_rows4_map(&tq, q, w.B, w.Hq, w.Sq, w.D, 32, NB);
   if (rc != MI_OK) return rc;
-  auto kern = resq ? weight_tiles_kernel<DT, DK, true> : weight_tiles_kernel<DT, DK, false>;
-  cudaError_t err = resq ? allow_smem<weight_tiles_kernel<DT, DK, true>>(L::kAlloc)
-                         : allow_smem<weight_tiles_kernel<DT, DK, false>>(L::kAlloc);
+  constexpr auto kern = weight_tiles_kernel<DT, DK, NB, RES>;
+  cudaError_t err = allow_smem<weight_tiles_kernel<DT, DK, NB, RES>>(L::kAlloc);
   if (err == cudaSuccess) {
-    kern<<<(unsigned)items, 192, L::kAlloc, st>>>(tk, tq, cp);
-    err = cudaGetLastError();
+    // beside the end of the statistics of the same call, whose own launch has
+    // waited for whatever wrote the keys
+    if (after) {
+      err = launch_after(kern, dim3((unsigned)items), kScanThreads, L::kAlloc, st, tk, tq, cp);
+    } else {
+      kern<<<(unsigned)items, kScanThreads, L::kAlloc, st>>>(tk, tq, cp);
+      err = cudaGetLastError();
+    }
   }
   if (err != cudaSuccess) {
-    debug_launch_failure("weight_tiles_kernel", reinterpret_cast<const void*>(kern), err, 192,
-                         L::kAlloc);
+    debug_launch_failure("weight_tiles_kernel", reinterpret_cast<const void*>(kern), err,
+                         kScanThreads, L::kAlloc);
     return MI_ERR_LAUNCH;
   }
   return MI_OK;
 }
 
-static int launch_weights_many(const WeightParams& p, int dtype, const mi_rows& q,
-                               const mi_rows& k, cudaStream_t st) {
-  const bool bf = dtype == MI_BF16;
-  if (p.D <= 64)
-    return bf ? launch_weight_tiles<__nv_bfloat16, 64>(p, q, k, st)
-              : launch_weight_tiles<__half, 64>(p, q, k, st);
-  if (p.D <= 96)
-    return bf ? launch_weight_tiles<__nv_bfloat16, 96>(p, q, k, st)
-              : launch_weight_tiles<__half, 96>(p, q, k, st);
-  return bf ? launch_weight_tiles<__nv_bfloat16, 128>(p, q, k, st)
-            : launch_weight_tiles<__half, 128>(p, q, k, st);
+// One resident block where the key/value head's rows fit it, else streamed
+// blocks of 128 rows of a head (64 where a head has no more).
+template <typename DT, int DK>
+static int launch_weights_many(const WeightParams& w, const mi_rows& q, const mi_rows& k,
+                               float2* ml, float* lse, cudaStream_t st) {
+  WeightParams p = w;
+  if (!p.lse) {
+    const int rc = launch_stats<DT, DK>(p, k, ml, lse, st);
+    if (rc != MI_OK) return rc;
+    p.lse = lse;
+    p.lse_mul = 1.f;
+  }
+  const long long rows = (long long)p.group * p.Sq;
+  if (rows <= 64) return launch_cols_t<DT, DK, 64, true>(p, q, k, !w.lse, st);
+  if (rows <= 128) return launch_cols_t<DT, DK, 128, true>(p, q, k, !w.lse, st);
+  if (p.Sq <= 64) return launch_cols_t<DT, DK, 64, false>(p, q, k, !w.lse, st);
+  return launch_cols_t<DT, DK, 128, false>(p, q, k, !w.lse, st);
 }
 
 }  // namespace mib200
 
 using namespace mib200;
 
+// Partial statistics per row of the call's split.
+static int64_t weights_slots(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t C) {
+  const CachePlan pl = cache_plan(B, Hkv, group, Sq, 1, 0, C);
+  return pl.tile[1] ? stat_ranges(B, Hkv, group * Sq, C) : pl.NS;
+}
+
 extern "C" size_t mi_attn_weights_workspace_size(const mi_attn_weights_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, 1, 0, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0 || a->C == 0 || a->lse) return 0;
-  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, 1, 0, a->C);
+  const int64_t ns = weights_slots(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->C);
   const size_t rows = (size_t)(a->B * a->Hq * a->S_q);
-  if ((double)rows * pl.NS > 1e13) return SIZE_MAX;
-  return align_up(rows * pl.NS * 8) + align_up(rows * 4);
+  if ((double)rows * ns > 1e13) return SIZE_MAX;
+  return align_up(rows * ns * 8) + align_up(rows * 4);
 }
 
 extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace,
@@ -396,48 +761,49 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   w.causal = a.causal ? 1 : 0;
   w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
 
-  // the rows' split, for their statistics and for the few-row form of the weights
   const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C);
   const size_t rows = (size_t)(B * Hq * S_q);
+  float2* ml = static_cast<float2*>(workspace);
+  float* lse2 = nullptr;
+  if (!lse)
+    lse2 = reinterpret_cast<float*>(
+        static_cast<uint8_t*>(workspace) +
+        align_up(rows * weights_slots(B, Hkv, group, S_q, C) * 8));
+  if (pl.tile[1]) {
+#define MI_MANY(DK)                                                                      \
+  if (D <= DK)                                                                           \
+    return dtype == MI_BF16 ? launch_weights_many<__nv_bfloat16, DK>(w, q, k, ml, lse2, st) \
+                            : launch_weights_many<__half, DK>(w, q, k, ml, lse2, st);
+    MI_MANY(64)
+    MI_MANY(96)
+    MI_MANY(128)
+#undef MI_MANY
+  }
   CacheParams p{};
   p.q = w.q;
   p.qs_b = w.qs_b;
   p.qs_h = w.qs_h;
   p.qs_s = w.qs_s;
-  p.Hq = w.Hq;
-  p.Hkv = w.Hkv;
-  p.group = w.group;
-  p.Sq = w.Sq;
-  p.D = w.D;
+  set_heads(p, Hq, Hkv, S_q, D);
   p.scale_log2 = w.scale_log2;
   p.seg[0].seqs = 1;
   set_seg(p.seg[1], k, k, lengths, C, B, 1, group * S_q, w.causal);
-  p.seg[1].rtiles = pl.rtiles[1];
-  p.seg[1].nsplit = pl.nsplit[1];
+  p.seg[1].rtiles = FastDiv(pl.rtiles[1]);
+  p.seg[1].nsplit = FastDiv(pl.nsplit[1]);
   p.seg[1].chunk = pl.chunk[1];
   p.NS = pl.NS;
   const long long items = (long long)B * Hkv * pl.rtiles[1] * pl.nsplit[1];
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   if (!lse) {
-    p.ml = static_cast<float2*>(workspace);
-    float* lse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                           align_up(rows * pl.NS * 8));
-    if (pl.tile[1]) {
-      TileParams tp{};
-      tp.c = p;
-      tp.grp[1] = {1, 0, 1, pl.rtiles[1], pl.nsplit[1], pl.chunk[1] / 64, 0, items};
-      rc = launch_tiles<true>(tp, dtype, k, k, k, k, st);
-    } else {
-      rc = launch_rows_dk<kStats>(p, dtype, pl.nt, items, false, st);
-    }
+    p.ml = ml;
+    rc = launch_rows_dk<kStats>(p, dtype, pl.nt[1], items, false, st);
     if (rc != MI_OK) return rc;
-    weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(p.ml, pl.NS, lse2,
+    weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(ml, pl.NS, lse2,
                                                                       (long long)rows);
     if (cudaGetLastError() != cudaSuccess) return MI_ERR_LAUNCH;
     w.lse = lse2;
     w.lse_mul = 1.f;
   }
-  if (pl.tile[1]) return launch_weights_many(w, dtype, q, k, st);
   p.z = w.lse;
   p.z_mul = w.lse_mul;
   p.win = w.win;
@@ -446,5 +812,5 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   p.wout = w.wout;
   p.wo_b = w.wo_b;
   p.wo_h = w.wo_h;
-  return launch_rows_dk<kWeights>(p, dtype, pl.nt, items, false, st);
+  return launch_rows_dk<kWeights>(p, dtype, pl.nt[1], items, false, st);
 }
