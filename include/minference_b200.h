@@ -315,9 +315,7 @@ typedef struct mi_evict_args {
   const int32_t* lengths;
   int64_t B, H, C, D, keep, sink, recent;
 } mi_evict_args;
-size_t mi_evict_cache_workspace_size(const mi_evict_args* args);
-int mi_evict_cache(const mi_evict_args* args, void* workspace, size_t workspace_bytes,
-                   void* stream);
+int mi_evict_cache(const mi_evict_args* args, void* stream);
 
 #ifdef __cplusplus
 }

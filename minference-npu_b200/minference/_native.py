@@ -114,11 +114,12 @@ def lib() -> ctypes.CDLL:
         L.mi_vs_convert_indexes.argtypes = [P, P, I64, P, I64, I64, I64, I64, P, P, P, P, P]
         L.mi_vs_convert_indexes.restype = I
         # argument structs (the *_ARGS layouts below), packed as bytes
-        for name in ("mi_shared_prefix_fwd", "mi_attn_weights", "mi_evict_cache"):
+        for name in ("mi_shared_prefix_fwd", "mi_attn_weights"):
             size = getattr(L, name + "_workspace_size")
             size.argtypes, size.restype = [ctypes.c_char_p], SZ
             getattr(L, name).argtypes = [ctypes.c_char_p, P, SZ, P]
             getattr(L, name).restype = I
+        L.mi_evict_cache.argtypes, L.mi_evict_cache.restype = [ctypes.c_char_p, P], I
         _lib = L
     return _lib
 
@@ -169,13 +170,16 @@ def stream_ptr(device: torch.device) -> int:
 
 def call_packed(name: str, args: bytes, device: torch.device) -> None:
     """Workspace and launch of a cache entry point on the device's current stream."""
-    L = lib()
-    need = getattr(L, name + "_workspace_size")(args)
-    if need > 1 << 62:
-        raise ValueError(f"{name}: sizes not supported")
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return call_packed(name, args, device)
+    L = lib()
+    if name == "mi_evict_cache":  # needs no workspace
+        rc = L.mi_evict_cache(args, _raw_stream(device.index))
+        return check(rc, name) if rc else None
+    need = getattr(L, name + "_workspace_size")(args)
+    if need > 1 << 62:
+        raise ValueError(f"{name}: sizes not supported")
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         rc = getattr(L, name)(args, ws.data_ptr(), need, _raw_stream(device.index))

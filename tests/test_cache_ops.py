@@ -414,6 +414,9 @@ EVICT = [
     (1, 1, 20000, 8, 7000, 4, 64, BF, "bhsd"),
     (3, 1, 64, 128, 64, 0, 0, BF, "bhsd"),       # everything stays
     (2, 2, 50, 16, 80, 4, 4, BF, "bhsd"),        # a budget past the capacity
+    (2, 80, 2500, 64, 900, 4, 16, BF, "bhsd"),   # a block per head
+    (1, 90, 4096, 40, 1500, 4, 16, FP, "bshd"),  # two blocks per head
+    (40, 4, 9000, 8, 700, 2, 30, BF, "bhsd"),    # more keys than a block's registers hold
 ]
 
 
@@ -461,7 +464,7 @@ def test_evict_matches_definition(cuda, case, kind):
 
 
 @pytest.mark.gpu
-def test_evict_long_cache_selects_past_shared_memory(cuda):
+def test_evict_long_cache_selects_past_registers(cuda):
     from minference import ops
 
     C = 400001
@@ -809,22 +812,18 @@ def test_c_entry_points_refuse():
     assert weights(lse=1 << 20, size=True) == 0 and weights(size=True) > 0
 
     def evict(k=ok, v=ok, w=1 << 20, ko=ok, vo=ok, wo=1 << 20, idx=1 << 20, nl=1 << 20, B=2, H=2,
-              C=8, D=64, keep=4, sink=0, recent=0, ws=None, n=0, size=False):
+              C=8, D=64, keep=4, sink=0, recent=0):
         args = _native.EVICT_ARGS.pack(*k, *v, w, 16, 8, *ko, *vo, wo, 8, 4, idx, nl, 0, B, H, C,
                                        D, keep, sink, recent)
-        if size:
-            return L.mi_evict_cache_workspace_size(args)
-        return L.mi_evict_cache(args, ws, n, None)
+        return L.mi_evict_cache(args, None)
 
-    assert L.mi_evict_cache(None, None, 0, None) == 1
+    assert L.mi_evict_cache(None, None) == 1
     for bad in (dict(keep=0), dict(sink=3, recent=2), dict(sink=-1), dict(recent=-1), dict(D=0),
                 dict(D=2000), dict(C=-1), dict(idx=0), dict(nl=0), dict(wo=0), dict(w=0),
-                dict(k=null), dict(vo=null), dict(sink=2**62, recent=2**62)):
+                dict(k=null), dict(vo=null), dict(sink=2**62, recent=2**62),
+                dict(B=1 << 20, H=1 << 20)):
         assert evict(**bad) == 1, bad
-    assert evict(C=400000) == 3  # keys past shared memory need a workspace
     assert evict(B=0) == 0 and evict(H=0) == 0
-    assert evict(C=65536, size=True) == 0 and evict(C=400000, size=True) >= 4 * 400000 * 4
-    assert evict(keep=0, size=True) == none
 
 
 def test_argument_structs_match_the_header():
