@@ -529,24 +529,29 @@ static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2], in
 // tcgen05 tile.
 constexpr int64_t kRowsMost = 32;
 
-// cache_tiles_kernel: ranges per tile.  Two items run on each of the 148 SMs;
-// an item costs its blocks plus kItemCost (set-up, first loads, epilogue), and
-// a partial result to be joined kJoinCost more, in units of a 64-key block.
-static int tile_ranges(int64_t tiles, int64_t blocks) {
-  constexpr double kItemCost = 6, kJoinCost = 4;
+// cache_tiles_kernel: key blocks per range, for tiles of up to two kinds.  Two
+// items run on each of the 148 SMs; an item costs its blocks plus kItemCost
+// (set-up, first loads, epilogue), and a partial result to be joined kJoinCost
+// more, in units of a 64-key block (1 us).
+static int64_t tile_blocks(const int64_t (&tiles)[2], const int64_t (&blocks)[2]) {
+  constexpr double kItemCost = 5, kJoinCost = 4;
   const int64_t slots = 2 * 148;
-  int best = 1;
+  const int64_t most = blocks[0] > blocks[1] ? blocks[0] : blocks[1];
+  const double total = (double)tiles[0] * blocks[0] + (double)tiles[1] * blocks[1];
+  int64_t best = most;
   double best_cost = 1e300;
   for (int64_t rounds = 0; rounds <= 6; ++rounds) {
-    int64_t ns = rounds * slots / tiles;  // as many ranges as fit these rounds
-    if (ns < 1) ns = 1;
-    if (ns > blocks) ns = blocks;
-    const int64_t per = (blocks + ns - 1) / ns;
-    const int64_t waves = (tiles * ns + slots - 1) / slots;
-    const double cost = (double)waves * (per + kItemCost + (ns > 1 ? kJoinCost : 0));
-    if (cost < best_cost) best_cost = cost, best = (int)ns;
+    int64_t per = most, items = 0;
+    if (rounds) per = (int64_t)(total / (rounds * slots)) + 1;
+    for (;; ++per) {  // the shortest ranges that fit these rounds
+      items = tiles[0] * ((blocks[0] + per - 1) / per) + tiles[1] * ((blocks[1] + per - 1) / per);
+      if (!rounds || items <= rounds * slots || per >= most) break;
+    }
+    const int64_t waves = (items + slots - 1) / slots;
+    const double cost = (double)waves * (per + kItemCost + (per < most ? kJoinCost : 0));
+    if (cost < best_cost) best_cost = cost, best = per < most ? per : most;
   }
-  return best;
+  return best < 1 ? 1 : best;
 }
 
 static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
@@ -565,8 +570,7 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
     pl.tile[0] = false;
     pl.rtiles[1] = (int)((rows[1] + 127) / 128);
     const int64_t blocks = (P + 63) / 64 + (C + 63) / 64;
-    const int ns = tile_ranges(B * Hkv * pl.rtiles[1], blocks);
-    pl.chunk[1] = (int)((blocks + ns - 1) / ns) * 64;
+    pl.chunk[1] = (int)tile_blocks({0, B * Hkv * pl.rtiles[1]}, {0, blocks}) * 64;
     pl.nsplit[1] = (int)((blocks * 64 + pl.chunk[1] - 1) / pl.chunk[1]);
     pl.NS = pl.nsplit[1];
     return pl;
@@ -579,17 +583,16 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
     pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
     if (!pl.tile[s]) tiles[s] = nb[s] * Hkv * pl.rtiles[s];
   }
+  int64_t many[2] = {0, 0}, blocks[2] = {0, 0};  // by cache_tiles_kernel
+  for (int s = 0; s < 2; ++s)
+    if (pl.tile[s]) many[s] = nb[s] * Hkv * pl.rtiles[s], blocks[s] = (cap[s] + 63) / 64;
   const int64_t caps[2] = {tiles[0] ? cap[0] : 0, tiles[1] ? cap[1] : 0};
   const int nt = tiles[0] && pl.nt[0] > pl.nt[1] ? pl.nt[0] : pl.nt[1];
-  const int64_t chunk = rows_chunk(tiles, caps, nt);
+  const int64_t chunk = tiles[0] || tiles[1] ? rows_chunk(tiles, caps, nt) : 0;
+  const int64_t tile_chunk = many[0] || many[1] ? tile_blocks(many, blocks) * 64 : 0;
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
-    int64_t ch = chunk;
-    if (pl.tile[s]) {
-      const int64_t blocks = (cap[s] + 63) / 64;
-      const int ns = tile_ranges(nb[s] * Hkv * pl.rtiles[s], blocks);
-      ch = (blocks + ns - 1) / ns * 64;
-    }
+    const int64_t ch = pl.tile[s] ? tile_chunk : chunk;
     pl.chunk[s] = (int)ch;
     // at least one range: with no key at all it writes the zeros
     pl.nsplit[s] = cap[s] ? (int)((cap[s] + ch - 1) / ch) : 1;

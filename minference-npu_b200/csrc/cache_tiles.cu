@@ -69,7 +69,7 @@ __device__ __forceinline__ void bulk_wait0() {
 }
 
 constexpr int kTileThreads = 192;
-constexpr float kTileRescale = 12.0f;  // log2 growth of a row's maximum that rescales O
+constexpr float kTileSum = 32768.0f;  // sum of a block's P from which its row's reference moves
 
 template <typename DT, int DK>
 __global__ void __launch_bounds__(kTileThreads, 2)
@@ -123,6 +123,28 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   const int n0 = (len0 + 63) >> 6, n1 = (end1 + 63) >> 6;
   const int j0 = min(n0 + n1, (int)min((long long)sp * gr.blocks, (long long)(n0 + n1)));
   const int nent = min(n0 + n1 - j0, gr.blocks);
+
+  // ---- Q: each softmax warp asks for its 32 rows (a lane per 16 bytes, addresses
+  // passed around by shuffle) before the first keys are asked for, whose burst
+  // it would otherwise wait behind (5 us) ------------------------------------------
+  constexpr int U = DK / 8;
+  const int row = threadIdx.x;
+  const bool live = row < nrows;
+  int b = 0, hd = 0, tk = 0;
+  uint4 qx[U];
+  if (live) cache_row(p, rs, e, h, r0 + row, b, hd, tk);
+  if (warp < 4 && nent > 0) {
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(
+        p.q + (live ? b * p.qs_b + hd * p.qs_h + tk * p.qs_s : 0));
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int idx = i * 32 + lane, r = idx / U, u = idx % U;
+      const unsigned long long a = __shfl_sync(0xffffffffu, mine, r);
+      qx[i] = make_uint4(0, 0, 0, 0);
+      if (warp * 32 + r < nrows && u * 8 < p.D)
+        qx[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + u * 8);
+    }
+  }
 
   // ---- set-up: barriers, TMEM --------------------------------------------------
   if (threadIdx.x == 0) {
@@ -226,37 +248,18 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     if (!ok && lane == 0) *abort_flag = 1;
   } else {
     // ---- softmax: thread = row ---------------------------------------------------
-    const int row = threadIdx.x;
-    const bool live = row < nrows;
-    int b = 0, hd = 0, tk = 0;
-    if (live) cache_row(p, rs, e, h, r0 + row, b, hd, tk);
-    // Q: each warp gathers its 32 rows (a lane per 16 bytes, addresses passed
-    // around by shuffle), into chunks of 32 dims with the 64-byte swizzle.  A
-    // negative scale is taken into Q (its sign bits), so that the largest score
-    // is the largest product.
+    // Q into chunks of 32 dims with the 64-byte swizzle.  A negative scale is
+    // taken into Q (its sign bits), so that the largest score is the largest
+    // product.
     if (nent > 0) {
-      constexpr int U = DK / 8, kBatch = U / 2;
       const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-      const unsigned long long mine = reinterpret_cast<unsigned long long>(
-          p.q + (live ? b * p.qs_b + hd * p.qs_h + tk * p.qs_s : 0));
 #pragma unroll
-      for (int i0 = 0; i0 < U; i0 += kBatch) {
-        uint4 x[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int idx = (i0 + i) * 32 + lane, r = idx / U, u = idx % U;
-          const unsigned long long a = __shfl_sync(0xffffffffu, mine, r);
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (warp * 32 + r < nrows && u * 8 < p.D)
-            x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + u * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int idx = (i0 + i) * 32 + lane, r = warp * 32 + idx / U, u = idx % U;
-          x[i].x ^= flip, x[i].y ^= flip, x[i].z ^= flip, x[i].w ^= flip;
-          *reinterpret_cast<uint4*>(smem + (u >> 2) * (128 * 64) + r * 64 +
-                                    (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x[i];
-        }
+      for (int i = 0; i < U; ++i) {
+        const int idx = i * 32 + lane, r = warp * 32 + idx / U, u = idx % U;
+        uint4 x = qx[i];
+        x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+        *reinterpret_cast<uint4*>(smem + (u >> 2) * (128 * 64) + r * 64 +
+                                  (((u & 3) ^ ((r >> 1) & 3)) << 4)) = x;
       }
       fence_proxy_async_smem();
       mbar_arrive(q_full);
@@ -334,14 +337,18 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         t0 = add2(t0, t1);
         return t0.x + t0.y;
       };
-      // P against the running maximum straight away; only if some row's maximum
-      // grew by more than 2^12 (or none is known yet) is it computed again.
+      // P against the row's reference straight away, without looking for its
+      // maximum: a sum below 2^15 says that every P is (fp16 holds it).  Only
+      // if some row passes that (or has seen nothing yet) does the warp look,
+      // move the references, rescale O and compute P again.
       const bool spec = !empty && all(m != -INFINITY);
-      float sum = 0.f, tmax = -INFINITY;
+      float sum = 0.f, mn = m;
       if (spec) sum = exp_block(-m);
-      if (!empty) tmax = row_max() * sc;
-      const float mn = fmaxf(m, tmax);
-      const bool need = mn > m + kTileRescale;
+      bool need = !empty && !(m != -INFINITY && sum < kTileSum);
+      if (!empty && __any_sync(0xffffffffu, need)) {
+        mn = fmaxf(m, row_max() * sc);
+        need = need && mn > m;
+      }
       bool again = !spec;
       if (__any_sync(0xffffffffu, need)) {
         if (j > 0) {

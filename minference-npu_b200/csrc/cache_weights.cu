@@ -588,9 +588,11 @@ __global__ void __launch_bounds__(kScanThreads, 2)
 }
 
 // Ranges per row tile of the statistics (two items per SM run at a time; see
-// tile_ranges), in 128-key blocks.
+// tile_blocks), in 128-key blocks.
 static int stat_ranges(int64_t B, int64_t Hkv, int64_t rows, int64_t C) {
-  return tile_ranges(B * Hkv * ((rows + 127) / 128), (C + 127) / 128);
+  const int64_t blocks = (C + 127) / 128;
+  const int64_t per = tile_blocks({0, B * Hkv * ((rows + 127) / 128)}, {0, blocks});
+  return (int)((blocks + per - 1) / per);
 }
 
 template <typename DT, int DK>
