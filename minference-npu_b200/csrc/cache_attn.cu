@@ -9,8 +9,8 @@
 namespace mib200 {
 
 // ---------------------------------------------------------------------------
-// Few rows (1 to 32 per key/value head): a work item is one tile of 8*NT rows
-// against `chunk` keys.  Its warps take groups of 16 keys in turn; each
+// Few rows (1 to 8 per key/value head): a work item is those rows against
+// `chunk` keys.  Its warps take groups of 16 keys in turn; each
 // warp streams its own groups through its own shared-memory ring (cp.async)
 // and keeps its own running maximum, sum and O, so there is no barrier in the
 // loop.  Their states are joined at the end.  Keys are the M side of both
@@ -24,38 +24,36 @@ namespace mib200 {
 // holds past its length cannot reach O through 0 * V.
 //
 // kStats: the rows' (maximum, sum) only; no V.
-// kWeights: given the rows' lse, a key's weight summed over the tile's rows
-// (all rows of the key/value head, at most 32) and added to win; no V.
+// kWeights: given the rows' lse, a key's weight summed over the rows and added to win; no V.
 // ---------------------------------------------------------------------------
 enum RowsMode { kAttention, kStats, kWeights };
 
-template <int DK, int NT, RowsMode MODE>
+template <int DK, RowsMode MODE>
 struct RowsSmem {
-  // Four blocks per SM either way: with one 8-row tile a warp waits on its own
-  // instruction latencies more than on memory, so four warps share the bytes in
-  // flight; taller tiles have the work, and the registers, of two.
-  static constexpr int W = NT == 1 ? 4 : 2;
+  // A warp waits on its own instruction latencies more than on memory, so four
+  // warps share a block's bytes in flight.
+  static constexpr int W = 4;
   static constexpr int kPitch = DK * 2 + 16;
   static constexpr int kTile = 16 * kPitch;  // 16 keys of K or V
   // one warp's stage; kWeights: and 16 of win
   static constexpr int kStage = MODE == kAttention ? 2 * kTile
                                                    : kTile + (MODE == kWeights ? 64 : 0);
-  // about 52 KB a block (70 KB and three blocks per SM for D = 128, NT = 1)
+  // four blocks per SM (three for the attention's 70 KB at D = 128)
   static constexpr int kFit =
-      (MODE == kAttention && DK == 128 && W == 4 ? 70 * 1024 : 55 * 1024) / (W * kStage);
+      (MODE == kAttention && DK == 128 ? 70 * 1024 : 55 * 1024) / (W * kStage);
   static constexpr int ST = kFit > 8 ? 8 : kFit;
   static_assert(ST >= 2, "a stage to load beside the one in use");
   static constexpr int kWarpRing = ST * kStage;
   static constexpr int kRing = W * kWarpRing;
 };
 
-template <typename DT, int DK, int NT, RowsMode MODE>
-__global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
-                                  MODE == kAttention && DK == 128 && NT == 1 ? 3 : 4)
+template <typename DT, int DK, RowsMode MODE>
+__global__ void __launch_bounds__(32 * RowsSmem<DK, MODE>::W,
+                                  MODE == kAttention && DK == 128 ? 3 : 4)
     cache_rows_kernel(const __grid_constant__ CacheParams p) {
-  using L = RowsSmem<DK, NT, MODE>;
+  using L = RowsSmem<DK, MODE>;
   constexpr int kRowsWarps = L::W;
-  constexpr int KS = DK / 16, R = 8 * NT, CPR = DK / 8;
+  constexpr int KS = DK / 16, R = 8, CPR = DK / 8;
   constexpr bool kO = MODE == kAttention;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float sm_m[kRowsWarps][R], sm_l[kRowsWarps][R];
@@ -125,20 +123,17 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
     cp_commit();
   };
 
-  // ---- Q tile: every warp fetches it for itself, ahead of its first keys (whose
-  // loads would otherwise queue before it), through the ring stage that is
-  // loaded last, 16 rows at a time, into fragments ------------------------------
-  uint32_t qf[NT][KS][2];
+  // ---- Q: every warp fetches the rows for itself, ahead of its first keys (whose
+  // loads would otherwise queue before them), through the ring stage that is
+  // loaded last, into fragments ---------------------------------------------------
   uint8_t* qs = smem + warp * L::kWarpRing + (L::ST - 1) * L::kStage;
-  static_assert(16 * L::kPitch <= L::kStage, "16 rows of Q fit a stage");
-  constexpr int kQRows = NT == 1 ? 8 : 16, kQIter = kQRows * CPR / 32;
+  constexpr int kQIter = R * CPR / 32;
   uint4 qx[kQIter];
-  auto fetch_q = [&](int half) {
-    const int hr = half * 16 + (lane & 15);  // row whose address this lane works out
-    const uint16_t* qp = p.q;
-    if (hr < nrows) {
+  {
+    const uint16_t* qp = p.q;  // lanes 0-7 work the rows' addresses out
+    if (lane < nrows) {
       int b, hd, tk;
-      cache_row(p, sg, e, h, r0 + hr, b, hd, tk);
+      cache_row(p, sg, e, h, r0 + lane, b, hd, tk);
       qp += b * p.qs_b + hd * p.qs_h + tk * p.qs_s;
     }
 #pragma unroll
@@ -147,102 +142,81 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
       const unsigned long long a =
           __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(qp), r);
       qx[i] = make_uint4(0, 0, 0, 0);
-      if (half * 16 + r < nrows && c * 8 < p.D)
+      if (r < nrows && c * 8 < p.D)
         qx[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a) + c * 8);
     }
-  };
-  fetch_q(0);
+  }
 #pragma unroll
   for (int s = 0; s < L::ST - 1; ++s) load(warp + s * kRowsWarps);
 #pragma unroll
-  for (int half = 0; half < (NT + 1) / 2; ++half) {
-    if (half) fetch_q(half);
-#pragma unroll
-    for (int i = 0; i < kQIter; ++i) {
-      const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
-      *reinterpret_cast<uint4*>(qs + r * L::kPitch + c * 16) = qx[i];
-    }
-    __syncwarp();
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (half * 2 + n >= NT) break;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks += 2) {
-        uint32_t b[4];
-        ldsm4(b, smem_u32(qs) + (n * 8 + (lane & 7)) * L::kPitch + ks * 32 + (lane >> 3) * 16);
-        qf[half * 2 + n][ks][0] = b[0];
-        qf[half * 2 + n][ks][1] = b[1];
-        qf[half * 2 + n][ks + 1][0] = b[2];
-        qf[half * 2 + n][ks + 1][1] = b[3];
-      }
-    }
-    __syncwarp();
+  for (int i = 0; i < kQIter; ++i) {
+    const int r = (i * 32 + lane) / CPR, c = (i * 32 + lane) % CPR;
+    *reinterpret_cast<uint4*>(qs + r * L::kPitch + c * 16) = qx[i];
   }
-  int lim[NT][2];  // keys that row 8n + (lane&3)*2 + x sees
+  __syncwarp();
+  uint32_t qf[KS][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks += 2) {
+    uint32_t b[4];
+    ldsm4(b, smem_u32(qs) + (lane & 7) * L::kPitch + ks * 32 + (lane >> 3) * 16);
+    qf[ks][0] = b[0], qf[ks][1] = b[1], qf[ks + 1][0] = b[2], qf[ks + 1][1] = b[3];
+  }
+  __syncwarp();
+  int lim[2];  // keys that row (lane & 3) * 2 + x sees
   int minlim = 0x7fffffff;
-  float nz[NT][2];  // kWeights: -lse (log2 units; -inf: the row adds nothing)
+  float nz[2];  // kWeights: -lse (log2 units; -inf: the row adds nothing)
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = n * 8 + (lane & 3) * 2 + x;
-      lim[n][x] = 0;
-      nz[n][x] = -INFINITY;
-      if (r < nrows) {
-        int tok;
-        const int g = p.div_sq.divmod(r0 + r, tok);
-        lim[n][x] = sg.causal ? len - (p.Sq - 1 - tok) : len;
-        minlim = min(minlim, lim[n][x]);
-        if constexpr (MODE == kWeights) {
-          const float z =
-              p.z[((long long)e * p.Hq + h * p.group + g) * p.Sq + tok];
-          if (z != -INFINITY) nz[n][x] = -z * p.z_mul;
-        }
+  for (int x = 0; x < 2; ++x) {
+    const int r = (lane & 3) * 2 + x;
+    lim[x] = 0;
+    nz[x] = -INFINITY;
+    if (r < nrows) {
+      int tok;
+      const int g = p.div_sq.divmod(r0 + r, tok);
+      lim[x] = sg.causal ? len - (p.Sq - 1 - tok) : len;
+      minlim = min(minlim, lim[x]);
+      if constexpr (MODE == kWeights) {
+        const float z = p.z[((long long)e * p.Hq + h * p.group + g) * p.Sq + tok];
+        if (z != -INFINITY) nz[x] = -z * p.z_mul;
       }
     }
+  }
   minlim = __reduce_min_sync(0xffffffffu, minlim);
 
-  float m[NT][2], l[NT][2];
-  float o[kO ? DK / 16 : 1][NT][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[kO ? DK / 16 : 1][4];
+  if constexpr (kO)
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-    if constexpr (kO)
-#pragma unroll
-      for (int d = 0; d < DK / 16; ++d) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.f;
-  }
+    for (int d = 0; d < DK / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
 
   for (int g = warp; g < ngroups; g += kRowsWarps) {
     load(g + (L::ST - 1) * kRowsWarps);
     cp_wait<L::ST - 1>();
     __syncwarp();
     const uint32_t st = ring + ((g / kRowsWarps) % L::ST) * L::kStage;
-    float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    // two accumulators: the products of one wait for each other
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
     const uint32_t ka = st + (lane & 15) * L::kPitch + (lane >> 4) * 16;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       uint32_t a[4];
       ldsm4(a, ka + ks * 32);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma16816<DT>(s[n], a, qf[n][ks][0], qf[n][ks][1]);
+      mma16816<DT>((ks & 1) ? s2 : s, a, qf[ks][0], qf[ks][1]);
     }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] += s2[c];
     const int key0 = kb + g * 16;
     const bool full = key0 + 16 <= min(minlim, ke);
     if constexpr (MODE == kWeights) {
       float t0 = 0.f, t1 = 0.f;  // keys lane/4 and lane/4 + 8
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int key = key0 + (lane >> 2), lm = min(lim[n][x], ke);
-          const float p0 = fast_exp2(fmaf(s[n][x], p.scale_log2, nz[n][x]));
-          const float p1 = fast_exp2(fmaf(s[n][2 + x], p.scale_log2, nz[n][x]));
-          t0 += full || key < lm ? p0 : 0.f;
-          t1 += full || key + 8 < lm ? p1 : 0.f;
-        }
+      for (int x = 0; x < 2; ++x) {
+        const int key = key0 + (lane >> 2), lm = min(lim[x], ke);
+        const float p0 = fast_exp2(fmaf(s[x], p.scale_log2, nz[x]));
+        const float p1 = fast_exp2(fmaf(s[2 + x], p.scale_log2, nz[x]));
+        t0 += full || key < lm ? p0 : 0.f;
+        t1 += full || key + 8 < lm ? p1 : 0.f;
+      }
       t0 += __shfl_xor_sync(0xffffffffu, t0, 1);
       t1 += __shfl_xor_sync(0xffffffffu, t1, 1);
       t0 += __shfl_xor_sync(0xffffffffu, t0, 2);
@@ -256,47 +230,38 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
         if (key0 + i < ke) wout[key0 + i] = w;
       }
     } else {
-      uint32_t pb[NT][2];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] *= p.scale_log2;
+      if (!full) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (key0 + (lane >> 2) + 8 * (c >> 1) >= min(lim[c & 1], ke)) s[c] = -INFINITY;
+      }
+      float pr[4], f[2];
       bool grew = false;
-      float f[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[n][c] *= p.scale_log2;
-        if (!full) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (key0 + (lane >> 2) + 8 * (c >> 1) >= min(lim[n][c & 1], ke)) s[n][c] = -INFINITY;
-        }
-        float pr[4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float t = fmaxf(s[n][x], s[n][2 + x]);
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          const float mn = fmaxf(m[n][x], t);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          f[n][x] = fast_exp2(m[n][x] - base);
-          grew |= mn != m[n][x];
-          m[n][x] = mn;
-          pr[x] = fast_exp2(s[n][x] - base);
-          pr[2 + x] = fast_exp2(s[n][2 + x] - base);
-          l[n][x] = l[n][x] * f[n][x] + (pr[x] + pr[2 + x]);
-        }
-        if constexpr (kO) {
-          pb[n][0] = movm_t(DType<DT>::pack2(pr[0], pr[1]));
-          pb[n][1] = movm_t(DType<DT>::pack2(pr[2], pr[3]));
-        }
+      for (int x = 0; x < 2; ++x) {
+        float t = fmaxf(s[x], s[2 + x]);
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+        const float mn = fmaxf(m[x], t);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        f[x] = fast_exp2(m[x] - base);
+        grew |= mn != m[x];
+        m[x] = mn;
+        pr[x] = fast_exp2(s[x] - base);
+        pr[2 + x] = fast_exp2(s[2 + x] - base);
+        l[x] = l[x] * f[x] + (pr[x] + pr[2 + x]);
       }
       if constexpr (kO) {
+        const uint32_t pb0 = movm_t(DType<DT>::pack2(pr[0], pr[1]));
+        const uint32_t pb1 = movm_t(DType<DT>::pack2(pr[2], pr[3]));
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
           for (int d = 0; d < DK / 16; ++d)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[d][n][c] *= f[n][c & 1];
+            for (int c = 0; c < 4; ++c) o[d][c] *= f[c & 1];
         }
         const uint32_t va = st + L::kTile + ((lane & 7) + ((lane >> 4) << 3)) * L::kPitch +
                             ((lane >> 3) & 1) * 16;
@@ -304,8 +269,7 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
         for (int d = 0; d < DK / 16; ++d) {
           uint32_t a[4];
           ldsm4_t(a, va + d * 32);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<DT>(o[d][n], a, pb[n][0], pb[n][1]);
+          mma16816<DT>(o[d], a, pb0, pb1);
         }
       }
     }
@@ -326,26 +290,24 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, NT, MODE>::W,
   constexpr int kOP = DK + 4;  // floats per row of O in shared memory
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
+    const int r = (lane & 3) * 2 + x;
+    if (lane < 4) {
+      sm_m[warp][r] = m[x];
+      sm_l[warp][r] = l[x];
+    }
+    if constexpr (kO) {
+      float* row = reinterpret_cast<float*>(smem) + (warp * R + r) * kOP + (lane >> 2);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
-      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
-      l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
-      const int r = n * 8 + (lane & 3) * 2 + x;
-      if (lane < 4) {
-        sm_m[warp][r] = m[n][x];
-        sm_l[warp][r] = l[n][x];
-      }
-      if constexpr (kO) {
-        float* row = reinterpret_cast<float*>(smem) + (warp * R + r) * kOP + (lane >> 2);
-#pragma unroll
-        for (int d = 0; d < DK / 16; ++d) {
-          row[d * 16] = o[d][n][x];
-          row[d * 16 + 8] = o[d][n][2 + x];
-        }
+      for (int d = 0; d < DK / 16; ++d) {
+        row[d * 16] = o[d][x];
+        row[d * 16 + 8] = o[d][2 + x];
       }
     }
+  }
   __syncthreads();
   const int D4 = kO ? p.D >> 2 : 1;
   const bool direct = kO && p.NS == 1;
@@ -489,7 +451,6 @@ struct CachePlan {
   // fields below; ranges cover both)
   bool joint;
   bool tile[2];            // segment by cache_tiles_kernel, otherwise by cache_rows_kernel
-  int nt[2];               // 8-row tiles per item of cache_rows_kernel
   int rtiles[2], nsplit[2];
   int chunk[2];            // keys per range
   int NS;
@@ -497,15 +458,14 @@ struct CachePlan {
 
 // cache_rows_kernel: keys per range.  Four items run on each of the 148 SMs.
 // An item costs its keys plus `extra` keys (set-up, first loads, the partial
-// result: 1 us for an 8-row tile, 4 us for taller ones, at 27 keys a
-// microsecond and block).  Items of several rounds start as others end, so
-// they fill the device but for a third of an item at the end; those of a
-// single round all wait for the slowest (15 % behind).  The join costs 4 us.  Measured on a 16384-key prefix of 32 heads:
-// 16 rows 42 us at 1024 keys a range (one round), 47 at 512, 54 at 256; 8 rows
-// 39, 39, 41; two 65536-key caches 218, 215, 216.
+// result: about 1 us at 27 keys a microsecond and block).  Items of several
+// rounds start as others end, so they fill the device but for a third of an
+// item at the end; those of a single round all wait for the slowest (15 %
+// behind).  The join costs 4 us.  Measured: two 65536-key caches of 32 heads
+// 218 us at 1024 keys a range, 215 at 512, 216 at 256, 255 in one round.
 constexpr int64_t kRowsSlots = 4 * 148, kRowsUnit = 32;
-static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2], int nt) {
-  const int64_t extra = nt == 1 ? 32 : 108;
+static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
+  constexpr int64_t extra = 32;
   const double total = (double)tiles[0] * cap[0] + (double)tiles[1] * cap[1];
   int64_t best = kRowsUnit;
   double best_cost = 1e300;
@@ -526,8 +486,10 @@ static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2], in
 }
 
 // Most rows for which streaming the keys past warp-level tiles beats a 128-row
-// tcgen05 tile.
-constexpr int64_t kRowsMost = 32;
+// tcgen05 tile.  Measured, a 16384-key prefix of 32 heads (us, warp tiles of 8,
+// 16 and 32 rows against tcgen05): 8 rows 45, 16 rows 63 against 44, 32 rows
+// 105 against 47; 65536 keys of 8 heads: 16 rows 62 against 55.
+constexpr int64_t kRowsMost = 8;
 
 // cache_tiles_kernel: key blocks per range, for tiles of up to two kinds.  Two
 // items run on each of the 148 SMs; an item costs its blocks plus kItemCost
@@ -578,8 +540,7 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
   int64_t tiles[2] = {0, 0};
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
-    pl.nt[s] = rows[s] > 16 ? 4 : (rows[s] > 8 ? 2 : 1);
-    const int per = pl.tile[s] ? 128 : 8 * pl.nt[s];
+    const int per = pl.tile[s] ? 128 : 8;
     pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
     if (!pl.tile[s]) tiles[s] = nb[s] * Hkv * pl.rtiles[s];
   }
@@ -587,8 +548,7 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
   for (int s = 0; s < 2; ++s)
     if (pl.tile[s]) many[s] = nb[s] * Hkv * pl.rtiles[s], blocks[s] = (cap[s] + 63) / 64;
   const int64_t caps[2] = {tiles[0] ? cap[0] : 0, tiles[1] ? cap[1] : 0};
-  const int nt = tiles[0] && pl.nt[0] > pl.nt[1] ? pl.nt[0] : pl.nt[1];
-  const int64_t chunk = tiles[0] || tiles[1] ? rows_chunk(tiles, caps, nt) : 0;
+  const int64_t chunk = tiles[0] || tiles[1] ? rows_chunk(tiles, caps) : 0;
   const int64_t tile_chunk = many[0] || many[1] ? tile_blocks(many, blocks) * 64 : 0;
   for (int s = 0; s < 2; ++s) {
     if (!use[s]) continue;
@@ -640,14 +600,14 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <typename DT, int DK, int NT, RowsMode MODE>
+template <typename DT, int DK, RowsMode MODE>
 static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
-  using L = RowsSmem<DK, NT, MODE>;
+  using L = RowsSmem<DK, MODE>;
   constexpr int kRowsWarps = L::W;
-  constexpr auto kern = cache_rows_kernel<DT, DK, NT, MODE>;
-  constexpr int kJoin = MODE == kAttention ? kRowsWarps * 8 * NT * (DK + 4) * 4 : 0;
+  constexpr auto kern = cache_rows_kernel<DT, DK, MODE>;
+  constexpr int kJoin = MODE == kAttention ? kRowsWarps * 8 * (DK + 4) * 4 : 0;
   constexpr int bytes = L::kRing > kJoin ? L::kRing : kJoin;
-  cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, NT, MODE>>(bytes);
+  cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, MODE>>(bytes);
   if (err == cudaSuccess) {
     if (after) {
       err = launch_after(kern, dim3((unsigned)items), 32 * kRowsWarps, bytes, stream, p);
@@ -665,23 +625,17 @@ static int launch_rows(const CacheParams& p, long long items, bool after, cudaSt
 }
 
 template <RowsMode MODE>
-static int launch_rows_dk(const CacheParams& p, int dtype, int nt, long long items, bool after,
+static int launch_rows_dk(const CacheParams& p, int dtype, long long items, bool after,
                           cudaStream_t st) {
-#define MI_ROWS_CASE(DK)                                                                \
-  if (p.D <= DK) {                                                                      \
-    if (dtype == MI_BF16)                                                               \
-      return nt == 1   ? launch_rows<__nv_bfloat16, DK, 1, MODE>(p, items, after, st)   \
-             : nt == 2 ? launch_rows<__nv_bfloat16, DK, 2, MODE>(p, items, after, st)   \
-                       : launch_rows<__nv_bfloat16, DK, 4, MODE>(p, items, after, st);  \
-    return nt == 1   ? launch_rows<__half, DK, 1, MODE>(p, items, after, st)            \
-           : nt == 2 ? launch_rows<__half, DK, 2, MODE>(p, items, after, st)            \
-                     : launch_rows<__half, DK, 4, MODE>(p, items, after, st);           \
-  }
-  MI_ROWS_CASE(64)
-  MI_ROWS_CASE(96)
-  MI_ROWS_CASE(128)
-#undef MI_ROWS_CASE
-  return MI_ERR_SHAPE;
+  const bool bf = dtype == MI_BF16;
+  if (p.D <= 64)
+    return bf ? launch_rows<__nv_bfloat16, 64, MODE>(p, items, after, st)
+              : launch_rows<__half, 64, MODE>(p, items, after, st);
+  if (p.D <= 96)
+    return bf ? launch_rows<__nv_bfloat16, 96, MODE>(p, items, after, st)
+              : launch_rows<__half, 96, MODE>(p, items, after, st);
+  return bf ? launch_rows<__nv_bfloat16, 128, MODE>(p, items, after, st)
+            : launch_rows<__half, 128, MODE>(p, items, after, st);
 }
 
 static void set_seg(CacheSeg& s, const mi_rows& k, const mi_rows& v, const int32_t* len,
@@ -798,18 +752,11 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
     const int rc = launch_tiles(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, st);
     if (rc != MI_OK) return rc;
   }
-  // Both segments in one launch where they take tiles of the same height,
-  // else one after the other (the second starts as the first's blocks end).
-  bool after = tiles;
-  for (int s = 0; s < 2; ++s) {
-    if (pl.tile[s] || !items[s]) continue;
-    const bool both = s == 0 && !pl.tile[1] && items[1] && pl.nt[0] == pl.nt[1];
-    p.items0 = s == 0 ? (int)items[0] : 0;
-    const int rc = launch_rows_dk<kAttention>(p, a.dtype, pl.nt[s],
-                                              items[s] + (both ? items[1] : 0), after, st);
+  const long long few = (pl.tile[0] ? 0 : items[0]) + (pl.tile[1] ? 0 : items[1]);
+  if (few) {
+    p.items0 = pl.tile[0] ? 0 : (int)items[0];
+    const int rc = launch_rows_dk<kAttention>(p, a.dtype, few, tiles, st);
     if (rc != MI_OK) return rc;
-    if (both) break;
-    after = true;
   }
   if (p.NS == 1) return MI_OK;
   const long long nrows = B * Hq * S_q;

@@ -112,13 +112,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe; x is held to [-126, 126].
+// 2^x of two values on the FMA pipe, for x < 128 (below -126: about 1e-38).
 // x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low
 // bits), 2^f by a polynomial of degree 5, the minimax one for the relative
 // error over [-1/2, 1/2] found by Remez exchange (7.5e-8), n into the exponent.
 __device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x.x = fminf(fmaxf(x.x, -126.f), 126.f);
-  x.y = fminf(fmaxf(x.y, -126.f), 126.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
   const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
   const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
   const float2 f = fma2(n, make_float2(-1.f, -1.f), x);

@@ -54,6 +54,8 @@ __global__ void weight_lse_kernel(const float2* ml, int NS, float* lse, long lon
 constexpr int kScanThreads = 320;
 
 // acc += sum over 32 columns of 2^(s * sc + z[c]); z per column in shared memory.
+// The exponents are at most about 0 (z is minus a log-sum-exp); an lse that is
+// no row's could bring one past 128, where only the MUFU's form overflows.
 __device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, const float* z,
                                              float2& a0, float2& a1) {
   const float2 sc2 = make_float2(sc, sc);
@@ -62,26 +64,29 @@ __device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, con
     const float4 zz = *reinterpret_cast<const float4*>(z + c);
     const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(zz.x, zz.y));
     const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(zz.z, zz.w));
-    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0 ? poly_exp2(x0)
-                                               : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
-    a1 = add2(a1, (c / 2 + 1) % MI_POLY_EVERY == 0
-                      ? poly_exp2(x1)
-                      : make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
+    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0
+                      ? poly_exp2(make_float2(fminf(x0.x, 127.f), fminf(x0.y, 127.f)))
+                      : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
+    a1 = add2(a1, make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
   }
 }
-// The same with one addend for all columns.
+// The same with one addend for all columns.  top: the largest exponent of those
+// that the polynomial took (it must stay below 128).
 __device__ __forceinline__ void exp_sum_row(const float (&s)[32], float sc, float z, float2& a0,
-                                            float2& a1) {
+                                            float2& a1, float& top) {
   const float2 sc2 = make_float2(sc, sc), z2 = make_float2(z, z);
+  top = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, z2);
     const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, z2);
-    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0 ? poly_exp2(x0)
-                                               : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
-    a1 = add2(a1, (c / 2 + 1) % MI_POLY_EVERY == 0
-                      ? poly_exp2(x1)
-                      : make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
+    if ((c / 2) % MI_POLY_EVERY == 0) {
+      top = fmax3(top, x0.x, x0.y);
+      a0 = add2(a0, poly_exp2(x0));
+    } else {
+      a0 = add2(a0, make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
+    }
+    a1 = add2(a1, make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
   }
 }
 
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 256);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 128);
     mbar_init(q_full, 256);
     *abort_flag = 0;
     fence_barrier_init();
@@ -243,7 +248,8 @@ __global__ void __launch_bounds__(kScanThreads, 2)
     }
     if (!ok && lane == 0) *abort_flag = 1;
   } else {
-    // thread = row (warp & 3) * 32 + lane, columns half * 64 ...
+    // thread = row (warp & 3) * 32 + lane; warps 0-3 take the even blocks, 4-7
+    // the odd ones, each group with its own S buffer
     const int row = (warp & 3) * 32 + lane, half = warp >> 2;
     const bool live = row < nrows;
     int tok;
@@ -259,50 +265,51 @@ __global__ void __launch_bounds__(kScanThreads, 2)
     const int whi = __reduce_max_sync(0xffffffffu, live ? lim : 0);
     // not 0: a hidden score of -inf has to stay -inf when it is scaled
     const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);
-    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < nent; ++j) {
-      if (!all(mbar_wait(&s_full[j & 1], (j >> 1) & 1, 155))) { ok = false; break; }
+    for (int j = half; j < nent; j += 2) {
+      if (!all(mbar_wait(&s_full[half], (j >> 1) & 1, 155))) { ok = false; break; }
       tc_fence_after();
-      const int key0 = (j0 + j) * 128 + half * 64;
-      if (key0 < whi) {
-        const bool whole = key0 + 64 <= wlo;
-        const uint64_t vis = bits_below((long long)lim - key0);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float s[32];
-          tmem_ld32(tcol + (j & 1) * 128 + q * 32, s);
-          tmem_wait_ld();
-          if (!whole) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] = ((vis >> (q * 32 + c)) & 1ull) ? s[c] : -INFINITY;
-          }
-          float2 a0 = make_float2(0.f, 0.f), a1 = a0;
-          exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1);
-          a0 = add2(a0, a1);
-          float sum = a0.x + a0.y;
-          const bool bad = m == -INFINITY || !(sum < 1.1e12f);
-          if (__any_sync(0xffffffffu, bad)) {
-            float t = s[0];
-#pragma unroll
-            for (int c = 1; c < 31; c += 2) t = fmax3(t, s[c], s[c + 1]);
-            t = fmaxf(t, s[31]) * sc;
-            if (bad) {
-              const float mn = fmaxf(m, t);
-              if (m != -INFINITY) l *= fast_exp2(m - mn);
-              m = mn;
-            }
-            a0 = a1 = make_float2(0.f, 0.f);
-            exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1);
-            a0 = add2(a0, a1);
-            sum = m == -INFINITY ? 0.f : a0.x + a0.y;
-          }
-          l += sum;
+      for (int q = 0; q < 4; ++q) {
+        const int key0 = (j0 + j) * 128 + q * 32;
+        float s[32];
+        tmem_ld32(tcol + q * 32, s);
+        tmem_wait_ld();
+        if (q == 3) {  // the buffer may be filled again
+          tc_fence_before();
+          mbar_arrive(&s_empty[half]);
         }
+        if (key0 >= whi) continue;
+        if (key0 + 32 > wlo) {
+          const uint64_t vis = bits_below((long long)lim - key0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[c] = ((vis >> c) & 1ull) ? s[c] : -INFINITY;
+        }
+        float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+        float top;
+        exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1, top);
+        a0 = add2(a0, a1);
+        float sum = a0.x + a0.y;
+        const bool bad = m == -INFINITY || !(sum < 1.1e12f) || top > 40.f;
+        if (__any_sync(0xffffffffu, bad)) {
+          float t = s[0];
+#pragma unroll
+          for (int c = 1; c < 31; c += 2) t = fmax3(t, s[c], s[c + 1]);
+          t = fmaxf(t, s[31]) * sc;
+          if (bad) {
+            const float mn = fmaxf(m, t);
+            if (m != -INFINITY) l *= fast_exp2(m - mn);
+            m = mn;
+          }
+          a0 = a1 = make_float2(0.f, 0.f);
+          exp_sum_row(s, sc, m == -INFINITY ? -INFINITY : -m, a0, a1, top);
+          a0 = add2(a0, a1);
+          sum = m == -INFINITY ? 0.f : a0.x + a0.y;
+        }
+        l += sum;
       }
-      tc_fence_before();
-      mbar_arrive(&s_empty[j & 1]);
     }
     if (!all(ok)) *abort_flag = 1;
     float2* join = reinterpret_cast<float2*>(smem + L::kJoinOff);
@@ -328,8 +335,9 @@ __global__ void __launch_bounds__(kScanThreads, 2)
 // ---------------------------------------------------------------------------
 // Key sums: S^T = K Q^T, a tile of 128 keys (the M rows, one per thread)
 // against blocks of NB query rows.  A key's weight is a sum along its own TMEM
-// lane, so nothing crosses threads (but the two halves of a step's columns, once
-// per tile) and nothing is written back.  What a cache holds past its length
+// lane, so nothing crosses threads (but the sums of the two groups of epilogue
+// warps, once per tile) and nothing is written back.  A step is one block
+// against one tile; warps 0-3 take the even steps, 4-7 the odd ones.  What a cache holds past its length
 // stays in its own lanes, whose sums are dropped.
 //
 // RES: the rows of the key/value head are one block (NB = 64 or 128, packed
@@ -345,9 +353,9 @@ struct ColsSmem {
   static constexpr int KS = RES ? (104 * 1024 - kQBlock) / kKTile : (DK == 128 ? 1 : 2);
   static constexpr int SB = 256 / NB;  // S buffers
   static constexpr int kQOff = KS * kKTile;
-  static constexpr int kRowOff = kQOff + QS * kQBlock;  // per warp: 2 x (NB/2 x (-lse, token))
+  static constexpr int kRowOff = kQOff + QS * kQBlock;  // per warp: NB x -lse, NB x token
   static constexpr int kJoinOff = kRowOff + 8 * 2 * NB * 4;
-  static constexpr int kBarOff = kJoinOff + 128 * 4;
+  static constexpr int kBarOff = kJoinOff + 2 * 128 * 4;
   // k_full[KS] k_empty[KS] q_full[QS] q_empty[QS] s_full[SB] s_empty[SB]
   static constexpr int kSlotOff = kBarOff + (2 * KS + 2 * QS + 2 * SB) * 8;
   static constexpr int kAlloc = kSlotOff + 8 + 512;
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
                         const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ ColsParams cp) {
   using L = ColsSmem<DK, NB, RES>;
-  constexpr int NC = L::NC, KS = L::KS, QS = L::QS, SB = L::SB, NH = NB / 2;
+  constexpr int NC = L::NC, KS = L::KS, QS = L::QS, SB = L::SB;
   const WeightParams& p = cp.w;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -399,7 +407,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < QS; ++i) mbar_init(&q_full[i], RES ? 256 : 1), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < SB; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 256);
+    for (int i = 0; i < SB; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 128);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -476,8 +484,8 @@ __global__ void __launch_bounds__(kScanThreads, 2)
     }
     if (!ok && lane == 0) *abort_flag = 1;
   } else {
-    // thread = key (warp & 3) * 32 + lane of the tile, columns half * NH ...
-    const int key = (warp & 3) * 32 + lane, half = warp >> 2;
+    // thread = key (warp & 3) * 32 + lane of the tile
+    const int key = (warp & 3) * 32 + lane, grp = warp >> 2;
     if constexpr (RES) {
       if (tv > t0) {
         if (warp * 16 < NB)
@@ -487,95 +495,111 @@ __global__ void __launch_bounds__(kScanThreads, 2)
       }
     }
     pdl_wait();  // lse may come from the kernel before
-    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * NH;
-    float* srow = reinterpret_cast<float*>(smem + L::kRowOff) + warp * (2 * NB);
+    const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    float* nz = reinterpret_cast<float*>(smem + L::kRowOff) + warp * (2 * NB);
+    int* tok = reinterpret_cast<int*>(nz) + NB;
     float* join = reinterpret_cast<float*>(smem + L::kJoinOff);
     const float* win = p.win ? p.win + b * p.wi_b + h * p.wi_h : nullptr;
     float* wout = p.wout + b * p.wo_b + h * p.wo_h;
     const float* lse = p.lse + ((long long)b * p.Hq + h * p.group) * p.Sq;
-    // -lse (log2 units; -inf: adds nothing) and tokens of this warp's columns of
-    // a block of rows, to shared memory; fetched a block ahead
-    float zn[NH / 32];
+    // a block's rows: -lse (log2 units; -inf: adds nothing) and tokens, in
+    // shared memory of the warp; fetched a step of the group ahead
+    float zn[NB / 32];
     auto fetch = [&](int g, int sb) {
 #pragma unroll
-      for (int x = 0; x < NH / 32; ++x) {
-        const int r = sb * NB + half * NH + x * 32 + lane;
-        zn[x] = r < (RES ? rows : p.Sq) ? lse[(long long)g * p.Sq + r] : -INFINITY;
+      for (int x = 0; x < NB / 32; ++x) {
+        const int r = sb * NB + x * 32 + lane;
+        zn[x] = g < heads && r < (RES ? rows : p.Sq) ? lse[(long long)g * p.Sq + r] : -INFINITY;
       }
     };
-    auto lay = [&](int sb, float* nz) {
-#pragma unroll
-      for (int x = 0; x < NH / 32; ++x) {
-        const int r = sb * NB + half * NH + x * 32 + lane;
-        nz[x * 32 + lane] = zn[x] == -INFINITY ? zn[x] : -zn[x] * p.lse_mul;
-        reinterpret_cast<int*>(nz)[NH + x * 32 + lane] = RES ? cp.div_sq.mod(r) : r;
-      }
-    };
-    if (RES && tv > t0) {
-      fetch(0, 0);
-      lay(0, srow);
+    auto lay = [&](int sb) {
       __syncwarp();
-    }
-    bool ok = true;
-    int n = 0;
-    for (int t = t0; t < t1; ++t) {
-      const int j = t * 128 + key;
-      const float w0 = !half && win && j < min(len, p.C) ? win[j] : 0.f;
-      float tot = 0.f;
-      // token from which a row sees the key
-      const int smin = p.causal ? j - len + p.Sq : 0;
-      const int wmin = __shfl_sync(0xffffffffu, smin, 31);
-      if (ok && t < tv) {
-        const int f = first_block(t);
-        if (!RES) fetch(0, f);
-        for (int g = 0; ok && g < heads; ++g)
-          for (int sb = f; sb < nsb; ++sb, ++n) {
-            float* nz = RES ? srow : srow + (n & 1) * NB;
-            if constexpr (!RES) {
-              lay(sb, nz);
-              __syncwarp();
-              if (sb + 1 < nsb) fetch(g, sb + 1);
-              else if (g + 1 < heads) fetch(g + 1, f);
-            }
-            const int buf = n % SB;
-            if (!all(mbar_wait(&s_full[buf], (n / SB) & 1, 146))) { ok = false; break; }
-            tc_fence_after();
-            const bool whole = RES ? wmin <= 0 : wmin <= sb * NB + half * NH;
-            float2 a0 = make_float2(0.f, 0.f), a1 = a0;
 #pragma unroll
-            for (int q = 0; q < NH / 32; ++q) {
-              float s[32];
-              tmem_ld32(tcol + buf * NB + q * 32, s);
-              tmem_wait_ld();
-              if (q == NH / 32 - 1) {
-                tc_fence_before();
-                mbar_arrive(&s_empty[buf]);
-              }
-              if (whole) {
-                exp_sum_cols(s, p.scale_log2, nz + q * 32, a0, a1);
-              } else {
-                const int* tok = reinterpret_cast<const int*>(nz) + NH + q * 32;
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  if (tok[c] >= smin) a0.x += fast_exp2(fmaf(s[c], p.scale_log2, nz[q * 32 + c]));
-              }
-            }
-            a0 = add2(a0, a1);
-            tot += a0.x + a0.y;  // two-level sum: a block, then the blocks
-          }
+      for (int x = 0; x < NB / 32; ++x) {
+        const int r = sb * NB + x * 32 + lane;
+        nz[x * 32 + lane] = zn[x] == -INFINITY ? zn[x] : -zn[x] * p.lse_mul;
+        tok[x * 32 + lane] = RES ? cp.div_sq.mod(r) : r;
       }
-      // the two halves of the columns meet once per tile
-      if (half) join[key] = tot;
-      named_barrier(1, 256);
-      if (!half) {
-        tot += join[key];
-        if (j < len) {
-          if (ok) wout[j] = w0 + tot;
-        } else if (j < p.C && win != wout) {
-          wout[j] = win ? win[j] : 0.f;
+      __syncwarp();
+    };
+    bool ok = true;
+    // Sum over the rows of step n's block; whole: all of them see all of the
+    // warp's keys, otherwise those of tokens from smin on see this thread's.
+    auto step = [&](int n, bool whole, int smin) -> float {
+      const int buf = n % SB;
+      ok = all(mbar_wait(&s_full[buf], (n / SB) & 1, 146));
+      if (!ok) return 0.f;
+      tc_fence_after();
+      float2 a0 = make_float2(0.f, 0.f), a1 = a0;
+#pragma unroll
+      for (int q = 0; q < NB / 32; ++q) {
+        float s[32];
+        tmem_ld32(tcol + buf * NB + q * 32, s);
+        tmem_wait_ld();
+        if (q == NB / 32 - 1) {  // the buffer may be filled again
+          tc_fence_before();
+          mbar_arrive(&s_empty[buf]);
+        }
+        if (whole) {
+          exp_sum_cols(s, p.scale_log2, nz + q * 32, a0, a1);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (tok[q * 32 + c] >= smin)
+              a0.x += fast_exp2(fmaf(s[c], p.scale_log2, nz[q * 32 + c]));
         }
       }
-      named_barrier(2, 256);
+      a0 = add2(a0, a1);
+      return a0.x + a0.y;  // a block's sum; the blocks add up outside
+    };
+    if constexpr (RES) {
+      // a step per tile: each group has its own tiles
+      if (tv > t0) {
+        fetch(0, 0);
+        lay(0);
+      }
+      for (int t = t0 + grp; t < t1; t += 2) {
+        const int j = t * 128 + key;
+        const float w0 = win && j < p.C ? win[j] : 0.f;
+        const int smin = p.causal ? j - len + p.Sq : 0;  // token from which a row sees the key
+        float tot = 0.f;
+        if (ok && t < tv) tot = step(t - t0, __shfl_sync(0xffffffffu, smin, 31) <= 0, smin);
+        if (j < len ? ok : (j < p.C && win != wout)) wout[j] = j < len ? w0 + tot : w0;
+      }
+    } else {
+      int n = 0;
+      for (int t = t0; t < t1; ++t) {
+        const int j = t * 128 + key;
+        const float w0 = !grp && win && j < p.C ? win[j] : 0.f;
+        const int smin = p.causal ? j - len + p.Sq : 0;
+        const int wmin = __shfl_sync(0xffffffffu, smin, 31);
+        float tot = 0.f;
+        if (t < tv) {
+          const int f = first_block(t), per = nsb - f, steps = heads * per;
+          // this group's steps of the tile: i, i + 2, ... as (head, block)
+          int i = (n ^ grp) & 1, g = 0, sb = f;
+          auto advance = [&](int by) {
+            sb += by;
+            while (sb >= nsb) sb -= per, ++g;
+          };
+          advance(i);
+          if (i < steps) fetch(g, sb);
+          for (; ok && i < steps; i += 2) {
+            const int cur = sb;
+            lay(cur);
+            advance(2);
+            if (i + 2 < steps) fetch(g, sb);
+            tot += step(n + i, wmin <= cur * NB, smin);
+          }
+          n += steps;
+        }
+        // the groups' sums meet once per tile; a buffer is written again two
+        // barriers after it was read
+        if (grp) join[(t & 1) * 128 + key] = tot;
+        named_barrier(1, 256);
+        if (!grp && (j < len ? ok : (j < p.C && win != wout)))
+          wout[j] = j < len ? w0 + (tot + join[(t & 1) * 128 + key]) : w0;
+      }
     }
     if (!all(ok)) *abort_flag = 1;
   }
@@ -637,10 +661,12 @@ static int launch_cols_t(const WeightParams& w, const mi_rows& q, const mi_rows&
   cp.w = w;
   cp.tiles = (w.C + 127) / 128;
   const long long all = (long long)w.B * w.Hkv * cp.tiles;
-  // tiles per item: with resident rows, two rounds of two items per SM;
+  // tiles per item: with resident rows three rounds of two items per SM
+  // (one: 162 us for 64 rows of 32 x 65536 keys, two and three: 138);
   // otherwise enough that an item has 16 blocks
   const long long steps = (long long)w.group * ((w.Sq + NB - 1) / NB);
-  const long long per = RES ? (all + 148 * 4 - 1) / (148 * 4) : (16 + steps - 1) / steps;
+  const long long slots = 148 * 2 * 3;
+  const long long per = RES ? (all + slots - 1) / slots : (16 + steps - 1) / steps;
   cp.per = (int)(per < 1 ? 1 : (per > cp.tiles ? cp.tiles : per));
   const int ranges = (cp.tiles + cp.per - 1) / cp.per;
   cp.ranges = FastDiv(ranges);
@@ -798,7 +824,7 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   if (!lse) {
     p.ml = ml;
-    rc = launch_rows_dk<kStats>(p, dtype, pl.nt[1], items, false, st);
+    rc = launch_rows_dk<kStats>(p, dtype, items, false, st);
     if (rc != MI_OK) return rc;
     weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(ml, pl.NS, lse2,
                                                                       (long long)rows);
@@ -814,5 +840,5 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   p.wout = w.wout;
   p.wo_b = w.wo_b;
   p.wo_h = w.wo_h;
-  return launch_rows_dk<kWeights>(p, dtype, pl.nt[1], items, false, st);
+  return launch_rows_dk<kWeights>(p, dtype, items, false, st);
 }
