@@ -505,7 +505,7 @@ static int64_t tile_blocks(const int64_t (&tiles)[2], const int64_t (&blocks)[2]
   for (int64_t rounds = 0; rounds <= 6; ++rounds) {
     int64_t per = most, items = 0;
     if (rounds) per = (int64_t)(total / (rounds * slots)) + 1;
-    for (;; ++per) {  // the shortest ranges that fit these rounds
+    for (;; per += per / 32 + 1) {  // about the shortest ranges that fit these rounds
       items = tiles[0] * ((blocks[0] + per - 1) / per) + tiles[1] * ((blocks[1] + per - 1) / per);
       if (!rounds || items <= rounds * slots || per >= most) break;
     }

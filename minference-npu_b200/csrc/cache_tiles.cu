@@ -328,11 +328,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         float2 t0 = make_float2(0.f, 0.f), t1 = t0;
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float x0 = fast_exp2(__fmaf_rn(s[2 * c], sc, nm));
-          const float x1 = fast_exp2(__fmaf_rn(s[2 * c + 1], sc, nm));
-          if (c & 1) t1 = add2(t1, make_float2(x0, x1));
-          else t0 = add2(t0, make_float2(x0, x1));
-          pk[c] = DType<DT>::pack2(x0, x1);
+          const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), make_float2(sc, sc),
+                                make_float2(nm, nm));
+          const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          if (c & 1) t1 = add2(t1, e);
+          else t0 = add2(t0, e);
+          pk[c] = DType<DT>::pack2(e.x, e.y);
         }
         t0 = add2(t0, t1);
         return t0.x + t0.y;

@@ -15,13 +15,15 @@ _DTYPES = {torch.float16: _native.MI_F16, torch.bfloat16: _native.MI_BF16}
 
 def check_same(name: str, x: torch.Tensor, like: torch.Tensor, shape: tuple) -> None:
     """`x` has the given shape and `like`'s dtype and device."""
+    if isinstance(x, torch.Tensor) and x.shape == shape and x.dtype is like.dtype \
+            and x.device == like.device:
+        return
     if not isinstance(x, torch.Tensor) or x.shape != shape:
         got = tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__
         raise ValueError(f"{name} must be {tuple(shape)}, got {got}")
     if x.dtype is not like.dtype:
         raise TypeError(f"{name} is {x.dtype}, expected {like.dtype}")
-    if x.device != like.device:
-        raise ValueError(f"{name} is on {x.device}, expected {like.device}")
+    raise ValueError(f"{name} is on {x.device}, expected {like.device}")
 
 
 def check_query(q: torch.Tensor, Hkv: int) -> int:

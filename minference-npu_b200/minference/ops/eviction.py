@@ -137,9 +137,8 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, keep: i
     clen = None if lengths is None else lengths_arg("lengths", lengths, B, C, dev)
     shape = (B, H, keep, D)
     if out is None:
-        ko = torch.empty(shape, dtype=k.dtype, device=dev)
-        vo = torch.empty(shape, dtype=k.dtype, device=dev)
-        wo = torch.empty(shape[:3], dtype=torch.float32, device=dev)
+        ko, vo = k.new_empty(shape), k.new_empty(shape)
+        wo = weights.new_empty(shape[:3])
     else:
         ko, vo, wo = out
         check_same("out[0]", ko, k, shape)

@@ -41,7 +41,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
     ``causal``, the own keys up to itself (bottom-right aligned), otherwise
     every valid own key.  Lengths are integer device tensors (None: whole),
     clamped to the capacity; rows past them are never used, whatever they hold.
-    A token that sees nothing gives 0.
+    Values within a length must be finite (one that a token does not see is
+    still multiplied by 0).  A token that sees nothing gives 0.
 
     ``scale`` defaults to ``1/sqrt(D)``.  Returns the output, of q's dtype, or
     with ``return_lse`` the pair (output, lse float32 ``[B,Hq,S_q]``: natural
@@ -88,7 +89,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
 
     dk = max(32, (D + 7) & ~7)
     if out is None:
-        res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
+        res = q.new_empty((B, Hq, S_q, dk))
     else:
         check_same("out", out, q, (B, Hq, S_q, D))
         check_output("out", out)
@@ -99,7 +100,7 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
         if dk == D:
             res = _common_out(out, (B, Hq, S_q, D), q)
         else:
-            res = torch.empty((B, Hq, S_q, dk), dtype=q.dtype, device=q.device)
+            res = q.new_empty((B, Hq, S_q, dk))
     lse = torch.empty((B, Hq, S_q), dtype=torch.float32, device=q.device) if return_lse else None
     hold: list = []
     args = _native.SHARED_PREFIX_ARGS.pack(

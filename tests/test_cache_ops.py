@@ -240,6 +240,30 @@ def test_attention_scales(cuda, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("Sq", [1, 5, 70])
+def test_attention_rising_scores(cuda, Sq, dtype):
+    """Every block's scores lie above those before, by hundreds in all: the
+    running reference has to move, at every height of the row tile."""
+    from minference import ops
+
+    q, kp, vp, k, v = make((2, 8, 2, Sq, 1, 900, 200, 128, dtype, "bhsd"), 30)
+    ramp = torch.linspace(0.2, 12.0, 1100, device="cuda")
+    q = q.abs()
+    kp = (kp.abs() * ramp[:900, None]).to(dtype)
+    k = (k.abs() * ramp[900:, None]).to(dtype)
+    out, lse = ops.shared_prefix_attention(q, kp, vp, k, v, return_lse=True)
+    ref, tol, rl, lt = ref_attention(q, kp, vp, k, v)
+    assert rl.max() - (q[0, 0, 0].double() @ kp[0, 0, 0].double()) * 128**-0.5 > 60
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert ((lse.double() - rl).abs() <= lt).all()
+    # and falling: what comes first stays the reference
+    out = ops.shared_prefix_attention(q, kp.flip(2), vp.flip(2), k, v)
+    ref, tol, _, _ = ref_attention(q, kp.flip(2), vp.flip(2), k, v)
+    assert ((out.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [96, 40, 33])
 def test_attention_writes_the_given_view_only(cuda, D):
     from minference import ops
@@ -361,6 +385,33 @@ def test_weights_ragged_and_added_in_place(cuda, case, given):
         out = torch.full((B, Hkv, C), 5.0, device="cuda")
         ops.accumulate_attention_weights(q, kk, w0[:, :, 1:C + 1], lt, lse=lse, out=out)
         assert torch.equal(out, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 64, 200])
+@pytest.mark.parametrize("scale", [0.0, -0.7, 3.0])
+def test_weights_scales(cuda, Sq, scale):
+    from minference import ops
+
+    q, _, _, k, _ = make((2, 4, 2, Sq, 1, 0, 777, 96, FP, "bhsd"), 31)
+    w = ops.accumulate_attention_weights(q, k, scale=scale)
+    ref, tol = ref_weights(q, k, None, scale=scale)
+    assert ((w.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 64, 300])
+def test_weights_rising_scores(cuda, Sq):
+    from minference import ops
+
+    for flip in (False, True):
+        q, _, _, k, _ = make((1, 4, 2, Sq, 1, 0, 1300, 128, BF, "bhsd"), 32)
+        q = q.abs()
+        ramp = torch.linspace(0.2, 12.0, 1300, device="cuda")
+        k = (k.abs() * (ramp.flip(0) if flip else ramp)[:, None]).to(BF)
+        w = ops.accumulate_attention_weights(q, k)
+        ref, tol = ref_weights(q, k, None)
+        assert ((w.double() - ref).abs() <= tol).all()
 
 
 @pytest.mark.gpu
