@@ -44,13 +44,14 @@ __global__ void weight_lse_kernel(const float2* ml, int NS, float* lse, long lon
 // Q K^T that keep nothing of it, row statistics and key sums.  Both are bound
 // by the exponentials, one per (row, key) and pass: 16 per clock and SM on the
 // MUFU unit.  Every fourth pair is computed on the FMA pipe instead
-// (poly_exp2), and eight epilogue warps (two per TMEM lane quadrant, each with
-// half of a step's columns) on each of two blocks per SM hide the latencies of
-// either.  Warp 8 issues TMA, warp 9 the products.
+// (poly_exp2), and eight epilogue warps (two per TMEM lane quadrant, taking
+// turns at the steps) on each of two blocks per SM hide the latencies of either.
+// Warp 8 issues TMA, warp 9 the products.  Measured, all queries of a 16384
+// prompt of 32 heads of 96: 2.50 ms with the MUFU alone, 2.39 with every eighth
+// pair on the FMA pipe, 2.37 with every fourth, 2.78 with every second; four
+// epilogue warps 3.66.
 // ---------------------------------------------------------------------------
-#ifndef MI_POLY_EVERY
-#define MI_POLY_EVERY 4
-#endif
+constexpr int kPolyEvery = 4;
 constexpr int kScanThreads = 320;
 
 // acc += sum over 32 columns of 2^(s * sc + z[c]); z per column in shared memory.
@@ -64,7 +65,7 @@ __device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, con
     const float4 zz = *reinterpret_cast<const float4*>(z + c);
     const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(zz.x, zz.y));
     const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(zz.z, zz.w));
-    a0 = add2(a0, (c / 2) % MI_POLY_EVERY == 0
+    a0 = add2(a0, (c / 2) % kPolyEvery == 0
                       ? poly_exp2(make_float2(fminf(x0.x, 127.f), fminf(x0.y, 127.f)))
                       : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
     a1 = add2(a1, make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
@@ -80,7 +81,7 @@ __device__ __forceinline__ void exp_sum_row(const float (&s)[32], float sc, floa
   for (int c = 0; c < 32; c += 4) {
     const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, z2);
     const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, z2);
-    if ((c / 2) % MI_POLY_EVERY == 0) {
+    if ((c / 2) % kPolyEvery == 0) {
       top = fmax3(top, x0.x, x0.y);
       a0 = add2(a0, poly_exp2(x0));
     } else {
