@@ -464,7 +464,7 @@ struct CachePlan {
 // behind).  The join costs 4 us.  Measured: two 65536-key caches of 32 heads
 // 218 us at 1024 keys a range, 215 at 512, 216 at 256, 255 in one round.
 constexpr int64_t kRowsSlots = 4 * 148, kRowsUnit = 32;
-static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
+static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2], double* out_cost) {
   constexpr int64_t extra = 32;
   const double total = (double)tiles[0] * cap[0] + (double)tiles[1] * cap[1];
   int64_t best = kRowsUnit;
@@ -482,20 +482,27 @@ static int64_t rows_chunk(const int64_t (&tiles)[2], const int64_t (&cap)[2]) {
     if (ch < cap[0] || ch < cap[1]) cost += 110;
     if (cost < best_cost) best_cost = cost, best = ch;
   }
+  *out_cost = best_cost;
   return best;
 }
 
-// Most rows for which streaming the keys past warp-level tiles beats a 128-row
-// tcgen05 tile.  Measured, a 16384-key prefix of 32 heads (us, warp tiles of 8,
-// 16 and 32 rows against tcgen05): 8 rows 45, 16 rows 63 against 44, 32 rows
-// 105 against 47; 65536 keys of 8 heads: 16 rows 62 against 55.
-constexpr int64_t kRowsMost = 8;
+// Up to kRowsMost rows go past warp-level tiles, more than kRowsPast to 128-row
+// tcgen05 tiles; between, one or several 8-row tiles win while there are few
+// keys (they need no second kernel and little set-up), the tcgen05 tile
+// otherwise, and the costs of both plans decide.  Measured (us, 8-row tiles
+// against tcgen05): 16 rows of 8 heads over a prefix of 256, 1024 and 4096 keys 7.4,
+// 11.6, 14.6 against 13.8, 14.9, 16.9; four own caches of 4096 keys 23.4 against 18.9;
+// 16384 keys of 32 heads 63 against 44.
+constexpr int64_t kRowsMost = 8, kRowsPast = 32;
+constexpr double kRowsKeysPerUs = 27.0 * 96;  // times the head dim; a block of cache_rows_kernel
+constexpr double kSecondKernelUs = 3;
 
 // cache_tiles_kernel: key blocks per range, for tiles of up to two kinds.  Two
 // items run on each of the 148 SMs; an item costs its blocks plus kItemCost
 // (set-up, first loads, epilogue), and a partial result to be joined kJoinCost
 // more, in units of a 64-key block (1 us).
-static int64_t tile_blocks(const int64_t (&tiles)[2], const int64_t (&blocks)[2]) {
+static int64_t tile_blocks(const int64_t (&tiles)[2], const int64_t (&blocks)[2],
+                           double* out_cost = nullptr) {
   constexpr double kItemCost = 5, kJoinCost = 4;
   const int64_t slots = 2 * 148;
   const int64_t most = blocks[0] > blocks[1] ? blocks[0] : blocks[1];
@@ -513,23 +520,55 @@ static int64_t tile_blocks(const int64_t (&tiles)[2], const int64_t (&blocks)[2]
     const double cost = (double)waves * (per + kItemCost + (per < most ? kJoinCost : 0));
     if (cost < best_cost) best_cost = cost, best = per < most ? per : most;
   }
+  if (out_cost) *out_cost = best_cost;
   return best < 1 ? 1 : best;
 }
 
-static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
-                            int64_t P, int64_t C) {
+// The plan with each segment by the kernel that `tile` names, and its cost in us.
+static CachePlan cache_plan_of(const bool (&tile)[2], const bool (&use)[2],
+                               const int64_t (&rows)[2], const int64_t (&cap)[2],
+                               const int64_t (&nb)[2], int64_t Hkv, int64_t D, double* cost) {
   CachePlan pl{};
+  int64_t few[2] = {0, 0}, few_cap[2] = {0, 0};   // tiles and keys by cache_rows_kernel
+  int64_t many[2] = {0, 0}, blocks[2] = {0, 0};   // tiles and key blocks by cache_tiles_kernel
+  for (int s = 0; s < 2; ++s) {
+    if (!use[s]) continue;
+    pl.tile[s] = tile[s];
+    const int per = tile[s] ? 128 : 8;
+    pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
+    if (tile[s]) many[s] = nb[s] * Hkv * pl.rtiles[s], blocks[s] = (cap[s] + 63) / 64;
+    else few[s] = nb[s] * Hkv * pl.rtiles[s], few_cap[s] = cap[s];
+  }
+  double few_cost = 0, many_cost = 0;
+  const bool any_few = few[0] || few[1], any_many = many[0] || many[1];
+  const int64_t chunk = any_few ? rows_chunk(few, few_cap, &few_cost) : 0;
+  const int64_t tile_chunk = any_many ? tile_blocks(many, blocks, &many_cost) * 64 : 0;
+  for (int s = 0; s < 2; ++s) {
+    if (!use[s]) continue;
+    const int64_t ch = tile[s] ? tile_chunk : chunk;
+    pl.chunk[s] = (int)ch;
+    // at least one range: with no key at all it writes the zeros
+    pl.nsplit[s] = cap[s] ? (int)((cap[s] + ch - 1) / ch) : 1;
+  }
+  pl.NS = pl.nsplit[0] + pl.nsplit[1];
+  *cost = few_cost * D / kRowsKeysPerUs + many_cost + (any_few && any_many ? kSecondKernelUs : 0);
+  return pl;
+}
+
+static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t G,
+                            int64_t P, int64_t C, int64_t D) {
   const bool use[2] = {P > 0, C > 0 || P == 0};
   const int64_t rows[2] = {use[0] ? B / G * group * Sq : 0, use[1] ? group * Sq : 0};
   const int64_t cap[2] = {P, C}, nb[2] = {G, B};
-  for (int s = 0; s < 2; ++s) pl.tile[s] = cap[s] > 0 && rows[s] > kRowsMost;
+  bool tile[2];
+  for (int s = 0; s < 2; ++s) tile[s] = cap[s] > 0 && rows[s] > kRowsMost;
   // One walk over prefix and own keys where a sequence's rows fill tiles about
   // as well as all sequences' rows together do.
   const int64_t own_tiles = B * ((rows[1] + 127) / 128);
   const int64_t all_tiles = G * ((rows[0] + 127) / 128);
-  pl.joint = pl.tile[0] && pl.tile[1] && own_tiles * 4 <= all_tiles * 5;
-  if (pl.joint) {
-    pl.tile[0] = false;
+  if (tile[0] && tile[1] && rows[1] > kRowsPast && own_tiles * 4 <= all_tiles * 5) {
+    CachePlan pl{};
+    pl.joint = pl.tile[1] = true;
     pl.rtiles[1] = (int)((rows[1] + 127) / 128);
     const int64_t blocks = (P + 63) / 64 + (C + 63) / 64;
     pl.chunk[1] = (int)tile_blocks({0, B * Hkv * pl.rtiles[1]}, {0, blocks}) * 64;
@@ -537,28 +576,16 @@ static CachePlan cache_plan(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, i
     pl.NS = pl.nsplit[1];
     return pl;
   }
-  int64_t tiles[2] = {0, 0};
-  for (int s = 0; s < 2; ++s) {
-    if (!use[s]) continue;
-    const int per = pl.tile[s] ? 128 : 8;
-    pl.rtiles[s] = (int)((rows[s] + per - 1) / per);
-    if (!pl.tile[s]) tiles[s] = nb[s] * Hkv * pl.rtiles[s];
+  double best_cost, cost;
+  CachePlan best = cache_plan_of(tile, use, rows, cap, nb, Hkv, D, &best_cost);
+  const bool open[2] = {tile[0] && rows[0] <= kRowsPast, tile[1] && rows[1] <= kRowsPast};
+  for (int c = 1; c < 4; ++c) {  // with the segments of few rows that are open the other way
+    if (((c & 1) && !open[0]) || ((c & 2) && !open[1])) continue;
+    const bool other[2] = {tile[0] && !(c & 1), tile[1] && !(c & 2)};
+    const CachePlan pl = cache_plan_of(other, use, rows, cap, nb, Hkv, D, &cost);
+    if (cost < best_cost) best_cost = cost, best = pl;
   }
-  int64_t many[2] = {0, 0}, blocks[2] = {0, 0};  // by cache_tiles_kernel
-  for (int s = 0; s < 2; ++s)
-    if (pl.tile[s]) many[s] = nb[s] * Hkv * pl.rtiles[s], blocks[s] = (cap[s] + 63) / 64;
-  const int64_t caps[2] = {tiles[0] ? cap[0] : 0, tiles[1] ? cap[1] : 0};
-  const int64_t chunk = tiles[0] || tiles[1] ? rows_chunk(tiles, caps) : 0;
-  const int64_t tile_chunk = many[0] || many[1] ? tile_blocks(many, blocks) * 64 : 0;
-  for (int s = 0; s < 2; ++s) {
-    if (!use[s]) continue;
-    const int64_t ch = pl.tile[s] ? tile_chunk : chunk;
-    pl.chunk[s] = (int)ch;
-    // at least one range: with no key at all it writes the zeros
-    pl.nsplit[s] = cap[s] ? (int)((cap[s] + ch - 1) / ch) : 1;
-  }
-  pl.NS = pl.nsplit[0] + pl.nsplit[1];
-  return pl;
+  return best;
 }
 
 static bool cache_sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t G, int64_t P,
@@ -674,7 +701,7 @@ using namespace mib200;
 extern "C" size_t mi_shared_prefix_fwd_workspace_size(const mi_shared_prefix_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, a->G, a->P, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0) return 0;
-  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C);
+  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C, a->D);
   if (pl.NS == 1) return 0;
   const double need = (double)a->B * a->Hq * a->S_q * pl.NS * (a->D * 4 + 8);
   if (need > 1e15) return SIZE_MAX;
@@ -695,7 +722,7 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
     return MI_ERR_ALIGN;
   if (C && (!rows_ok(a.k, B, Hkv, C) || !rows_ok(a.v, B, Hkv, C))) return MI_ERR_ALIGN;
   const int64_t group = Hq / Hkv;
-  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C);
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C, D);
   const size_t need = mi_shared_prefix_fwd_workspace_size(args);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||

@@ -40,7 +40,7 @@ __global__ void weight_lse_kernel(const float2* ml, int NS, float* lse, long lon
 }
 
 // ---------------------------------------------------------------------------
-// Many rows (more than kRowsMost per key/value head): two tcgen05 passes over
+// Many rows (more than 8 per key/value head): two tcgen05 passes over
 // Q K^T that keep nothing of it, row statistics and key sums.  Both are bound
 // by the exponentials, one per (row, key) and pass: 16 per clock and SM on the
 // MUFU unit.  Every fourth pair is computed on the FMA pipe instead
@@ -724,15 +724,16 @@ static int launch_weights_many(const WeightParams& w, const mi_rows& q, const mi
 using namespace mib200;
 
 // Partial statistics per row of the call's split.
-static int64_t weights_slots(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t C) {
-  const CachePlan pl = cache_plan(B, Hkv, group, Sq, 1, 0, C);
-  return pl.tile[1] ? stat_ranges(B, Hkv, group * Sq, C) : pl.NS;
+static int64_t weights_slots(int64_t B, int64_t Hkv, int64_t group, int64_t Sq, int64_t C,
+                             int64_t D) {
+  return group * Sq > kRowsMost ? stat_ranges(B, Hkv, group * Sq, C)
+                                : cache_plan(B, Hkv, group, Sq, 1, 0, C, D).NS;
 }
 
 extern "C" size_t mi_attn_weights_workspace_size(const mi_attn_weights_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, 1, 0, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0 || a->C == 0 || a->lse) return 0;
-  const int64_t ns = weights_slots(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->C);
+  const int64_t ns = weights_slots(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->C, a->D);
   const size_t rows = (size_t)(a->B * a->Hq * a->S_q);
   if ((double)rows * ns > 1e13) return SIZE_MAX;
   return align_up(rows * ns * 8) + align_up(rows * 4);
@@ -790,15 +791,14 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   w.causal = a.causal ? 1 : 0;
   w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
 
-  const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C);
   const size_t rows = (size_t)(B * Hq * S_q);
   float2* ml = static_cast<float2*>(workspace);
   float* lse2 = nullptr;
   if (!lse)
     lse2 = reinterpret_cast<float*>(
         static_cast<uint8_t*>(workspace) +
-        align_up(rows * weights_slots(B, Hkv, group, S_q, C) * 8));
-  if (pl.tile[1]) {
+        align_up(rows * weights_slots(B, Hkv, group, S_q, C, D) * 8));
+  if (group * S_q > kRowsMost) {  // the few-row form needs all rows in one tile
 #define MI_MANY(DK)                                                                      \
   if (D <= DK)                                                                           \
     return dtype == MI_BF16 ? launch_weights_many<__nv_bfloat16, DK>(w, q, k, ml, lse2, st) \
@@ -808,6 +808,7 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
     MI_MANY(128)
 #undef MI_MANY
   }
+  const CachePlan pl = cache_plan(B, Hkv, group, S_q, 1, 0, C, D);
   CacheParams p{};
   p.q = w.q;
   p.qs_b = w.qs_b;

@@ -16,7 +16,7 @@ _DTYPES = {torch.float16: _native.MI_F16, torch.bfloat16: _native.MI_BF16}
 def check_same(name: str, x: torch.Tensor, like: torch.Tensor, shape: tuple) -> None:
     """`x` has the given shape and `like`'s dtype and device."""
     if isinstance(x, torch.Tensor) and x.shape == shape and x.dtype is like.dtype \
-            and x.device == like.device:
+            and x.get_device() == like.get_device():
         return
     if not isinstance(x, torch.Tensor) or x.shape != shape:
         got = tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__
@@ -49,22 +49,21 @@ def lengths_arg(name: str, x, n: int, cap: int, device: torch.device):
         raise ValueError(f"{name} must be ({n},), got {tuple(x.shape)}")
     if x.dtype is not torch.int32:
         x = x.clamp(0, cap).to(torch.int32)
-    if x.device != device:
+    if x.get_device() != device.index:
         x = x.to(device)
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
-def rows_arg(x: torch.Tensor, D: int, hold: list) -> tuple[int, int, int, int]:
-    """(address, strides) of `x`'s rows for the C structs: the head dim padded to
-    D by zeros, rows that 16-byte loads and tensor maps can read.  A view without
-    them is copied; `hold` then keeps the copy until the launch."""
+def rows_arg(x: torch.Tensor, pad: int, hold: list) -> tuple[int, int, int, int]:
+    """(address, strides) of `x`'s rows for the C structs: the head dim with `pad`
+    zeros behind it, rows that 16-byte loads and tensor maps can read.  A view
+    without them is copied; `hold` then keeps the copy until the launch."""
     p = x.data_ptr()
     b, h, s, d = x.stride()
-    if x.shape[3] == D and d == 1 and not (p | b * 2 | h * 2 | s * 2) & 15 \
-            and b > 0 and h > 0 and s > 0:
+    if not pad and d == 1 and not (p | (b | h | s) << 1) & 15 and b > 0 and h > 0 and s > 0:
         return p, b, h, s
-    if x.shape[3] != D:
-        x = F.pad(x, (0, D - x.shape[3]))
+    if pad:
+        x = F.pad(x, (0, pad))
     elif d != 1 or p & 15 or any(
             n > 1 and (t <= 0 or t % 8) for n, t in zip(x.shape[:3], (b, h, s))):
         x = x.clone(memory_format=torch.contiguous_format)
@@ -74,8 +73,12 @@ def rows_arg(x: torch.Tensor, D: int, hold: list) -> tuple[int, int, int, int]:
 
 def span(x: torch.Tensor) -> tuple[int, int]:
     """Addresses [first, end) that a strided view covers."""
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return 0, 0
+    if x.is_contiguous():
+        p = x.data_ptr()
+        return p, p + n * x.element_size()
     last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
     return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
 
@@ -87,6 +90,8 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def check_output(name: str, x: torch.Tensor) -> None:
     """Every element of an output view has its own address."""
+    if x.is_contiguous():
+        return
     need = 1
     for n, s in sorted(zip(x.shape, x.stride()), key=lambda t: t[1]):
         if n > 1:

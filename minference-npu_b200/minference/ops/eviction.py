@@ -32,6 +32,9 @@ class EvictedCache(NamedTuple):
 
 
 def _check_weights(name: str, w, shape: tuple, device: torch.device) -> None:
+    if isinstance(w, torch.Tensor) and w.shape == shape and w.dtype is torch.float32 \
+            and w.get_device() == device.index and w.is_contiguous():
+        return
     if not isinstance(w, torch.Tensor) or w.shape != shape:
         got = tuple(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__
         raise ValueError(f"{name} must be {shape}, got {got}")
@@ -77,7 +80,7 @@ def accumulate_attention_weights(q: torch.Tensor, k: torch.Tensor,
             torch.empty((B, Hkv, C), dtype=torch.float32, device=dev)
     else:
         _check_weights("out", out, (B, Hkv, C), dev)
-        if weights is not None and overlap(out, weights) and (
+        if weights is not None and weights is not out and overlap(out, weights) and (
                 out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride()):
             raise ValueError("out overlaps weights without being the same view")
     check_output("out", out)
@@ -100,7 +103,7 @@ def accumulate_attention_weights(q: torch.Tensor, k: torch.Tensor,
     dk = max(32, (D + 7) & ~7)
     hold: list = []
     args = _native.ATTN_WEIGHTS_ARGS.pack(
-        *rows_arg(q, dk, hold), *rows_arg(k, dk, hold), 0 if lse is None else lse.data_ptr(),
+        *rows_arg(q, dk - D, hold), *rows_arg(k, dk - D, hold), 0 if lse is None else lse.data_ptr(),
         0 if clen is None else clen.data_ptr(),
         *((weights.data_ptr(), *weights.stride()[:2]) if weights is not None else (0, 0, 0)),
         out.data_ptr(), *out.stride()[:2], B, Hq, Hkv, S_q, C, dk, code, 1 if causal else 0,

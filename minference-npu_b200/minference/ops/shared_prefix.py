@@ -103,11 +103,12 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
             res = q.new_empty((B, Hq, S_q, dk))
     lse = torch.empty((B, Hq, S_q), dtype=torch.float32, device=q.device) if return_lse else None
     hold: list = []
+    pad = dk - D
     args = _native.SHARED_PREFIX_ARGS.pack(
-        *rows_arg(q, dk, hold),
-        *(rows_arg(k_prefix, dk, hold) if P else _NONE),
-        *(rows_arg(v_prefix, dk, hold) if P else _NONE),
-        *(rows_arg(k, dk, hold) if C else _NONE), *(rows_arg(v, dk, hold) if C else _NONE),
+        *rows_arg(q, pad, hold),
+        *(rows_arg(k_prefix, pad, hold) if P else _NONE),
+        *(rows_arg(v_prefix, pad, hold) if P else _NONE),
+        *(rows_arg(k, pad, hold) if C else _NONE), *(rows_arg(v, pad, hold) if C else _NONE),
         res.data_ptr(), *res.stride()[:3], 0 if lse is None else lse.data_ptr(),
         plen.data_ptr() if plen is not None and P else 0,
         clen.data_ptr() if clen is not None and C else 0, B, Hq, Hkv, S_q, G, P, C, dk, code,

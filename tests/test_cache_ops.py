@@ -175,6 +175,10 @@ ATTENTION = [
     (4, 4, 2, 2, 2, 600, 0, 40, BF, "bhsd"),        # no own cache
     (1, 8, 8, 200, 1, 0, 333, 64, BF, "bhsd"),      # a chunk of a prompt
     (2, 16, 2, 64, 1, 1500, 64, 128, FP, "bhsd"),   # 512 rows a cache
+    (8, 32, 8, 9, 1, 0, 1500, 96, BF, "bshd"),      # several key blocks an item
+    (40, 8, 8, 1, 1, 5000, 30, 128, BF, "bhsd"),
+    (16, 16, 16, 40, 1, 0, 1200, 64, FP, "bhsd"),   # whole caches an item
+    (16, 16, 16, 33, 1, 700, 500, 128, BF, "bhsd"),
 ]
 
 
@@ -336,6 +340,8 @@ WEIGHTS = [
     (1, 3, 1, 300, 777, 64, FP, "bhsd"),
     (1, 2, 1, 9, 65, 33, BF, "bhsd"),
     (2, 2, 2, 129, 513, 72, FP, "bshd"),
+    (6, 32, 32, 12, 2000, 64, BF, "bhsd"),    # several key tiles an item
+    (1, 16, 16, 1500, 1500, 128, FP, "bhsd"),
 ]
 
 
