@@ -624,7 +624,9 @@ static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cud
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (err != cudaSuccess) cudaGetLastError();  // reported by the status alone
+  return err;
 }
 
 template <typename DT, int DK, RowsMode MODE>

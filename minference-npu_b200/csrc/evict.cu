@@ -209,9 +209,11 @@ __global__ void __launch_bounds__(kEvictThreads, 2)
     }
     int gt = 0, eq = 0;
     walk([&](int, uint32_t kk, bool valid) {
-      gt += __popc(__ballot_sync(0xffffffffu, valid && kk > prefix));
-      eq += __popc(__ballot_sync(0xffffffffu, valid && kk == prefix));
+      gt += valid && kk > prefix;
+      eq += valid && kk == prefix;
     });
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) cnt_gt[warp] = gt, cnt_eq[warp] = eq;
     __syncthreads();
     gt = eq = 0;
@@ -327,6 +329,7 @@ static int launch_evict(const EvictParams& p, int64_t BH, cudaStream_t st) {
   cudaError_t err = allow_smem<evict_kernel<CL, KPT, V>>(sizeof(EvictSmem));
   if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kern, p);
   if (err != cudaSuccess) {
+    cudaGetLastError();  // reported by the status alone
     debug_launch_failure("evict_kernel", reinterpret_cast<const void*>(kern), err, kEvictThreads,
                          0);
     return MI_ERR_LAUNCH;

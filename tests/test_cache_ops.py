@@ -179,6 +179,7 @@ ATTENTION = [
     (40, 8, 8, 1, 1, 5000, 30, 128, BF, "bhsd"),
     (16, 16, 16, 40, 1, 0, 1200, 64, FP, "bhsd"),   # whole caches an item
     (16, 16, 16, 33, 1, 700, 500, 128, BF, "bhsd"),
+    (6, 4, 2, 33, 2, 300, 80, 96, FP, "bhsd"),      # one walk over a shared prefix and own keys
 ]
 
 
