@@ -349,9 +349,6 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, MODE>::W,
       if (c == 0) p.ml[at] = make_float2(M, lt);
     }
   }
-  // The kernel that this call launched before may still run: end after it, so
-  // that what waits for this kernel waits for both.
-  pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -609,28 +606,8 @@ static bool rows_ok(const mi_rows& t, int64_t n0, int64_t n1, int64_t n2) {
   return true;
 }
 
-template <typename K, typename... A>
-static cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
-                                A... args) {
-  // Programmatic launch: the kernel may be set up while the one before it
-  // drains; it waits (griddepcontrol.wait) before it reads its results.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...);
-  if (err != cudaSuccess) cudaGetLastError();  // reported by the status alone
-  return err;
-}
-
 template <typename DT, int DK, RowsMode MODE>
-static int launch_rows(const CacheParams& p, long long items, bool after, cudaStream_t stream) {
+static int launch_rows(const CacheParams& p, long long items, cudaStream_t stream) {
   using L = RowsSmem<DK, MODE>;
   constexpr int kRowsWarps = L::W;
   constexpr auto kern = cache_rows_kernel<DT, DK, MODE>;
@@ -638,12 +615,8 @@ static int launch_rows(const CacheParams& p, long long items, bool after, cudaSt
   constexpr int bytes = L::kRing > kJoin ? L::kRing : kJoin;
   cudaError_t err = allow_smem<cache_rows_kernel<DT, DK, MODE>>(bytes);
   if (err == cudaSuccess) {
-    if (after) {
-      err = launch_after(kern, dim3((unsigned)items), 32 * kRowsWarps, bytes, stream, p);
-    } else {
-      kern<<<(unsigned)items, 32 * kRowsWarps, bytes, stream>>>(p);
-      err = cudaGetLastError();
-    }
+    kern<<<(unsigned)items, 32 * kRowsWarps, bytes, stream>>>(p);
+    err = cudaGetLastError();
   }
   if (err != cudaSuccess) {
     debug_launch_failure("cache_rows_kernel", reinterpret_cast<const void*>(kern), err,
@@ -654,17 +627,16 @@ static int launch_rows(const CacheParams& p, long long items, bool after, cudaSt
 }
 
 template <RowsMode MODE>
-static int launch_rows_dk(const CacheParams& p, int dtype, long long items, bool after,
-                          cudaStream_t st) {
+static int launch_rows_dk(const CacheParams& p, int dtype, long long items, cudaStream_t st) {
   const bool bf = dtype == MI_BF16;
   if (p.D <= 64)
-    return bf ? launch_rows<__nv_bfloat16, 64, MODE>(p, items, after, st)
-              : launch_rows<__half, 64, MODE>(p, items, after, st);
+    return bf ? launch_rows<__nv_bfloat16, 64, MODE>(p, items, st)
+              : launch_rows<__half, 64, MODE>(p, items, st);
   if (p.D <= 96)
-    return bf ? launch_rows<__nv_bfloat16, 96, MODE>(p, items, after, st)
-              : launch_rows<__half, 96, MODE>(p, items, after, st);
-  return bf ? launch_rows<__nv_bfloat16, 128, MODE>(p, items, after, st)
-            : launch_rows<__half, 128, MODE>(p, items, after, st);
+    return bf ? launch_rows<__nv_bfloat16, 96, MODE>(p, items, st)
+              : launch_rows<__half, 96, MODE>(p, items, st);
+  return bf ? launch_rows<__nv_bfloat16, 128, MODE>(p, items, st)
+            : launch_rows<__half, 128, MODE>(p, items, st);
 }
 
 static void set_seg(CacheSeg& s, const mi_rows& k, const mi_rows& v, const int32_t* len,
@@ -775,16 +747,19 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
     g.slot0 = p.seg[s].slot0;
     g.items = (int)items[s];
   }
-  const bool tiles = pl.tile[0] || pl.tile[1];
-  if (tiles) {
-    tp.c = p;
-    const int rc = launch_tiles(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, st);
-    if (rc != MI_OK) return rc;
-  }
+  // The own caches' kernel first: the prefix's tiles start as its blocks end
+  // (the other way round the last tiles end alone: 35 us against 32 for 32
+  // sequences of 512 keys over 8192).
   const long long few = (pl.tile[0] ? 0 : items[0]) + (pl.tile[1] ? 0 : items[1]);
   if (few) {
     p.items0 = pl.tile[0] ? 0 : (int)items[0];
-    const int rc = launch_rows_dk<kAttention>(p, a.dtype, few, tiles, st);
+    const int rc = launch_rows_dk<kAttention>(p, a.dtype, few, st);
+    if (rc != MI_OK) return rc;
+  }
+  if (pl.tile[0] || pl.tile[1]) {
+    tp.c = p;
+    const int rc =
+        launch_tiles(tp, a.dtype, a.k_prefix, a.v_prefix, a.k, a.v, few > 0, st);
     if (rc != MI_OK) return rc;
   }
   if (p.NS == 1) return MI_OK;

@@ -457,11 +457,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
   }
+  // The own caches' kernel of the same call may still run: end after it, so that
+  // what waits for this kernel waits for both.
+  pdl_wait();
 }
 
 template <typename DT, int DK>
 static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows& vp,
-                          const mi_rows& k, const mi_rows& v, cudaStream_t st) {
+                          const mi_rows& k, const mi_rows& v, bool after,
+                          cudaStream_t st) {
   using L = TileSmem<DK>;
   const CacheParams& p = tp.c;
   CUtensorMap m[4];
@@ -478,9 +482,13 @@ static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows
   constexpr auto kern = cache_tiles_kernel<DT, DK>;
   cudaError_t err = allow_smem<cache_tiles_kernel<DT, DK>>(L::kAlloc);
   if (err == cudaSuccess) {
-    kern<<<(unsigned)(tp.grp[0].items + tp.grp[1].items), kTileThreads, L::kAlloc, st>>>(
-        m[0], m[1], m[2], m[3], tp);
-    err = cudaGetLastError();
+    const dim3 grid((unsigned)(tp.grp[0].items + tp.grp[1].items));
+    if (after) {
+      err = launch_after(kern, grid, kTileThreads, L::kAlloc, st, m[0], m[1], m[2], m[3], tp);
+    } else {
+      kern<<<grid, kTileThreads, L::kAlloc, st>>>(m[0], m[1], m[2], m[3], tp);
+      err = cudaGetLastError();
+    }
   }
   if (err != cudaSuccess) {
     debug_launch_failure("cache_tiles_kernel", reinterpret_cast<const void*>(kern), err,
@@ -491,17 +499,18 @@ static int launch_tiles_t(const TileParams& tp, const mi_rows& kp, const mi_rows
 }
 
 static int launch_tiles(const TileParams& tp, int dtype, const mi_rows& kp, const mi_rows& vp,
-                        const mi_rows& k, const mi_rows& v, cudaStream_t st) {
+                        const mi_rows& k, const mi_rows& v, bool after,
+                        cudaStream_t st) {
   const bool bf = dtype == MI_BF16;
   const int D = tp.c.D;
   if (D <= 64)
-    return bf ? launch_tiles_t<__nv_bfloat16, 64>(tp, kp, vp, k, v, st)
-              : launch_tiles_t<__half, 64>(tp, kp, vp, k, v, st);
+    return bf ? launch_tiles_t<__nv_bfloat16, 64>(tp, kp, vp, k, v, after, st)
+              : launch_tiles_t<__half, 64>(tp, kp, vp, k, v, after, st);
   if (D <= 96)
-    return bf ? launch_tiles_t<__nv_bfloat16, 96>(tp, kp, vp, k, v, st)
-              : launch_tiles_t<__half, 96>(tp, kp, vp, k, v, st);
-  return bf ? launch_tiles_t<__nv_bfloat16, 128>(tp, kp, vp, k, v, st)
-            : launch_tiles_t<__half, 128>(tp, kp, vp, k, v, st);
+    return bf ? launch_tiles_t<__nv_bfloat16, 96>(tp, kp, vp, k, v, after, st)
+              : launch_tiles_t<__half, 96>(tp, kp, vp, k, v, after, st);
+  return bf ? launch_tiles_t<__nv_bfloat16, 128>(tp, kp, vp, k, v, after, st)
+            : launch_tiles_t<__half, 128>(tp, kp, vp, k, v, after, st);
 }
 
 }  // namespace mib200

@@ -826,7 +826,7 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   if (items > 0x7fffffffll) return MI_ERR_SHAPE;
   if (!lse) {
     p.ml = ml;
-    rc = launch_rows_dk<kStats>(p, dtype, items, false, st);
+    rc = launch_rows_dk<kStats>(p, dtype, items, st);
     if (rc != MI_OK) return rc;
     weight_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(ml, pl.NS, lse2,
                                                                       (long long)rows);
@@ -842,5 +842,5 @@ extern "C" int mi_attn_weights(const mi_attn_weights_args* args, void* workspace
   p.wout = w.wout;
   p.wo_b = w.wo_b;
   p.wo_h = w.wo_h;
-  return launch_rows_dk<kWeights>(p, dtype, items, false, st);
+  return launch_rows_dk<kWeights>(p, dtype, items, st);
 }

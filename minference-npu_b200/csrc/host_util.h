@@ -120,6 +120,28 @@ inline cudaError_t allow_smem(int bytes) {
   return err;
 }
 
+// Programmatic launch: the kernel may be set up and start while the one before
+// it drains; it waits (griddepcontrol.wait) before it reads that one's results.
+// Only behind a kernel of the same call, whose own launch has waited for
+// whatever wrote the inputs.
+template <typename K, typename... A>
+inline cudaError_t launch_after(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (err != cudaSuccess) cudaGetLastError();  // reported by the status alone
+  return err;
+}
+
 // 4-D map of a [B, H, S, D] tensor given by its rows (see make_bnsd_map).
 inline int make_rows4_map(CUtensorMap* map, const mi_rows& r, int64_t B, int64_t H, int64_t S,
                           int64_t D, int box_d, int box_s) {
