@@ -9,11 +9,11 @@
 namespace mib200 {
 
 // ---------------------------------------------------------------------------
-// Few rows (1 to 8 per key/value head): a work item is those rows against
-// `chunk` keys.  Its warps take groups of 16 keys in turn; each
-// warp streams its own groups through its own shared-memory ring (cp.async)
-// and keeps its own running maximum, sum and O, so there is no barrier in the
-// loop.  Their states are joined at the end.  Keys are the M side of both
+// Few rows: a work item is a tile of up to 8 rows against `chunk` keys.  Its
+// warps take groups of 16 keys in turn; each warp streams its own groups
+// through its own shared-memory ring (cp.async) and keeps its own running
+// maximum, sum and O, so there is no barrier in the loop.  Their states are
+// joined at the end.  Bound by the cache's bytes.  Keys are the M side of both
 // products, so that a single row costs an 8-wide tile, not a 16-wide one:
 //   S^T (16 keys x 8 rows) = K Q^T     Q fragments stay in registers
 //   O^T (D x 8 rows) += V^T P^T        P^T is S^T's registers rounded to the
@@ -22,9 +22,14 @@ namespace mib200 {
 // of 128, 192 and 256 bytes fall into distinct banks.  Keys past the end of
 // the range are filled with zeros instead of being read, so whatever a cache
 // holds past its length cannot reach O through 0 * V.
+// Measured: two caches of 65536 and 49152 keys, 32 heads of 96, 219 us
+// (6.4 TB/s); 201 MB of 1024-key caches 39 us.  With the rows as the M side and
+// two blocks of 100 KB an SM the first took 257 us.
 //
 // kStats: the rows' (maximum, sum) only; no V.
-// kWeights: given the rows' lse, a key's weight summed over the rows and added to win; no V.
+// kWeights: given the lse of all the head's rows (one tile), a key's weight is
+// summed over them and added to win; no V.  16 caches of 8192 keys, 8 heads of
+// 128: 40 us (5.1 TB/s).
 // ---------------------------------------------------------------------------
 enum RowsMode { kAttention, kStats, kWeights };
 
@@ -672,15 +677,21 @@ static void set_heads(CacheParams& p, int64_t Hq, int64_t Hkv, int64_t Sq, int64
 
 using namespace mib200;
 
+namespace mib200 {
+// Workspace of a call with plan `pl`; SIZE_MAX past any memory.
+static size_t shared_prefix_need(const mi_shared_prefix_args& a, const CachePlan& pl) {
+  if (pl.NS == 1) return 0;
+  if ((double)a.B * a.Hq * a.S_q * pl.NS * (a.D * 4 + 8) > 1e15) return SIZE_MAX;
+  const size_t slots = (size_t)(a.B * a.Hq * a.S_q) * pl.NS;
+  return align_up(slots * a.D * 4) + align_up(slots * 8);
+}
+}  // namespace mib200
+
 extern "C" size_t mi_shared_prefix_fwd_workspace_size(const mi_shared_prefix_args* a) {
   if (!a || !cache_sizes_ok(a->B, a->Hq, a->Hkv, a->S_q, a->G, a->P, a->C, a->D)) return SIZE_MAX;
   if (a->B == 0 || a->Hq == 0 || a->S_q == 0) return 0;
-  const CachePlan pl = cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C, a->D);
-  if (pl.NS == 1) return 0;
-  const double need = (double)a->B * a->Hq * a->S_q * pl.NS * (a->D * 4 + 8);
-  if (need > 1e15) return SIZE_MAX;
-  const size_t slots = (size_t)(a->B * a->Hq * a->S_q) * pl.NS;
-  return align_up(slots * a->D * 4) + align_up(slots * 8);
+  return shared_prefix_need(
+      *a, cache_plan(a->B, a->Hkv, a->Hq / a->Hkv, a->S_q, a->G, a->P, a->C, a->D));
 }
 
 extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* workspace,
@@ -697,7 +708,7 @@ extern "C" int mi_shared_prefix_fwd(const mi_shared_prefix_args* args, void* wor
   if (C && (!rows_ok(a.k, B, Hkv, C) || !rows_ok(a.v, B, Hkv, C))) return MI_ERR_ALIGN;
   const int64_t group = Hq / Hkv;
   const CachePlan pl = cache_plan(B, Hkv, group, S_q, G, P, C, D);
-  const size_t need = mi_shared_prefix_fwd_workspace_size(args);
+  const size_t need = shared_prefix_need(a, pl);
   if (need == SIZE_MAX) return MI_ERR_SHAPE;
   if (need && (!workspace || workspace_bytes < need ||
                (reinterpret_cast<uintptr_t>(workspace) & 15)))

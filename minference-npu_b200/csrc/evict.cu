@@ -40,14 +40,17 @@ __device__ __forceinline__ uint32_t evict_key(float w, int j, int n, int sink, i
 // shared memory one warp of each block then adds up the cluster's sums of 32
 // digits, finds the group, adds up that group's digits, and all blocks find the
 // same digit (3 KB read a block and pass; adding up all 2048 counts took 3 us a
-// pass).  With T the k-th key and e of the keys equal to it to be
-// kept, a kept key's place is the number of keys above T before it plus the
-// smaller of e and the number of keys equal to T before it.
+// pass).  With T the k-th key and e of the keys equal to it to be kept, a kept
+// key's place is the number of keys above T before it plus the smaller of e and
+// the number of keys equal to T before it.  Bound by the barriers' latency.
 //
 // Move: the kept rows are shared out evenly over the cluster, whichever block
 // found them, in 16-byte pieces (V; single elements for rows without that
 // alignment); bound by their bytes.
 //
+// Measured: 32 heads of 65536 rows of 96 to 8192: 52 us, of which the search 19;
+// 256 heads of up to 4097 rows of 128 to 2048: 93 us (5.7 TB/s).  As a search
+// kernel over a cluster and a move kernel they took 81 and 107.
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kMoveRows = 512;
