@@ -644,6 +644,41 @@ def test_steps_captured_in_graphs_follow_lengths(cuda):
             check_evicted(e, k, v, w, 32, lens.tolist(), 2, 4)
 
 
+_FIRST_CALL = """
+import sys
+sys.path[:0] = [{root!r}, {root!r} + "/minference-npu_b200", {root!r} + "/tests"]
+import torch
+from minference import ops
+import test_cache_ops as t
+c = (4, 8, 2, 1, 1, 900, 200, 128, t.BF, "bhsd")
+q, kp, vp, k, v = t.make(c, 40)
+k2, q2 = k[:, :, :100].contiguous(), q.expand(-1, -1, 70, -1).contiguous()
+w = torch.rand(4, 2, 200, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    o = ops.shared_prefix_attention(q, kp, vp, k, v)
+    x = ops.accumulate_attention_weights(q2, k2)
+    e = ops.evict_cache(k, v, w, 50)
+g.replay()
+torch.cuda.synchronize()
+ref, tol, _, _ = t.ref_attention(q, kp, vp, k, v)
+assert ((o.double() - ref).abs() <= tol).all()
+ref, tol = t.ref_weights(q2, k2, None)
+assert ((x.double() - ref).abs() <= tol).all()
+t.check_evicted(e, k, v, w, 50, None, 0, 0)
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_can_be_captured(cuda):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", _FIRST_CALL.format(root=root)], check=True, timeout=240)
+
+
 @pytest.mark.gpu
 def test_streams_and_repeated_calls_agree(cuda):
     """Calls on side streams at once, each equal to the call alone, bit for bit."""
