@@ -77,7 +77,9 @@ __device__ __forceinline__ void bulk_wait0() {
 }
 
 constexpr int kTileThreads = 192;
-constexpr float kTileSum = 32768.0f;  // sum of a block's P from which its row's reference moves
+// Sum of a block's P from which its row's reference moves; its logarithm, for
+// a block's maximum over the reference.
+constexpr float kTileSum = 32768.0f, kTileRise = 15.0f;
 
 template <typename DT, int DK>
 __global__ void __launch_bounds__(kTileThreads, 2)
@@ -348,15 +350,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       };
       // P against the row's reference straight away, without looking for its
       // maximum: a sum below 2^15 says that every P is (fp16 holds it).  Only
-      // if some row passes that (or has seen nothing yet) does the warp look,
-      // move the references, rescale O and compute P again.
+      // if some row passes that does the warp look, move the references,
+      // rescale O and compute P again.  While some row of the warp has no
+      // reference (it has seen nothing yet, or never will), there are no sums
+      // to go by: the warp looks, and every row's maximum is held to 2^15.
       const bool spec = !empty && all(m != -INFINITY);
-      float sum = 0.f, mn = m;
+      float sum = INFINITY, mn = m;
       if (spec) sum = exp_block(-m);
-      bool need = !empty && !(m != -INFINITY && sum < kTileSum);
-      if (!empty && __any_sync(0xffffffffu, need)) {
+      bool need = !empty && !(sum < kTileSum);
+      if (__any_sync(0xffffffffu, need)) {
         mn = fmaxf(m, row_max() * sc);
-        need = need && mn > m;
+        need = mn > m && (spec ? need : m == -INFINITY || mn - m >= kTileRise);
       }
       bool again = !spec;
       if (__any_sync(0xffffffffu, need)) {

@@ -268,6 +268,63 @@ def test_attention_rising_scores(cuda, Sq, dtype):
     assert ((out.double() - ref).abs() <= tol).all()
 
 
+def blocks_an_item(q, kp, k):
+    """64-key blocks that a tile walks in one item, at least: from the partial
+    results a row has (0 bytes: one), where one kind of item covers the call."""
+    from minference import _native
+
+    B, Hq, Sq, D = q.shape
+    Hkv, C = k.shape[1:3]
+    G, P = (kp.shape[0], kp.shape[2]) if kp is not None else (1, 0)
+    none = (0, 0, 0, 0)
+    need = _native.lib().mi_shared_prefix_fwd_workspace_size(_native.SHARED_PREFIX_ARGS.pack(
+        *none * 6, 0, 0, 0, B, Hq, Hkv, Sq, G, P, C, D, 1, 1, 1.0))
+    slots = max(1, round(need / (B * Hq * Sq * (4 * D + 8))))
+    return (-(-P // 64) + -(-C // 64)) / slots
+
+
+#   B  Hq  Hkv Sq   P    C     D   lengths / prefix lengths
+MIXED = [
+    (4, 32, 8, 100, 0, 1500, 128, [860, 1500, 99, 70], None),  # rows wrap into the next head
+    (1, 4, 2, 1000, 0, 1000, 64, None, None),         # ranges that start among the new tokens
+    (2, 4, 2, 200, 0, 300, 96, [150, 300], None),     # fewer keys than new tokens
+    (16, 16, 8, 100, 256, 600, 128, [600, 90, 80, 555] * 4, [256, 0]),  # one walk over both
+    (16, 16, 16, 40, 0, 1200, 64, None, None),        # every row of a warp sees something
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rise", [3, 13, 100])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("case", MIXED, ids=ids)
+def test_attention_rising_scores_beside_rows_that_see_nothing(cuda, case, dtype, rise):
+    """Scores rise by `rise` from each 64-key block to the next: a row's reference
+    has to move from one block of an item to a later one, also while other rows
+    of its warp have none yet."""
+    from minference import ops
+
+    B, Hq, Hkv, Sq, P, C, D, lens, plens = case
+    G = 2 if P else 1
+    q, kp, vp, k, v = make((B, Hq, Hkv, Sq, G, P, C, D, dtype, "bhsd"), 33)
+    assert blocks_an_item(q, kp, k) > 1
+    q = (0.25 * q).contiguous()
+    q[..., 0] = 4
+    step = torch.arange((P + C + 63) // 64, device="cuda").repeat_interleave(64)
+    step = (step * (rise * D**0.5 / 4)).to(dtype)
+    k[..., 0] = step[P:P + C]
+    if P:
+        kp[..., 0] = step[:P]
+    cu = [None if x is None else torch.tensor(x, dtype=torch.int32).cuda() for x in (lens, plens)]
+    out, lse = ops.shared_prefix_attention(q, kp, vp, k, v, cu[0], prefix_lengths=cu[1],
+                                           return_lse=True)
+    ref, tol, rl, lt = ref_attention(q, kp, vp, k, v, lens, plens)
+    assert torch.equal(lse.isinf(), rl.isinf())
+    seen = ~rl.isinf()
+    assert ((lse.double() - rl).abs() <= lt)[seen].all()
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert (out[~seen] == 0).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [96, 40, 33])
 def test_attention_writes_the_given_view_only(cuda, D):
