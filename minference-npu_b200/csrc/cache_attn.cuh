@@ -112,13 +112,35 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe, for x < 128 (below -126: about 1e-38).
-// x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low
-// bits), 2^f by a polynomial of degree 5, the minimax one for the relative
-// error over [-1/2, 1/2] found by Remez exchange (7.5e-8), n into the exponent.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+
+// The larger / smaller of two values, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe, for x up to 128 (0 below -126.5, infinity
+// from 127.5, NaN for NaN).  x = n + f with n the nearest integer (adding
+// 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial of degree 5, the
+// minimax one for the relative error over [-1/2, 1/2] found by Remez exchange
+// (7.5e-8; 1.5e-7 with its coefficients in fp32, 2.1e-7 computed in fp32), times
+// 2^n put together from its bits: n = -127 gives 0 and n = 128 infinity.
 __device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
   const float2 t = add2(x, make_float2(12582912.f, 12582912.f));
   const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
   const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
@@ -128,9 +150,8 @@ __device__ __forceinline__ float2 poly_exp2(float2 x) {
   r = fma2(r, f, make_float2(2.4022120e-1f, 2.4022120e-1f));
   r = fma2(r, f, make_float2(6.9314697e-1f, 6.9314697e-1f));
   r = fma2(r, f, make_float2(1.0000001f, 1.0000001f));
-  r.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
-  r.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
-  return r;
+  return mul2(r, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                             __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 
 }  // namespace mib200

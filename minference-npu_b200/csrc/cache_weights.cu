@@ -55,8 +55,8 @@ constexpr int kPolyEvery = 4;
 constexpr int kScanThreads = 320;
 
 // acc += sum over 32 columns of 2^(s * sc + z[c]); z per column in shared memory.
-// The exponents are at most about 0 (z is minus a log-sum-exp); an lse that is
-// no row's could bring one past 128, where only the MUFU's form overflows.
+// The exponents are at most about 0 (z is minus a log-sum-exp; -inf adds 0); an
+// lse that is no row's could bring one past 128, the polynomial's range.
 __device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, const float* z,
                                              float2& a0, float2& a1) {
   const float2 sc2 = make_float2(sc, sc);
@@ -66,7 +66,7 @@ __device__ __forceinline__ void exp_sum_cols(const float (&s)[32], float sc, con
     const float2 x0 = fma2(make_float2(s[c], s[c + 1]), sc2, make_float2(zz.x, zz.y));
     const float2 x1 = fma2(make_float2(s[c + 2], s[c + 3]), sc2, make_float2(zz.z, zz.w));
     a0 = add2(a0, (c / 2) % kPolyEvery == 0
-                      ? poly_exp2(make_float2(fminf(x0.x, 127.f), fminf(x0.y, 127.f)))
+                      ? poly_exp2(make_float2(min_nan(x0.x, 128.f), min_nan(x0.y, 128.f)))
                       : make_float2(fast_exp2(x0.x), fast_exp2(x0.y)));
     a1 = add2(a1, make_float2(fast_exp2(x1.x), fast_exp2(x1.y)));
   }

@@ -479,6 +479,48 @@ def test_weights_rising_scores(cuda, Sq):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 5, 20, 33, 40, 70, 300])
+def test_weights_of_nothing_are_exactly_zero(cuda, Sq):
+    """Rows whose lse is -inf add nothing, and probabilities far below fp32's range
+    are 0, whatever path a key takes: eviction's ties among zeros depend on it."""
+    from minference import ops
+
+    q, _, _, k, _ = make((2, 4, 2, Sq, 1, 0, 900, 96, BF, "bhsd"), 34)
+    none = torch.full((2, 4, Sq), -math.inf, device="cuda")
+    for causal in (False, True):
+        assert (ops.accumulate_attention_weights(q, k, lse=none, causal=causal) == 0).all()
+    some = ref_attention(q, None, None, k, k, causal=False)[2].float()
+    some[:, :, ::2] = -math.inf
+    w = ops.accumulate_attention_weights(q, k, lse=some, causal=False)
+    ref, tol = ref_weights(q, k, None, lse=some, causal=False)
+    assert ((w.double() - ref).abs() <= tol).all()
+    q = (0.25 * q).contiguous()
+    q[..., 0] = 4
+    far = torch.zeros(900, dtype=torch.bool, device="cuda")
+    far[100:700] = True
+    k[..., 0] = torch.where(far, -1000.0, 0.0).to(BF)  # 400 below the others
+    lse = ref_attention(q, None, None, k, k, causal=False)[2].float()
+    for z in (None, lse):
+        w = ops.accumulate_attention_weights(q, k, lse=z, causal=False)
+        assert (w[..., far] == 0).all() and (w[..., ~far] > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [5, 20, 40, 300])
+def test_weights_of_an_lse_far_too_small_overflow(cuda, Sq):
+    """A sum of exponentials past fp32's range is infinite, in every column."""
+    from minference import ops
+
+    q, _, _, k, _ = make((1, 2, 2, Sq, 1, 0, 300, 64, BF, "bhsd"), 35)
+    lse = torch.full((1, 2, Sq), -500.0, device="cuda")
+    assert (ops.accumulate_attention_weights(q, k, lse=lse, causal=False) == math.inf).all()
+    for at in range(8):  # one such row among rows that add nothing
+        lse = torch.full((1, 2, Sq), -math.inf, device="cuda")
+        lse[:, :, at % Sq] = -500.0
+        assert (ops.accumulate_attention_weights(q, k, lse=lse, causal=False) == math.inf).all()
+
+
+@pytest.mark.gpu
 def test_weights_of_an_attention_with_prefix(cuda):
     """lse of the attention: own weights plus the prefix's add up to the rows."""
     from minference import ops
