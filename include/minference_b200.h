@@ -257,7 +257,8 @@ typedef struct mi_rows {
  * float [B, Hq, S_q], the natural logarithm of the sum of exp(scale q.k).
  * D is a multiple of 8 from 32 to 128; P or C may be 0 (the rows are then not
  * read), P + C at most 2^30.  What a cache holds past its length does not
- * reach the result; values within it must be finite.  The workspace (16-byte aligned) may be reused once the
+ * reach the result; values within it must be finite.  A row of q that holds a
+ * NaN gives NaN.  The workspace (16-byte aligned) may be reused once the
  * call's work has finished; its size is SIZE_MAX for sizes the call refuses. */
 typedef struct mi_shared_prefix_args {
   mi_rows q, k_prefix, v_prefix, k, v, out;

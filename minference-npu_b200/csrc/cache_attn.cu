@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(32 * RowsSmem<DK, MODE>::W,
         acc.w += f * x.w;
       }
     }
+    if (lt != lt) M = 0.f;  // NaN scores, perhaps none else: -inf means nothing seen
     int b, hd, tk;
     cache_row(p, sg, e, h, r0 + r, b, hd, tk);
     const long long row = ((long long)b * p.Hq + hd) * p.Sq + tk;

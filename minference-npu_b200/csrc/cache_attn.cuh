@@ -132,6 +132,20 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A row's reference m after scores whose maximum is t.  A NaN among them
+// (t is NaN) leaves it finite: the row's sums carry the NaN, and -inf keeps
+// meaning that nothing has been seen.
+__device__ __forceinline__ float next_ref(float m, float t) {
+  if (t != t) return m == -INFINITY ? 0.f : m;
+  return fmaxf(m, t);
+}
+
 // 2^x of two values on the FMA pipe, for x up to 128 (0 below -126.5, infinity
 // from 127.5, NaN for NaN).  x = n + f with n the nearest integer (adding
 // 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial of degree 5, the

@@ -323,16 +323,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
       }
       auto row_max = [&]() -> float {
-        float a = fmax3(s[0], s[1], s[2]), b = fmax3(s[3], s[4], s[5]);
-        float c = fmax3(s[6], s[7], s[8]), d = fmax3(s[9], s[10], s[11]);
+        float a = max3_nan(s[0], s[1], s[2]), b = max3_nan(s[3], s[4], s[5]);
+        float c = max3_nan(s[6], s[7], s[8]), d = max3_nan(s[9], s[10], s[11]);
 #pragma unroll
         for (int x = 12; x < 60; x += 8) {
-          a = fmax3(a, s[x], s[x + 1]);
-          b = fmax3(b, s[x + 2], s[x + 3]);
-          c = fmax3(c, s[x + 4], s[x + 5]);
-          d = fmax3(d, s[x + 6], s[x + 7]);
+          a = max3_nan(a, s[x], s[x + 1]);
+          b = max3_nan(b, s[x + 2], s[x + 3]);
+          c = max3_nan(c, s[x + 4], s[x + 5]);
+          d = max3_nan(d, s[x + 6], s[x + 7]);
         }
-        return fmaxf(fmax3(a, b, fmax3(s[60], s[61], s[62])), fmax3(c, d, s[63]));
+        return max_nan(max3_nan(a, b, max3_nan(s[60], s[61], s[62])), max3_nan(c, d, s[63]));
       };
       auto exp_block = [&](float nm) -> float {
         float2 t0 = make_float2(0.f, 0.f), t1 = t0;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       if (spec) sum = exp_block(-m);
       bool need = !empty && !(sum < kTileSum);
       if (__any_sync(0xffffffffu, need)) {
-        mn = fmaxf(m, row_max() * sc);
+        mn = next_ref(m, row_max() * sc);
         need = mn > m && (spec ? need : m == -INFINITY || mn - m >= kTileRise);
       }
       bool again = !spec;

@@ -299,10 +299,10 @@ __global__ void __launch_bounds__(kScanThreads, 2)
         if (__any_sync(0xffffffffu, bad)) {
           float t = s[0];
 #pragma unroll
-          for (int c = 1; c < 31; c += 2) t = fmax3(t, s[c], s[c + 1]);
-          t = fmaxf(t, s[31]) * sc;
+          for (int c = 1; c < 31; c += 2) t = max3_nan(t, s[c], s[c + 1]);
+          t = max_nan(t, s[31]) * sc;
           if (bad) {
-            const float mn = fmaxf(m, t);
+            const float mn = next_ref(m, t);
             if (m != -INFINITY) l *= fast_exp2(m - mn);
             m = mn;
           }

@@ -42,7 +42,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor | None,
     every valid own key.  Lengths are integer device tensors (None: whole),
     clamped to the capacity; rows past them are never used, whatever they hold.
     Values within a length must be finite (one that a token does not see is
-    still multiplied by 0).  A token that sees nothing gives 0.
+    still multiplied by 0).  A token that sees nothing gives 0; one whose query
+    holds a NaN gives NaN, in the log-sum-exp too.
 
     ``scale`` defaults to ``1/sqrt(D)``.  Returns the output, of q's dtype, or
     with ``return_lse`` the pair (output, lse float32 ``[B,Hq,S_q]``: natural

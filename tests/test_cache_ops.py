@@ -537,6 +537,39 @@ def test_weights_of_an_attention_with_prefix(cuda):
         assert torch.allclose(total, torch.full_like(total, 8 * Sq), rtol=1e-4)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("Sq, P, C", [(1, 0, 700), (1, 900, 50), (3, 40, 0), (4, 0, 4000),
+                                      (40, 0, 900), (70, 700, 100), (130, 0, 333)])
+def test_nan_queries_come_out_as_nan(cuda, Sq, P, C, dtype):
+    """A NaN in a query is no row that sees nothing: its output and log-sum-exp are
+    NaN, the keys it sees get NaN weights, and no other row or head changes."""
+    from minference import ops
+
+    q, kp, vp, k, v = make((3, 4, 2, Sq, 1, P, C, 128, dtype, "bhsd"), 36)
+    lens = [C, C // 2, 0]
+    lt = torch.tensor(lens, dtype=torch.int32).cuda() if C else None
+    bad = torch.zeros(3, 4, Sq, dtype=torch.bool, device="cuda")
+    bad[0, 1, Sq // 2] = bad[1, 0, Sq - 1] = bad[2, 0, 0] = True
+    q2 = torch.where(bad[..., None] & (torch.arange(128, device="cuda") == 5), float("nan"), q)
+    o, z = ops.shared_prefix_attention(q, kp, vp, k, v, lt, return_lse=True)
+    o2, z2 = ops.shared_prefix_attention(q2, kp, vp, k, v, lt, return_lse=True)
+    nan = bad & ~z.isinf()
+    assert nan.any()
+    assert o2[nan].isnan().all() and z2[nan].isnan().all()
+    assert torch.equal(o2[~nan], o[~nan]) and torch.equal(z2[~nan], z[~nan])
+    if not C:
+        return
+    seen = torch.zeros(3, 2, C, dtype=torch.bool, device="cuda")
+    for b, h, r in bad.nonzero().tolist():
+        seen[b, h // 2, :max(0, lens[b] - (Sq - 1 - r))] = True
+    for lse, lse2 in ((None, None), (z, z2)):
+        w = ops.accumulate_attention_weights(q, k, None, lt, lse=lse)
+        w2 = ops.accumulate_attention_weights(q2, k, None, lt, lse=lse2)
+        assert torch.equal(w2.isnan(), seen)
+        assert torch.equal(w2[~seen], w[~seen])
+
+
 # ---------------------------------------------------------------------------
 # Eviction
 # ---------------------------------------------------------------------------
