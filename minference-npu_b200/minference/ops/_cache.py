@@ -48,7 +48,8 @@ def lengths_arg(name: str, x, n: int, cap: int, device: torch.device):
     if x.shape != (n,):
         raise ValueError(f"{name} must be ({n},), got {tuple(x.shape)}")
     if x.dtype is not torch.int32:
-        x = x.clamp(0, cap).to(torch.int32)
+        # in 64 bits: a narrow type need not hold the capacity
+        x = x.to(torch.int64).clamp(0, cap).to(torch.int32)
     if x.get_device() != device.index:
         x = x.to(device)
     return x if x.is_contiguous() else x.contiguous()

@@ -936,6 +936,39 @@ def test_attention_refuses_types_and_overlaps(no_device_check):
         f(q, None, None, c, t(2, 2, 8, 64), out=c.view(2, 4, 4, 64)[:, :, :1])
 
 
+@pytest.mark.parametrize("cap", [100, 200, 40000, 1 << 20])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64,
+                                   torch.uint16, torch.uint32])
+def test_lengths_of_every_integer_type(dtype, cap):
+    """Types that cannot hold the capacity too: their values are clamped as numbers."""
+    from minference.ops._cache import lengths_arg
+
+    values = [0, 1, 99, 127]
+    if dtype not in (torch.uint8, torch.uint16, torch.uint32):
+        values += [-5, -128]
+    if dtype is torch.int64:
+        values += [1 << 40, -(1 << 40)]
+    got = lengths_arg("lengths", torch.tensor(values, dtype=dtype), len(values), cap,
+                      torch.device("cpu"))
+    assert got.dtype == torch.int32
+    assert got.clamp(0, cap).tolist() == [min(max(x, 0), cap) for x in values]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16])
+def test_narrow_lengths_of_a_long_cache(cuda, dtype):
+    from minference import ops
+
+    q, _, _, k, v = make((2, 2, 2, 1, 1, 0, 40000, 64, BF, "bhsd"), 37)
+    lt, l32 = (torch.tensor([200, 7], dtype=x).cuda() for x in (dtype, torch.int32))
+    assert torch.equal(ops.shared_prefix_attention(q, None, None, k, v, lt),
+                       ops.shared_prefix_attention(q, None, None, k, v, l32))
+    w = ops.accumulate_attention_weights(q, k, None, lt)
+    assert torch.equal(w, ops.accumulate_attention_weights(q, k, None, l32))
+    assert torch.equal(ops.evict_cache(k, v, w, 50, lt).index,
+                       ops.evict_cache(k, v, w, 50, l32).index)
+
+
 def test_weights_refuse(no_device_check):
     from minference import ops
 
