@@ -85,8 +85,23 @@ def span(x: torch.Tensor) -> tuple[int, int]:
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two views may share an element (views that interleave do not)."""
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    return a0 < b1 and b0 < a1 and not _interleaved(a, b)
+
+
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Some stride tells the views apart: modulo it, each covers one stretch of
+    addresses (what its dimensions of other strides reach), clear of the other's."""
+    dims = [[(n, s * x.element_size()) for n, s in zip(x.shape, x.stride()) if n > 1]
+            for x in (a, b)]
+    for step in {s for d in dims for _, s in d if s > 0}:
+        na, nb = (sum((n - 1) * s for n, s in d if s % step) + x.element_size()
+                  for d, x in zip(dims, (a, b)))
+        gap = (b.data_ptr() - a.data_ptr()) % step
+        if na <= gap and gap + nb <= step:
+            return True
+    return False
 
 
 def check_output(name: str, x: torch.Tensor) -> None:

@@ -969,6 +969,66 @@ def test_narrow_lengths_of_a_long_cache(cuda, dtype):
                        ops.evict_cache(k, v, w, 50, l32).index)
 
 
+def test_overlap_of_interleaved_views():
+    """Views whose elements lie between each other's do not overlap; views that
+    share an element always do."""
+    import random
+
+    from minference.ops._cache import overlap
+
+    kv = t(2, 4, 10, 128)
+    assert not overlap(kv[..., :64], kv[..., 64:])
+    assert overlap(kv[..., :65], kv[..., 64:])
+    kv = t(3, 2, 4, 10, 64)
+    assert not overlap(kv[:, 0], kv[:, 1])
+    assert not overlap(kv[:, 0], kv[1, 1])
+    assert overlap(kv[:, 0, :, 2:], kv[:, 0, :, :3])
+    assert not overlap(kv[:, 1, :, 3:], kv[:, 1, :, :3])
+    flat = t(4, 10, 3, 8, 64)  # [B, S, 3, H, D]: a packed projection
+    q, k, v = (flat[:, :, i].transpose(1, 2) for i in range(3))
+    assert not overlap(q, k) and not overlap(v, q) and overlap(q, q[:, 3:])
+    rng = random.Random(1)
+    apart = 0
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            size = [rng.randint(1, 4) for _ in range(3)]
+            stride = [rng.choice([1, 2, 3, 4, 6, 8, 12, 24]) for _ in range(3)]
+            base = torch.arange(400)
+            views.append(base.as_strided(size, stride, rng.randint(0, 60)))
+        sets = [set(x.flatten().tolist()) for x in views]
+        base = torch.arange(400)
+        a, b = (base.as_strided(x.shape, x.stride(), x.storage_offset()) for x in views)
+        if sets[0] & sets[1]:
+            assert overlap(a, b)
+        apart += not overlap(a, b)
+    assert apart > 1000
+
+
+@pytest.mark.gpu
+def test_interleaved_buffers(cuda):
+    """Keys beside values in one buffer, and an output among a packed projection."""
+    from minference import ops
+
+    g = torch.Generator().manual_seed(38)
+    for shape in ((2, 3, 300, 2, 64), (2, 2, 3, 300, 64)):  # [B,H,S,2,D], [B,2,H,S,D]
+        d = shape.index(2, 1)
+        kv = torch.randn(shape, generator=g).to(BF).cuda()
+        out = torch.full([100 if n == 300 else n for n in shape], 7.0, dtype=BF, device="cuda")
+        w = torch.rand(2, 3, 300, generator=g).cuda()
+        k, v = kv.unbind(d)
+        res = ops.evict_cache(k, v, w, 100, sink=4, recent=8,
+                              out=(*out.unbind(d), torch.empty(2, 3, 100, device="cuda")))
+        check_evicted(res, k, v, w, 100, None, 4, 8)
+    packed = torch.randn(2, 5, 4, 6, 64, generator=g).to(BF).cuda()  # [B, S, q k v o, H, D]
+    q, k, v, o = (x.transpose(1, 2) for x in packed.clone().unbind(2))
+    ops.shared_prefix_attention(q, None, None, k, v, out=o)
+    ref, tol, _, _ = ref_attention(q, None, None, k, v)
+    assert ((o.double() - ref).abs() <= tol).all()
+    for x, y in zip((q, k, v), packed.unbind(2)):
+        assert torch.equal(x, y.transpose(1, 2))
+
+
 def test_weights_refuse(no_device_check):
     from minference import ops
 
