@@ -132,6 +132,13 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+// A block that gave up a wait may have asked for copies or products just before.
+// They take microseconds; a millisecond goes by before it gives up the memory
+// that they write to.
+__device__ __noinline__ void let_land() {
+  for (int i = 0; i < 64; ++i) __nanosleep(20000);
+}
+
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

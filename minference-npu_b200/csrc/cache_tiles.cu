@@ -465,6 +465,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) let_land();
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);

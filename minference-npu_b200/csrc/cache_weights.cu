@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) let_land();
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 256);
@@ -608,6 +609,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) let_land();
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 256);
