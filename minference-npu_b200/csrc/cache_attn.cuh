@@ -145,6 +145,13 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
+// |scale|, but not 0: a hidden score of -inf has to stay -inf when it is scaled.
+// A scale that is NaN stays one.
+__device__ __forceinline__ float score_scale(float scale) {
+  const float a = fabsf(scale);
+  return a < 1e-30f ? 1e-30f : a;
+}
+
 // A row's reference m after scores whose maximum is t.  A NaN among them
 // (t is NaN) leaves it finite: the row's sums carry the NaN, and -inf keeps
 // meaning that nothing has been seen.

@@ -285,8 +285,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const int none0 = __reduce_max_sync(0xffffffffu, live ? lim0 : 0);
     const int none1 = __reduce_max_sync(0xffffffffu, live ? lim1 : 0);
     if (!live) lim0 = none0, lim1 = none1;
-    // not 0: a hidden score of -inf has to stay -inf when it is scaled
-    const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const float sc = score_scale(p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };

@@ -266,8 +266,7 @@ __global__ void __launch_bounds__(kScanThreads, 2)
     const int lim = p.causal ? len - (p.Sq - 1 - tok) : len;  // keys that the row sees
     const int wlo = __reduce_min_sync(0xffffffffu, live ? lim : 0x7fffffff);
     const int whi = __reduce_max_sync(0xffffffffu, live ? lim : 0);
-    // not 0: a hidden score of -inf has to stay -inf when it is scaled
-    const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const float sc = score_scale(p.scale_log2);
     const uint32_t tcol = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
     float m = -INFINITY, l = 0.f;
     bool ok = true;

@@ -245,6 +245,17 @@ def test_attention_scales(cuda, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 70, 200])
+def test_a_scale_that_is_nan_gives_nan(cuda, Sq):
+    from minference import ops
+
+    q, kp, vp, k, v = make((2, 4, 2, Sq, 1, 300, 250, 64, BF, "bhsd"), 39)
+    out, lse = ops.shared_prefix_attention(q, kp, vp, k, v, scale=math.nan, return_lse=True)
+    assert out.isnan().all() and lse.isnan().all()
+    assert ops.accumulate_attention_weights(q, k, scale=math.nan).isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("Sq", [1, 5, 70])
 def test_attention_rising_scores(cuda, Sq, dtype):
