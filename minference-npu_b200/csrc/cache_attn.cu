@@ -19,9 +19,10 @@ namespace mib200 {
 //   O^T (D x 8 rows) += V^T P^T        P^T is S^T's registers rounded to the
 //                                      inputs' type and transposed in place
 // Rows of a ring stage are padded by 16 bytes, which makes the ldmatrix rows
-// of 128, 192 and 256 bytes fall into distinct banks.  Keys past the end of
-// the range are filled with zeros instead of being read, so whatever a cache
-// holds past its length cannot reach O through 0 * V.
+// of 128, 192 and 256 bytes fall into distinct banks.  P is rounded because both
+// operands of a product have one type; the row sums are taken before.  Keys past
+// the end of the range are filled with zeros instead of being read, so whatever a
+// cache holds past its length cannot reach O through 0 * V.
 // Measured: two caches of 65536 and 49152 keys, 32 heads of 96, 219 us
 // (6.4 TB/s); 201 MB of 1024-key caches 39 us.  With the rows as the M side and
 // two blocks of 100 KB an SM the first took 257 us.

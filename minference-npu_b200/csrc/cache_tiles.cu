@@ -13,12 +13,17 @@
 // reference moves only when a block's sum of P says so; O leaves unnormalised
 // (or finished, when the item has the whole row).
 //
-// Bound by the keys' bytes at few rows and by the softmax (issue and MUFU, 1 us
-// a 64-key block and item) at many.  Measured: 128 rows of 8 heads of 128 over
-// 65536 keys 50 us (5.4 TB/s); 4096 rows over 16384 keys and 384 own 264 us
-// (1.06 PFLOP/s); with a running maximum in every block 285.  Eight softmax
-// warps on alternate blocks were slower (D = 64 235 -> 274 us), and so were
-// exponentials on the FMA pipe (every eighth pair 267, every fourth 290).
+// P is rounded to the inputs' type, which V has (both operands of a product
+// have one type); the row sums are taken before.  Against 64 bits a bf16 output
+// is 2.2e-3 off (2-norm), where its own rounding alone makes 1.7e-3.
+//
+// Bound by the keys' bytes at few rows and by the latency of the softmax's chain
+// (1 us a 64-key block and item; tensor and MUFU pipes both at 58 %) at many.
+// Measured: 128 rows of 8 heads of 128 over 65536 keys 50 us (5.4 TB/s); 4096
+// rows over 16384 keys and 384 own 264 us for a call alone on the GPU (1.06
+// PFLOP/s), 289 among others; with a running maximum in every block 285 alone.
+// Eight softmax warps on alternate blocks were slower (D = 64 235 -> 274 us), and
+// so were exponentials on the FMA pipe (every eighth pair 267, every fourth 290).
 #include <cstring>
 
 #include "cache_attn.cuh"
